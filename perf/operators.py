@@ -1,0 +1,330 @@
+"""The microscaled 4-bit row store: writing rows into it, reading them back, scoring queries against it, the k best rows.
+
+A store keeps rows in the OCP microscaling format MXFP4: blocks of 32 elements share a power of two (E8M0), elements are
+E2M1.  32 rows form a panel: codes [k-steps of 64][half][row][16 bytes], scale bytes [groups of 4 k-steps][half][row][4],
+then 32 fp32 row norms.  Queries are rounded the same way, to E4M3 (`query_bits` 8) or E2M1 (4), and every score is the
+distance between the two rounded vectors: IP 1 - q.x, L2 |q|^2 + |x|^2 - 2 q.x, Cosine 1 - q.x / (|q| |x|).
+"""
+import math
+
+import torch
+
+own = False
+
+F32, BF16, F16 = "float32", "bfloat16", "float16"
+L2, IP, COSINE = 0, 1, 2   # VecSimMetric_L2, _IP, _Cosine
+
+
+def listed():
+    return [
+        # one document's embedding arrives while the service runs: latency of a write and of the read-back that checks it
+        {"name": "write-1x768-f32", "op": "write", "m": 1, "n": 4096, "dim": 768, "dtype": F32, "pad": 0},
+        # a re-embedding batch overwrites scattered rows; the batch is padded to a fixed length with slot -1
+        {"name": "write-4097x1000-f16", "op": "write", "m": 4097, "n": 20011, "dim": 1000, "dtype": F16, "pad": 97},
+        # bulk ingest of an embedding model's bf16 output
+        {"name": "write-1Mx768-bf16", "op": "write", "m": 1000003, "n": 1000003, "dim": 768, "dtype": BF16, "pad": 0},
+        # fetching stored vectors of a result page, and of a training set sampled from the store
+        {"name": "read-100x128-f32", "op": "read", "m": 100, "n": 100000, "dim": 128, "dtype": F32, "pad": 3},
+        {"name": "read-700Kx1024-bf16", "op": "read", "m": 700001, "n": 1000000, "dim": 1024, "dtype": BF16, "pad": 0},
+        # every score of one query (a batch iterator's first step), of a small batch, of a wide one
+        {"name": "scores-1x100Kx128-L2", "op": "scores", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 8},
+        {"name": "scores-33x200Kx1000-IP-4bit", "op": "scores", "nq": 33, "n": 200003, "dim": 1000, "dtype": F16, "metric": IP, "bits": 4},
+        {"name": "scores-256x1Mx1024-cos", "op": "scores", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 8},
+        # the Flat index's workloads: one query on a small table, the batch of 64, a wide batch with many neighbours, odd sizes
+        {"name": "topk-1x100Kx128-L2", "op": "topk", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 8, "k": 10},
+        {"name": "topk-64x4Mx768-L2", "op": "topk", "nq": 64, "n": 4000000, "dim": 768, "dtype": F32, "metric": L2, "bits": 8, "k": 10},
+        {"name": "topk-256x1Mx1024-cos", "op": "topk", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 8, "k": 100},
+        {"name": "topk-7x300Kx300-IP-4bit", "op": "topk", "nq": 7, "n": 300007, "dim": 300, "dtype": F16, "metric": IP, "bits": 4, "k": 1000},
+    ]
+
+
+def draw(rng):
+    def spread(lo, hi):
+        v = int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+        return max(lo, min(hi, v | 1 if rng.random() < 0.5 else v))
+
+    op = rng.choice(["write", "read", "scores", "topk"])
+    case = {"op": op, "dim": spread(1, 4096), "dtype": rng.choice([F32, BF16, F16])}
+    if op in ("write", "read"):
+        case["m"] = min(spread(1, 1000003), 768000000 // case["dim"])
+        case["n"] = case["m"] + (rng.randrange(0, case["m"] + 33) if case["m"] < 300000 else 0)
+        case["pad"] = rng.randrange(0, min(64, case["m"]))
+    else:
+        case["nq"] = spread(1, 256)
+        most = min(4000000, 3000000000 // case["dim"], 256000000 // case["nq"], 190000000000 // (case["dim"] * case["nq"]))
+        case["n"] = spread(1, max(1, most))
+        case["metric"] = rng.choice([L2, IP, COSINE])
+        case["bits"] = rng.choice([4, 8])
+        if op == "topk":
+            case["k"] = spread(1, 1000)
+    return case
+
+
+# ---- the plain form -----------------------------------------------------------------------------------------------------------
+def _pow2(e):
+    """2^e for whole e in [-126, 127], exactly"""
+    return ((e + 127) << 23).view(torch.float32)
+
+
+def _shared(x, emax):
+    """blocks of 32 along the last axis of fp32 x (padded with zeros to a multiple of 64): blocks, shared exponents, bad blocks"""
+    dim = x.shape[1]
+    x = torch.nn.functional.pad(x, (0, -dim % 64)).view(x.shape[0], -1, 32)
+    top = x.abs().amax(2)
+    bad = ~torch.isfinite(top)
+    _, e = torch.frexp(torch.where(bad, 0.0, top))
+    e = torch.where(top == 0, -127, (e - 1 - emax).clamp(-127, 127)).to(torch.int32)
+    return x, e, bad
+
+
+def _fp4_codes(x):
+    """rows of fp32 -> 4-bit codes [m, blocks, 32], scale bytes [m, blocks], norms of the rounded rows"""
+    x, e, bad = _shared(x, 2)
+    mag = x.abs() * _pow2(-e).unsqueeze(2)
+    code = ((mag > 0.25).to(torch.uint8) + (mag >= 0.75) + (mag > 1.25) + (mag >= 1.75) + (mag > 2.5) + (mag >= 3.5) + (mag > 5.0))
+    code = torch.where(bad.unsqueeze(2), 0, code | (torch.signbit(x).to(torch.uint8) << 3))
+    scale = torch.where(bad, 255, e + 127).to(torch.uint8)
+    norm = _fp4_values(code, scale, torch.float64).square().sum((1, 2)).sqrt()
+    return code, scale, norm.to(torch.float32)
+
+
+def _fp4_values(code, scale, dtype=torch.float32):
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0], dtype=dtype, device=code.device)
+    # 2^(byte - 127) as the product of two halves: the smallest are below fp32's normal numbers
+    e = scale.to(torch.int32) - 127
+    half = torch.div(e, 2, rounding_mode="floor")
+    power = torch.where(scale == 255, float("nan"), _pow2(half).to(dtype) * _pow2((e - half).clamp(-126, 127)).to(dtype))
+    return table[code.to(torch.int32)] * power.unsqueeze(-1)
+
+
+def _fp8_values(x, dtype):
+    x, e, bad = _shared(x, 8)
+    v = x * _pow2(-e).unsqueeze(2)
+    _, f = torch.frexp(v)
+    step = _pow2((f - 1).clamp(min=-6).to(torch.int32) - 3)
+    v = (torch.round(v / step) * step).clamp(-448.0, 448.0).to(dtype)
+    half = torch.div(e, 2, rounding_mode="floor")
+    power = torch.where(bad, float("nan"), _pow2(half).to(dtype) * _pow2(e - half).to(dtype))
+    return (v * power.unsqueeze(2)).flatten(1)
+
+
+def _sizes(dim):
+    steps = (dim + 63) // 64
+    return steps, (steps + 3) // 4
+
+
+def _views(table, dim):
+    steps, groups = _sizes(dim)
+    at = steps * 1024
+    codes = table[:, :at].view(-1, steps, 2, 32, 16)
+    scales = table[:, at:at + groups * 256].view(-1, groups, 2, 32, 4)
+    norms = table[:, at + groups * 256:].view(torch.float32)
+    return codes, scales, norms
+
+
+def _put(table, slots, x):
+    """writes the rows of fp32 x into `slots` of the panels"""
+    dim = x.shape[1]
+    steps, groups = _sizes(dim)
+    codes, scales, norms = _views(table, dim)
+    code, scale, norm = _fp4_codes(x)
+    packed = (code[..., 0::2] | (code[..., 1::2] << 4)).view(-1, steps, 2, 16)
+    scale = torch.nn.functional.pad(scale.view(-1, steps, 2), (0, 0, 0, groups * 4 - steps)).view(-1, groups, 4, 2).transpose(2, 3)
+    p, r = slots // 32, slots % 32
+    codes[p, :, :, r] = packed
+    scales[p, :, :, r] = scale
+    norms[p, r] = norm
+
+
+def _get(table, dim, slots, dtype):
+    """the rows in `slots` (None: every row of every panel) as values of `dtype`, with their padding to a multiple of 64"""
+    steps, groups = _sizes(dim)
+    codes, scales, norms = _views(table, dim)
+    if slots is None:
+        packed, scale, norm = codes.permute(0, 3, 1, 2, 4), scales.permute(0, 3, 1, 4, 2), norms.flatten()
+    else:
+        p, r = slots // 32, slots % 32
+        packed, scale, norm = codes[p, :, :, r], scales[p, :, :, r].transpose(2, 3), norms[p, r]
+    packed = packed.reshape(-1, steps * 2, 16)
+    scale = scale.reshape(-1, groups * 8)[:, :steps * 2]
+    code = torch.stack((packed & 15, packed >> 4), 3).flatten(2)
+    return _fp4_values(code, scale, dtype).flatten(1), norm
+
+
+def _distances(table, n, queries, metric, bits, dtype):
+    dim = queries.shape[1]
+    q = queries.to(torch.float32)
+    q = _fp8_values(q, dtype) if bits == 8 else _fp4_values(*_fp4_codes(q)[:2], dtype).flatten(1)
+    x, norm = _get(table, dim, None, dtype)
+    x = x[:n]
+    dot = q @ x.T
+    if metric == IP:
+        return 1 - dot
+    # the norms the store keeps are rounded to fp32; where 64 bits are asked for they are taken from the values
+    norm = norm[:n] if dtype == torch.float32 else x.square().sum(1).sqrt()
+    qq = q.square().sum(1, keepdim=True)
+    if metric == L2:
+        return qq + norm.square() - 2 * dot
+    return 1 - dot / (qq.sqrt() * norm)
+
+
+# ---- what a user has in hand ----------------------------------------------------------------------------------------------------
+def _vectors(gen, m, dim, device):
+    """embedding-like rows: directions of unequal weight, lengths around one"""
+    weight = torch.exp(0.5 * torch.randn(dim, generator=gen, device=device))
+    x = torch.randn(m, dim, generator=gen, device=device) * weight
+    return x * ((0.5 + torch.rand(m, 1, generator=gen, device=device)) / (weight.norm() + 1e-6))
+
+
+def _store(gen, n, dim, device):
+    steps, groups = _sizes(dim)
+    table = torch.zeros((n + 31) // 32, steps * 1024 + groups * 256 + 128, dtype=torch.uint8, device=device)
+    piece = max(32, (1 << 27) // dim)
+    for a in range(0, n, piece):
+        m = min(piece, n - a)
+        _put(table, torch.arange(a, a + m, device=device), _vectors(gen, m, dim, device))
+    return table
+
+
+def prepare(case, seed):
+    device = "cuda"
+    gen = torch.Generator(device).manual_seed(seed)
+    dim, n = case["dim"], case["n"]
+    dtype = getattr(torch, case["dtype"])
+    state = dict(case, table=None)
+    if case["op"] in ("write", "read"):
+        m, pad = case["m"], case["pad"]
+        slots = torch.arange(n, device=device) if m == n else torch.randperm(n, generator=gen, device=device)[:m]
+        if pad:
+            slots[m - pad:] = -1
+        state["slots"] = slots
+    if case["op"] == "write":
+        steps, groups = _sizes(dim)
+        state["table"] = torch.zeros((n + 31) // 32, steps * 1024 + groups * 256 + 128, dtype=torch.uint8, device=device)
+        state["x"] = _vectors(gen, m, dim, device).to(dtype)
+        return state
+    state["table"] = _store(gen, n, dim, device)
+    if case["op"] in ("scores", "topk"):
+        # half the queries look for something near a stored row
+        nq = case["nq"]
+        near = torch.randint(0, n, (nq,), generator=gen, device=device)
+        base, _ = _get(state["table"], dim, near, torch.float32)
+        q = _vectors(gen, nq, dim, device)
+        q[::2] = base[::2, :dim] + 0.3 * q[::2]
+        state["q"] = q.to(dtype)
+    return state
+
+
+def run(state):
+    op, table, dim = state["op"], state["table"], state["dim"]
+    dtype = getattr(torch, state["dtype"])
+    if own:
+        from vectorsimilarity_amd import mx4
+        if op == "write":
+            mx4.write(table, state["x"], state["slots"])
+            return mx4.read(table, dim, state["slots"], dtype)
+        if op == "read":
+            return mx4.read(table, dim, state["slots"], dtype)
+        if op == "scores":
+            return mx4.scores(table, state["n"], state["q"], state["metric"], state["bits"])
+        return mx4.topk(table, state["n"], state["q"], state["k"], state["metric"], state["bits"])
+    if op in ("write", "read"):
+        slots = state["slots"]
+        kept = (slots >= 0).unsqueeze(1)
+        if op == "write":
+            _put(table, slots[kept[:, 0]], state["x"][kept[:, 0]].to(torch.float32))
+        rows, _ = _get(table, dim, slots.clamp(min=0), torch.float32)
+        return torch.where(kept, rows[:, :dim], 0.0).to(dtype)
+    if op == "scores":
+        return _distances(table, state["n"], state["q"], state["metric"], state["bits"], torch.float32)
+    # the order of the k best is a matter of the last bits, and of the lower row among equals
+    score = _distances(table, state["n"], state["q"], state["metric"], state["bits"], torch.float64).to(torch.float32)
+    k = min(state["k"], state["n"])
+    score, ids = torch.sort(score, dim=1, stable=True)
+    pad = (0, state["k"] - k)
+    return torch.nn.functional.pad(ids[:, :k], pad, value=-1), torch.nn.functional.pad(score[:, :k], pad, value=-1.0)
+
+
+def work(case):
+    dim, size = case["dim"], 4 if case["dtype"] == F32 else 2
+    blocks = (dim + 31) // 32
+    row = (dim + 1) // 2 + blocks + 4     # codes, scales, norm
+    if case["op"] in ("write", "read"):
+        m = case["m"]
+        rows = m * (row + dim * size) + m * 8
+        return {"bytes": rows * (2 if case["op"] == "write" else 1), "flops": m * dim * (6 if case["op"] == "write" else 2)}
+    nq, n = case["nq"], case["n"]
+    out = nq * n * 4 if case["op"] == "scores" else nq * case["k"] * 12
+    return {"bytes": n * row + nq * dim * size + out, "flops": 2 * nq * n * dim}
+
+
+# ---- the definition in 64 bits --------------------------------------------------------------------------------------------------
+def _round_to(v, lowest, digits, largest):
+    """v (float64) to the nearest number with `digits` bits after the leading one, exponents from `lowest` up, ties to even"""
+    exponent = torch.floor(torch.log2(v.abs().clamp(min=2.0 ** lowest)))
+    # log2 may be off by one next to a power of two
+    exponent = torch.where(v.abs() < torch.exp2(exponent), exponent - 1, exponent)
+    exponent = torch.where(v.abs() >= torch.exp2(exponent + 1), exponent + 1, exponent).clamp(min=lowest)
+    unit = torch.exp2(exponent - digits)
+    return (torch.round(v / unit) * unit).clamp(-largest, largest)
+
+
+def _micro(x, bits):
+    """the microscaled rounding of float64 rows, as values"""
+    lowest, digits, largest, emax = (0, 1, 6.0, 2) if bits == 4 else (-6, 3, 448.0, 8)
+    out = torch.empty_like(x)
+    for a in range(0, x.shape[1], 32):
+        block = x[:, a:a + 32]
+        top = block.abs().amax(1, keepdim=True)
+        e = torch.floor(torch.log2(top.clamp(min=2.0 ** -149)))
+        e = torch.where(top < torch.exp2(e), e - 1, torch.where(top >= torch.exp2(e + 1), e + 1, e))
+        e = (e - emax).clamp(-127, 127)
+        value = _round_to(block / torch.exp2(e), lowest, digits, largest) * torch.exp2(e)
+        out[:, a:a + 32] = torch.where(torch.isfinite(top), value, float("nan"))
+    return out
+
+
+def _decode64(table, dim, a, b):
+    """rows [a, b) of the store (a a multiple of 32), one block at a time"""
+    out = torch.empty(b - a, dim, dtype=torch.float64, device=table.device)
+    codes, scales, _ = _views(table[a // 32:(b + 31) // 32], dim)
+    for block in range((dim + 31) // 32):
+        step, half = block // 2, block % 2
+        byte = codes[:, step, half].reshape(-1, 16)[:b - a].to(torch.int64)
+        nib = torch.stack((byte % 16, byte // 16), 2).flatten(1)[:, :dim - block * 32]
+        exponent, odd = (nib % 8) // 2, nib % 2
+        mag = torch.where(exponent == 0, 0.5 * odd, torch.exp2(exponent.to(torch.float64) - 1) * (1 + 0.5 * odd))
+        scale = scales[:, step // 4, half, :, step % 4].reshape(-1)[:b - a].to(torch.float64)
+        value = torch.where(nib >= 8, -mag, mag) * torch.exp2(scale - 127).unsqueeze(1)
+        out[:, block * 32:block * 32 + 32] = torch.where((scale == 255).unsqueeze(1), float("nan"), value)
+    return out
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    table, dim, n = state["table"], state["dim"], state["n"]
+    if case["op"] in ("write", "read"):
+        slots = state["slots"]
+        if case["op"] == "write":
+            rows = _micro(state["x"].to(torch.float64), 4)
+        else:
+            rows = torch.cat([_decode64(table, dim, a, min(n, a + 65536)) for a in range(0, n, 65536)])[slots.clamp(min=0)]
+        return torch.where((slots >= 0).unsqueeze(1), rows, 0.0)
+    q = _micro(state["q"].to(torch.float64), case["bits"])
+    parts = []
+    for a in range(0, n, 65536):
+        x = _decode64(table, dim, a, min(n, a + 65536))
+        dot = (x @ q.T).T
+        if case["metric"] == IP:
+            parts.append(1 - dot)
+        elif case["metric"] == COSINE:
+            parts.append(1 - dot / torch.outer((q * q).sum(1).sqrt(), (x * x).sum(1).sqrt()))
+        else:
+            parts.append((q * q).sum(1, keepdim=True) + (x * x).sum(1) - 2 * dot)
+    score = torch.cat(parts, 1)
+    if case["op"] == "scores":
+        return score
+    order = torch.sort(score.to(torch.float32), dim=1, stable=True).indices[:, :case["k"]]
+    best = torch.gather(score, 1, order)
+    pad = (0, case["k"] - order.shape[1])
+    return torch.nn.functional.pad(order, pad, value=-1), torch.nn.functional.pad(best, pad, value=-1.0)
