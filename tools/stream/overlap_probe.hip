@@ -5,7 +5,7 @@
 //  1. hipExtStreamCreateWithCUMask: where do workgroups of a masked stream land (XCC, SE, CU from the hardware id registers)?
 //  2. How fast does a streaming read run on 256 / 248 / 240 / 224 CUs (a scan that leaves CUs to the small kernels)?
 //  3. A second stream reading other memory on the reserved CUs at the same time: what does each side get?
-//  4. Tile dealing: static grid-stride against a shared counter (vector atomic by one lane, and s_atomic_add), alone and with
+//  4. Tile dealing: static grid-stride against a shared counter (a vector atomic by one lane), alone and with
 //     an interfering kernel that occupies every CU for part of the run (late / slowed workgroups -> a tail for the static deal).
 #include <hip/hip_runtime.h>
 #include <cstdio>
@@ -32,8 +32,7 @@ __global__ void k_where(uint32_t *out) {
     while (__builtin_readcyclecounter() - t0 < 200000) {}
 }
 
-// MODE 0: static grid-stride over tiles; 1: shared counter, vector atomic by lane 0 of wave 0 + LDS broadcast, one tile ahead;
-// 2: the same through s_atomic_add (scalar cache path, lgkmcnt: no VM counter involved)
+// MODE 0: static grid-stride over tiles; 1: shared counter, vector atomic by lane 0 of wave 0 + LDS broadcast, one tile ahead
 template <int MODE>
 __global__ __launch_bounds__(256) void k_tiles(const uint4 *p, uint32_t n_tiles, uint32_t *counter, uint32_t *sink, uint32_t *per_wg) {
     __shared__ uint32_t next_s[2];
@@ -42,12 +41,7 @@ __global__ __launch_bounds__(256) void k_tiles(const uint4 *p, uint32_t n_tiles,
     if (MODE == 0) tile = blockIdx.x;
     else {
         if (threadIdx.x == 0) {
-            if (MODE == 1) next_s[0] = atomicAdd(counter, 1u);
-            else {
-                uint32_t v;
-                asm volatile("s_atomic_add %0, %1, %2 glc\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(counter), "s"(1u) : "memory");
-                next_s[0] = v;
-            }
+            next_s[0] = atomicAdd(counter, 1u);
         }
         __syncthreads();
         tile = next_s[0];
@@ -55,8 +49,7 @@ __global__ __launch_bounds__(256) void k_tiles(const uint4 *p, uint32_t n_tiles,
     uint32_t par = 0;
     while (tile < n_tiles) {
         if (MODE != 0 && threadIdx.x == 0) {   // fetch the tile after this one while this one streams
-            if (MODE == 1) nxt = atomicAdd(counter, 1u);
-            else asm volatile("s_atomic_add %0, %1, %2 glc" : "=s"(nxt) : "s"(counter), "s"(1u) : "memory");
+            nxt = atomicAdd(counter, 1u);
         }
         const uint4 *q = p + (size_t)tile * TILE_U4 + threadIdx.x;
         uint4 v[12];
@@ -71,7 +64,6 @@ __global__ __launch_bounds__(256) void k_tiles(const uint4 *p, uint32_t n_tiles,
         if (MODE == 0) tile += gridDim.x;
         else {
             if (threadIdx.x == 0) {
-                if (MODE == 2) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 next_s[par ^ 1] = nxt;
             }
             __syncthreads();
@@ -229,8 +221,7 @@ int main(int argc, char **argv) {
             if (interfere) hipLaunchKernelGGL(k_busy, dim3(cu * 2), dim3(256), 0, s2, (uint64_t)30000 /* x 100 MHz counter ~ 0.3 ms */, sink);
             CHECK(hipEventRecord(e0, s_all));
             if (mode == 0) hipLaunchKernelGGL((k_tiles<0>), dim3(grid), dim3(256), 0, s_all, d, n_tiles, counter, sink, per_wg);
-            else if (mode == 1) hipLaunchKernelGGL((k_tiles<1>), dim3(grid), dim3(256), 0, s_all, d, n_tiles, counter, sink, per_wg);
-            else hipLaunchKernelGGL((k_tiles<2>), dim3(grid), dim3(256), 0, s_all, d, n_tiles, counter, sink, per_wg);
+            else hipLaunchKernelGGL((k_tiles<1>), dim3(grid), dim3(256), 0, s_all, d, n_tiles, counter, sink, per_wg);
             CHECK(hipEventRecord(e1, s_all));
             hipError_t e = hipDeviceSynchronize();
             if (e != hipSuccess) { printf("%s: kernel failed: %s\n", tag, hipGetErrorString(e)); return; }
@@ -248,9 +239,7 @@ int main(int argc, char **argv) {
     };
     run_mode(0, cu * 2, false, "static deal, alone");
     run_mode(1, cu * 2, false, "counter (vector atomic), alone");
-    if (argc > 1 && !strcmp(argv[1], "satomic")) run_mode(2, cu * 2, false, "counter (s_atomic_add), alone");
     run_mode(0, cu * 2, true, "static deal, busy kernel holding the CUs");
     run_mode(1, cu * 2, true, "counter (vector atomic), busy kernel");
-    if (argc > 1 && !strcmp(argv[1], "satomic")) run_mode(2, cu * 2, true, "counter (s_atomic_add), busy kernel");
     return 0;
 }
