@@ -2,7 +2,7 @@
 
 A store keeps rows in the OCP microscaling format MXFP4: blocks of 32 elements share a power of two (E8M0), elements are
 E2M1.  32 rows form a panel: codes [k-steps of 64][half][row][16 bytes], scale bytes [groups of 4 k-steps][half][row][4],
-then 32 fp32 row norms.  Queries are rounded the same way, to E4M3 (`query_bits` 8) or E2M1 (4), and every score is the
+then 32 fp32 row norms.  Queries are rounded the same way, to MXFP6's E2M3 (`query_bits` 6) or to E2M1 (4), and every score is the
 distance between the two rounded vectors: IP 1 - q.x, L2 |q|^2 + |x|^2 - 2 q.x, Cosine 1 - q.x / (|q| |x|).
 """
 import math
@@ -27,13 +27,13 @@ def listed():
         {"name": "read-100x128-f32", "op": "read", "m": 100, "n": 100000, "dim": 128, "dtype": F32, "pad": 3},
         {"name": "read-700Kx1024-bf16", "op": "read", "m": 700001, "n": 1000000, "dim": 1024, "dtype": BF16, "pad": 0},
         # every score of one query (a batch iterator's first step), of a small batch, of a wide one
-        {"name": "scores-1x100Kx128-L2", "op": "scores", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 8},
+        {"name": "scores-1x100Kx128-L2", "op": "scores", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 6},
         {"name": "scores-33x200Kx1000-IP-4bit", "op": "scores", "nq": 33, "n": 200003, "dim": 1000, "dtype": F16, "metric": IP, "bits": 4},
-        {"name": "scores-256x1Mx1024-cos", "op": "scores", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 8},
+        {"name": "scores-256x1Mx1024-cos", "op": "scores", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 6},
         # the Flat index's workloads: one query on a small table, the batch of 64, a wide batch with many neighbours, odd sizes
-        {"name": "topk-1x100Kx128-L2", "op": "topk", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 8, "k": 10},
-        {"name": "topk-64x4Mx768-L2", "op": "topk", "nq": 64, "n": 4000000, "dim": 768, "dtype": F32, "metric": L2, "bits": 8, "k": 10},
-        {"name": "topk-256x1Mx1024-cos", "op": "topk", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 8, "k": 100},
+        {"name": "topk-1x100Kx128-L2", "op": "topk", "nq": 1, "n": 100000, "dim": 128, "dtype": F32, "metric": L2, "bits": 6, "k": 10},
+        {"name": "topk-64x4Mx768-L2", "op": "topk", "nq": 64, "n": 4000000, "dim": 768, "dtype": F32, "metric": L2, "bits": 6, "k": 10},
+        {"name": "topk-256x1Mx1024-cos", "op": "topk", "nq": 256, "n": 1000000, "dim": 1024, "dtype": BF16, "metric": COSINE, "bits": 6, "k": 100},
         {"name": "topk-7x300Kx300-IP-4bit", "op": "topk", "nq": 7, "n": 300007, "dim": 300, "dtype": F16, "metric": IP, "bits": 4, "k": 1000},
     ]
 
@@ -54,7 +54,7 @@ def draw(rng):
         most = min(4000000, 3000000000 // case["dim"], 256000000 // case["nq"], 190000000000 // (case["dim"] * case["nq"]))
         case["n"] = spread(1, max(1, most))
         case["metric"] = rng.choice([L2, IP, COSINE])
-        case["bits"] = rng.choice([4, 8])
+        case["bits"] = rng.choice([4, 6])
         if op == "topk":
             case["k"] = spread(1, 1000)
     return case
@@ -66,20 +66,20 @@ def _pow2(e):
     return ((e + 127) << 23).view(torch.float32)
 
 
-def _shared(x, emax):
+def _shared(x):
     """blocks of 32 along the last axis of fp32 x (padded with zeros to a multiple of 64): blocks, shared exponents, bad blocks"""
     dim = x.shape[1]
     x = torch.nn.functional.pad(x, (0, -dim % 64)).view(x.shape[0], -1, 32)
     top = x.abs().amax(2)
     bad = ~torch.isfinite(top)
     _, e = torch.frexp(torch.where(bad, 0.0, top))
-    e = torch.where(top == 0, -127, (e - 1 - emax).clamp(-127, 127)).to(torch.int32)
+    e = torch.where(top == 0, -127, (e - 3).clamp(-127, 127)).to(torch.int32)
     return x, e, bad
 
 
 def _fp4_codes(x):
     """rows of fp32 -> 4-bit codes [m, blocks, 32], scale bytes [m, blocks], norms of the rounded rows"""
-    x, e, bad = _shared(x, 2)
+    x, e, bad = _shared(x)
     mag = x.abs() * _pow2(-e).unsqueeze(2)
     code = ((mag > 0.25).to(torch.uint8) + (mag >= 0.75) + (mag > 1.25) + (mag >= 1.75) + (mag > 2.5) + (mag >= 3.5) + (mag > 5.0))
     code = torch.where(bad.unsqueeze(2), 0, code | (torch.signbit(x).to(torch.uint8) << 3))
@@ -97,12 +97,13 @@ def _fp4_values(code, scale, dtype=torch.float32):
     return table[code.to(torch.int32)] * power.unsqueeze(-1)
 
 
-def _fp8_values(x, dtype):
-    x, e, bad = _shared(x, 8)
+def _fp6_values(x, dtype):
+    """rows of fp32 rounded to E2M3: steps of 1/8 below 2, of 1/4 below 4, of 1/2 up to 7.5"""
+    x, e, bad = _shared(x)
     v = x * _pow2(-e).unsqueeze(2)
-    _, f = torch.frexp(v)
-    step = _pow2((f - 1).clamp(min=-6).to(torch.int32) - 3)
-    v = (torch.round(v / step) * step).clamp(-448.0, 448.0).to(dtype)
+    mag = v.abs()
+    step = torch.where(mag < 2, 0.125, torch.where(mag < 4, 0.25, 0.5))
+    v = (torch.round(v / step) * step).clamp(-7.5, 7.5).to(dtype)
     half = torch.div(e, 2, rounding_mode="floor")
     power = torch.where(bad, float("nan"), _pow2(half).to(dtype) * _pow2(e - half).to(dtype))
     return (v * power.unsqueeze(2)).flatten(1)
@@ -154,7 +155,7 @@ def _get(table, dim, slots, dtype):
 def _distances(table, n, queries, metric, bits, dtype):
     dim = queries.shape[1]
     q = queries.to(torch.float32)
-    q = _fp8_values(q, dtype) if bits == 8 else _fp4_values(*_fp4_codes(q)[:2], dtype).flatten(1)
+    q = _fp6_values(q, dtype) if bits == 6 else _fp4_values(*_fp4_codes(q)[:2], dtype).flatten(1)
     x, norm = _get(table, dim, None, dtype)
     x = x[:n]
     dot = q @ x.T
@@ -259,27 +260,27 @@ def work(case):
 
 
 # ---- the definition in 64 bits --------------------------------------------------------------------------------------------------
-def _round_to(v, lowest, digits, largest):
-    """v (float64) to the nearest number with `digits` bits after the leading one, exponents from `lowest` up, ties to even"""
-    exponent = torch.floor(torch.log2(v.abs().clamp(min=2.0 ** lowest)))
+def _round_to(v, digits, largest):
+    """v (float64) to the nearest number with `digits` bits after the leading one, exponents from 0 up, ties to even"""
+    exponent = torch.floor(torch.log2(v.abs().clamp(min=1.0)))
     # log2 may be off by one next to a power of two
     exponent = torch.where(v.abs() < torch.exp2(exponent), exponent - 1, exponent)
-    exponent = torch.where(v.abs() >= torch.exp2(exponent + 1), exponent + 1, exponent).clamp(min=lowest)
+    exponent = torch.where(v.abs() >= torch.exp2(exponent + 1), exponent + 1, exponent).clamp(min=0)
     unit = torch.exp2(exponent - digits)
     return (torch.round(v / unit) * unit).clamp(-largest, largest)
 
 
 def _micro(x, bits):
     """the microscaled rounding of float64 rows, as values"""
-    lowest, digits, largest, emax = (0, 1, 6.0, 2) if bits == 4 else (-6, 3, 448.0, 8)
+    digits, largest = (1, 6.0) if bits == 4 else (3, 7.5)
     out = torch.empty_like(x)
     for a in range(0, x.shape[1], 32):
         block = x[:, a:a + 32]
         top = block.abs().amax(1, keepdim=True)
         e = torch.floor(torch.log2(top.clamp(min=2.0 ** -149)))
         e = torch.where(top < torch.exp2(e), e - 1, torch.where(top >= torch.exp2(e + 1), e + 1, e))
-        e = (e - emax).clamp(-127, 127)
-        value = _round_to(block / torch.exp2(e), lowest, digits, largest) * torch.exp2(e)
+        e = (e - 2).clamp(-127, 127)
+        value = _round_to(block / torch.exp2(e), digits, largest) * torch.exp2(e)
         out[:, a:a + 32] = torch.where(torch.isfinite(top), value, float("nan"))
     return out
 
