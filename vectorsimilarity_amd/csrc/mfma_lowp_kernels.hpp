@@ -768,33 +768,27 @@ __global__ __launch_bounds__(NWAVES * 64, MINW) void k_mfma_filter_lowp(LowpPara
                 // Screen: survivors are rare, so one branch-free pass decides whether any lane of the wave has a value that may
                 // pass; only then does the per-value loop below run.  With g = 2 (L2) or 1 (IP) the screen evaluates
                 //     lowS = [x_sq | 1 - shift] + min (-g y_sum) + delta (-g (s f + 128 sum e)) - g delta |c'| |e|
-                // in four fused operations on pairs of rows (v_pk_fma_f32: 4 + a conversion + a compare per value, against ~18 for
-                // `bounds`) and rejects when lowS > sc_T = tau [- y_sq] + slack.  slack (per query, kernel prologue) holds what
+                // in four fused operations (6 with the conversion and the compare, against ~18 for `bounds`; single ones: packed fp32 is not
+                // used in this library) and rejects when lowS > sc_T = tau [- y_sq] + slack.  slack (per query, kernel prologue) holds what
                 // the screen leaves out of `bounds`' E with the table-wide maxima in place of the row's values: g max(delta) Wref
                 // and 192 ulp of every magnitude involved (64 for E's own term, the rest for the screen's roundings) -- the
                 // Cauchy-Schwarz term, which dominates E by orders of magnitude, stays per row.  A NaN anywhere rejects nothing.
                 bool any = false;
-                const f32x2_t x0 = {1.0f - ysq, 0.0f};   // IP: the score's constant part (ysq holds the shift)
+                const float x0 = 1.0f - ysq;   // IP: the score's constant part (ysq holds the shift)
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
                     f32x4_t mn, dl, xs, pp;
                     read_aux(mt, mn, dl, xs, pp);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const f32x2_t f = {(float)(int)acc[mt][0][2 * h], (float)(int)acc[mt][0][2 * h + 1]};
-                        const f32x2_t mn2 = {mn[2 * h], mn[2 * h + 1]}, dl2 = {dl[2 * h], dl[2 * h + 1]}, pp2 = {pp[2 * h], pp[2 * h + 1]};
-                        f32x2_t t, s1, s2, lo;
-                        // (op_sel picks the dword of a register pair each half of the result reads: the constants are broadcast)
-                        asm("v_pk_fma_f32 %0, %1, %2, %1 op_sel:[0,0,1] op_sel_hi:[0,1,1]" : "=v"(t) : "v"(sq_a), "v"(f));
-                        if (L2) {
-                            const f32x2_t x2 = {xs[2 * h], xs[2 * h + 1]};
-                            asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(s1) : "v"(dl2), "v"(t), "v"(x2));
-                        } else {
-                            asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[1,1,0]" : "=v"(s1) : "v"(dl2), "v"(t), "v"(x0));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float f = (float)(int)acc[mt][0][2 * h + e];
+                            const float t = __fmaf_rn(sq_a[0], f, sq_a[1]);
+                            const float s1 = __fmaf_rn(dl[2 * h + e], t, L2 ? xs[2 * h + e] : x0);
+                            const float s2 = __fmaf_rn(mn[2 * h + e], sq_b[0], s1);
+                            any |= !(__fmaf_rn(pp[2 * h + e], sq_b[1], s2) > sq_T);
                         }
-                        asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[1,0,1]" : "=v"(s2) : "v"(mn2), "v"(sq_b), "v"(s1));
-                        asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,1,0] op_sel_hi:[1,1,1]" : "=v"(lo) : "v"(pp2), "v"(sq_b), "v"(s2));
-                        any |= !(lo[0] > sq_T) | !(lo[1] > sq_T);
                     }
                 }
                 if (!__any(any)) return;
@@ -984,7 +978,7 @@ static __global__ __launch_bounds__(256) void k_row_norms_h16(const char *rows, 
 // SQ8: {min, delta, sum_squares, delta |c - 128|_2} of every row, taken out of the (unaligned) metadata behind the codes
 // (sum_squares only exists in L2 blobs).  Layout: per group of 64 rows four arrays of 64 floats (1 KiB, fetched by ONE
 // LDS-DMA piece of the filter like 16-byte records would be), so that a lane's ds_read_b128 returns the same field of its
-// four rows -- operands of v_pk_fma_f32 as they land.  `first` = the in-slab index of rows[0], `out` = the slab's aux base.
+// four rows as they land.  `first` = the in-slab index of rows[0], `out` = the slab's aux base.
 // tmax: {max delta, max |min|, max sum_squares} over every row ever stored (float bits; all values >= 0, so unsigned
 // order = float order and a NaN wins): the filter's screen takes its table-wide slack terms from them.
 static __global__ __launch_bounds__(256) void k_row_aux_sq8(const char *rows, uint32_t row_stride, uint32_t dim, uint32_t n,
