@@ -132,6 +132,43 @@ int vsgpu_table_set_sq8_mean_sum_squares(vsgpu_table *t, float mean_sum_squares)
  * (k_row_aux_sq8), so the call is accepted, kept with the table and has no effect on any result or kernel. */
 int vsgpu_table_set_sq8_block_bounds(vsgpu_table *t, const float bounds[8]);
 
+/* ---- MXFP4 row stores: rows rounded to 4 bits as they are written, read back, scored, the k best ----
+ * No counterpart in the reference, whose quantised rows (SQ8 above) are 8-bit codes with one FP32 range per row.  The format is the
+ * OCP microscaling specification's MXFP4: blocks of 32 elements share a power of two, E = clamp(floor(log2 max|x|) - 2, -127, 125),
+ * stored as the byte E + 127; elements are E2M1 codes of x 2^-E, rounded to nearest even, saturating at 6.  A block that holds an
+ * infinity or a NaN gets scale byte 255 and is NaN as a whole.  Queries are rounded the same way, to E2M1 (bits = 4) or to MXFP6's
+ * E2M3 (bits = 6, saturating at 7.5).  Scores are the kernel metrics of the ROUNDED vectors: IP 1 - q.x, L2 |q|^2 + |x|^2 - 2 q.x,
+ * Cosine 1 - q.x / (|q| |x|) (nothing is normalised before it is rounded; a zero vector scores NaN, as in int8 Cosine).
+ *
+ * These entries work on DEVICE memory of `device` and enqueue on `stream` (a hipStream_t, 0: the default one), which may be
+ * captured into a graph: they allocate nothing, wait for nothing and keep nothing.  The caller keeps writers and readers of one
+ * table in order, and gives calls that may run at the same time workspaces of their own.  The calling thread's device is unchanged.
+ *
+ * A table of capacity rows is ceil(capacity / 32) panels of vsgpu_mx4_panel_bytes(dim) bytes, 16-byte aligned; a panel holds 32
+ * rows: codes [ceil(dim / 64)][half][row][16 bytes] (block 2 step + half, element j in byte j / 2, low nibble first), scale bytes
+ * [ceil(dim / 256)][half][row][4] (byte i: step 4 group + i), row norms [32] fp32.  Zero bytes are zero rows. */
+size_t vsgpu_mx4_panel_bytes(size_t dim);   /* 0: dim is not in 1 .. 65536 */
+/* m vectors (VSGPU_F32, _F16 or _BF16; `stride` bytes apart) into slots[0 .. m) (device integers of slot_bytes = 4 or 8 bytes), or
+ * into rows first .. first + m - 1 when slots is NULL.  A negative slot is padding: its vector is skipped; so is one whose slot is
+ * not below capacity.  Of several vectors with one slot the last is kept.  Rows that no slot names stay as they are. */
+int vsgpu_mx4_write(int device, void *stream, void *table, size_t capacity, size_t dim, const void *vectors, int type, size_t m, size_t stride,
+                    const void *slots, int slot_bytes, size_t first);
+/* the values of m rows, by slots or from `first` on, as fp32, fp16 or bf16 (fp16: rounded, beyond its range infinite; the others
+ * hold them exactly).  A negative slot reads zeros, one that is not below capacity NaN. */
+int vsgpu_mx4_read(int device, void *stream, const void *table, size_t capacity, size_t dim, const void *slots, int slot_bytes, size_t first, size_t m,
+                   void *out, int type, size_t stride);
+/* fp32 scores of every query against rows [0, n): scores[q * scores_stride + row].  Dots are accumulated in fp32 and norms are kept
+ * in fp32, so a Cosine score of vectors shorter than 2^-100 has few digits.  Workspace: 256-byte aligned device memory. */
+size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits);   /* 0: bad arguments */
+int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride,
+                     int metric, int bits, float *scores, size_t scores_stride, void *workspace, size_t workspace_bytes);
+/* per query the k rows (1 .. 4096) of smallest score among rows [0, n), ascending by (score, row): ids / scores [nq][k], device
+ * memory, padded with -1 / -1.0.  A score is computed in 64 bits from the codes and rounded once to fp32, before rows are
+ * compared.  Rows whose score is NaN are never returned. */
+size_t vsgpu_mx4_topk_workspace(size_t n, size_t dim, size_t nq, size_t k, int bits);   /* 0: bad arguments */
+int vsgpu_mx4_topk(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride, size_t k,
+                   int metric, int bits, int64_t *ids, float *scores, void *workspace, size_t workspace_bytes);
+
 /* ---- HNSW query loops (algorithms/hnsw/hnsw.h:530-613, 1210-1258, 1967-2084) ----
  * A device snapshot of the graph the host index built (vectors stay in the vsgpu_table): level-0
  * adjacency [n][2M] + counts, upper-level blocks, deletion flags, labels, entry point.  The search

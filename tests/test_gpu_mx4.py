@@ -1,0 +1,345 @@
+"""GPU: the MXFP4 row store (vectorsimilarity_amd/mx4.py) against the format's definition in float64 (mx4_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import mx4_ref as ref
+from vectorsimilarity_amd import mx4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+METRICS = [ref.L2, ref.IP, ref.COSINE]
+
+
+def vectors(m, dim, seed, dtype=torch.float32):
+    """values over a few powers of two, exact in dtype"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, dim, generator=g) * torch.exp(0.7 * torch.randn(dim, generator=g)) / dim ** 0.5
+    return x.to(dtype)
+
+
+def store_of(x, capacity=None):
+    t = mx4.empty(x.shape[0] if capacity is None else capacity, x.shape[1], DEV)
+    mx4.write(t, x.to(DEV))
+    return t
+
+
+def same(a, b):
+    """equal values, NaN at the same places"""
+    a, b = a.double().cpu().numpy(), np.asarray(b, dtype=np.float64)
+    assert a.shape == b.shape
+    np.testing.assert_array_equal(a, b)
+
+
+# ---- write and read -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,dim", [(1, 1), (1, 768), (3, 31), (32, 32), (33, 33), (64, 64), (65, 65), (7, 127), (100, 300), (257, 1000),
+                                   (40, 1024), (5, 4097), (2, 20001)])
+def test_rows_come_back_rounded(m, dim, dtype):
+    x = vectors(m, dim, m * 7 + dim, dtype)
+    got = mx4.read(store_of(x), dim, n=m)
+    same(got, ref.micro(x.double().numpy(), 4))
+    # bf16 holds every value; fp16 is the rounding of the exact value
+    same(mx4.read(store_of(x), dim, n=m, dtype=torch.bfloat16), got.double().cpu().numpy())
+    same(mx4.read(store_of(x), dim, n=m, dtype=torch.float16), got.half().double().cpu().numpy())
+
+
+def test_every_tie_and_border():
+    """all multiples of 1/64 up to 8 beside a largest element that fixes the scale, at several scales"""
+    v = torch.arange(-512, 513) / 64.0
+    rows = []
+    for e in (-120, -20, -1, 0, 1, 30, 120):
+        for a in range(0, len(v), 31):
+            piece = torch.zeros(32)
+            piece[:len(v[a:a + 31])] = v[a:a + 31]
+            piece[31] = 7.5
+            rows.append(piece.double() * 2.0 ** e)
+    x = torch.stack(rows)
+    assert torch.equal(x.float().double(), x)
+    same(mx4.read(store_of(x.float()), 32, n=len(x)), ref.micro(x.numpy(), 4))
+
+
+def test_extreme_and_special_values():
+    big, tiny = torch.finfo(torch.float32).max, 2.0 ** -149
+    rows = torch.zeros(12, 40)
+    rows[1, :4] = torch.tensor([big, -big, big / 2, big / 16])
+    rows[2, :4] = torch.tensor([tiny, -tiny, 2.0 ** -126, 2.0 ** -127])
+    rows[3, 0] = tiny
+    rows[4, 3] = float("inf")
+    rows[5, 35] = float("-inf")
+    rows[6, 7] = float("nan")
+    rows[7, :32] = -0.0
+    rows[8, :8] = torch.tensor([2.0 ** -128, 2.0 ** -129, 1.5 * 2.0 ** -128, 2.0 ** -127, 2.0 ** -126, 2.0 ** -125, 0, -2.0 ** -128])
+    rows[9] = 1e-30
+    rows[10, 39] = 5
+    rows[11, :3] = torch.tensor([float("nan"), float("inf"), 1.0])
+    got = mx4.read(store_of(rows), 40, n=12)
+    same(got, ref.micro(rows.double().numpy(), 4))
+    assert torch.isnan(got[4, :32]).all() and not torch.isnan(got[4, 32:]).any()
+    same(mx4.read(store_of(rows), 40, n=12, dtype=torch.bfloat16), got.double().cpu().numpy())
+
+
+@pytest.mark.parametrize("slot_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("m", [1, 50, 4096, 5000])
+def test_slots_padding_and_the_last_of_equal_slots(m, slot_type):
+    dim, capacity = 70, 6000
+    g = torch.Generator().manual_seed(m)
+    x = vectors(m, dim, m + 1)
+    slots = torch.randint(0, max(2, m // 2), (m,), generator=g, dtype=slot_type) * 3
+    slots[torch.rand(m, generator=g) < 0.1] = -1
+    if m > 3:
+        slots[2] = capacity + 500    # beyond the store: skipped
+        slots[3] = torch.iinfo(slot_type).max
+    before = vectors(capacity, dim, 5)
+    table = store_of(before)
+    mx4.write(table, x.to(DEV), slots.to(DEV))
+    want = ref.micro(before.double().numpy(), 4)
+    rounded = ref.micro(x.double().numpy(), 4)
+    for i, s in enumerate(slots.tolist()):
+        if 0 <= s < capacity:
+            want[s] = rounded[i]
+    same(mx4.read(table, dim, n=capacity), want)
+    # norms belong to the rows that stayed
+    s = mx4.scores(table, capacity, torch.zeros(1, dim, device=DEV), ref.L2)[0].cpu().numpy()
+    np.testing.assert_allclose(s, (want ** 2).sum(1), rtol=2.0 ** -22, atol=0)
+
+
+def test_read_by_slots():
+    x = vectors(500, 96, 3)
+    table = store_of(x)
+    slots = torch.tensor([499, 0, -1, 33, 33, 5000, -7, 250], device=DEV)
+    want = ref.micro(x.double().numpy(), 4)
+    got = mx4.read(table, 96, slots).double().cpu().numpy()
+    for i, s in enumerate(slots.tolist()):
+        want_row = np.zeros(96) if s < 0 else (np.full(96, np.nan) if s >= 512 else want[s])
+        np.testing.assert_array_equal(got[i], want_row)
+    assert mx4.read(table, 96, slots[:0]).shape == (0, 96)
+
+
+def test_first_and_rows_beside():
+    table = store_of(vectors(100, 50, 1))
+    old = mx4.read(table, 50, n=128).clone()
+    x = vectors(10, 50, 2)
+    mx4.write(table, x.to(DEV), first=45)
+    new = mx4.read(table, 50, n=128)
+    same(new[45:55], ref.micro(x.double().numpy(), 4))
+    assert torch.equal(new[:45], old[:45]) and torch.equal(new[55:], old[55:])
+    mx4.write(table, x[:0].to(DEV), first=3)
+    mx4.write(table, x.to(DEV), slots=torch.full((10,), -1, device=DEV))
+    assert torch.equal(mx4.read(table, 50, n=128), new)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(dtype):
+    """rows of a wider matrix, from odd offsets, every second row, transposed"""
+    wide = vectors(41, 333, 9, dtype).to(DEV)
+    for x in (wide[:, 1:300], wide[:, 8:296], wide[::2, 3:131], wide.T[:, :40], wide[:1, 5:], wide[5:6].expand(3, -1)):
+        table = mx4.empty(x.shape[0], x.shape[1], DEV)
+        mx4.write(table, x)
+        same(mx4.read(table, x.shape[1], n=x.shape[0]), ref.micro(x.double().cpu().numpy(), 4))
+        q = x[:3]
+        got = mx4.scores(table, x.shape[0], q, ref.IP, 4)
+        assert torch.equal(got, mx4.scores(table, x.shape[0], q.contiguous().clone(), ref.IP, 4))
+
+
+# ---- scores ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("nq,n,dim", [(1, 1, 1), (1, 33, 64), (2, 31, 65), (5, 1000, 128), (33, 257, 300), (64, 100, 768), (65, 999, 1000),
+                                      (130, 64, 1024), (300, 40, 200), (3, 70, 4096), (40, 50, 6500), (2, 35, 9001)])
+def test_scores(nq, n, dim, bits, metric):
+    dtype = DTYPES[(nq + n + dim) % 3]
+    x, q = vectors(n, dim, 1, dtype), vectors(nq, dim, 2, dtype)
+    values = ref.micro(x.double().numpy(), 4)
+    got = mx4.scores(store_of(x), n, q.to(DEV), metric, bits).double().cpu().numpy()
+    want = ref.scores(q.double().numpy(), values, metric, bits)
+    assert got.shape == (nq, n)
+    assert (np.abs(got - want) <= ref.bound(q.double().numpy(), values, metric, bits)).all()
+
+
+def test_scores_of_part_of_a_store_and_of_rows_that_are_not_numbers():
+    x = vectors(200, 100, 4)
+    x[17, 50] = float("nan")
+    x[18] = 0
+    q = vectors(3, 100, 5)
+    q[1, 3] = float("inf")
+    values = ref.micro(x.double().numpy(), 4)
+    for metric in METRICS:
+        for n in (19, 97, 200):
+            got = mx4.scores(store_of(x), n, q.to(DEV), metric).double().cpu().numpy()
+            want = ref.scores(q.double().numpy(), values[:n], metric, 6)
+            np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+            ok = ~np.isnan(want)
+            assert (np.abs(got - want)[ok] <= ref.bound(q.double().numpy(), values[:n], metric, 6)[ok]).all()
+
+
+# ---- the k best -----------------------------------------------------------------------------------------------------------------
+def check_topk(x, q, k, metric, bits, table=None, n=None):
+    n = x.shape[0] if n is None else n
+    table = store_of(x) if table is None else table
+    values = ref.micro(x.double().numpy(), 4)[:n]
+    ids, best = mx4.topk(table, n, q.to(DEV), k, metric, bits)
+    want_ids, want = ref.topk(q.double().numpy(), values, k, metric, bits)
+    np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+    np.testing.assert_array_equal(best.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("nq,n,dim,k", [(1, 1, 1, 1), (1, 5, 3, 10), (2, 33, 64, 33), (3, 2000, 100, 1), (1, 3000, 128, 10), (33, 5000, 300, 10),
+                                        (70, 4000, 768, 5), (130, 3000, 64, 100), (5, 20000, 96, 1000), (2, 9000, 40, 4096), (9, 700, 6500, 7),
+                                        (300, 2500, 32, 3)])
+def test_topk(nq, n, dim, k, bits, metric):
+    dtype = DTYPES[(nq + n + dim) % 3]
+    check_topk(vectors(n, dim, 1, dtype), vectors(nq, dim, 2, dtype), k, metric, bits)
+
+
+@pytest.mark.parametrize("metric", METRICS)
+def test_topk_probed_table(metric):
+    """a table large enough for the sampled probe (n >= 64 k)"""
+    x, q = vectors(60000, 64, 1), vectors(40, 64, 2)
+    table = store_of(x)
+    for k in (1, 10, 100):
+        check_topk(x, q, k, metric, 6, table)
+    check_topk(x, q[:1], 10, metric, 4, table)
+    check_topk(x, q[:7], 10, metric, 6, table, n=50001)
+
+
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("kind", ["equal", "two", "cluster", "copies"])
+def test_topk_ties_and_crowded_thresholds(kind, metric):
+    """more rows at the threshold than the candidate list holds: every row is looked at, and the lowest rows win ties"""
+    n, dim = 60000, 64
+    x = vectors(n, dim, 3)
+    if kind == "equal":
+        x[:] = x[0]
+    elif kind == "two":
+        x[0::2], x[1::2] = x[0].clone(), x[1].clone()
+    elif kind == "cluster":      # one run of near rows that the probe's panels hardly meet
+        x[20000:26000] = x[0] + 1e-3 * x[20000:26000]
+    else:
+        x[1000:] = x[torch.randint(0, 1000, (n - 1000,), generator=torch.Generator().manual_seed(1))]
+    q = torch.cat([x[:2] * 1.01, vectors(3, dim, 8)])
+    check_topk(x, q, 10, metric, 6)
+    check_topk(x, q, 300, metric, 4)
+
+
+def test_topk_rows_that_are_not_numbers():
+    x = vectors(40000, 64, 6)
+    x[::3] = 0
+    x[1::6, 5] = float("nan")
+    q = vectors(4, 64, 7)
+    q[1] = 0
+    q[2, 1] = float("inf")
+    for metric in METRICS:
+        check_topk(x, q, 10, metric, 6)
+    few = x[:60]
+    few[3:] = float("nan")
+    for metric in METRICS:
+        check_topk(few, q, 10, metric, 6)
+
+
+def test_topk_far_apart_magnitudes():
+    """thresholds of rows and queries between 2^-60 and 2^60"""
+    g = torch.Generator().manual_seed(2)
+    x = vectors(20000, 64, 1) * torch.exp2(torch.randint(-60, 60, (20000, 1), generator=g).float())
+    q = vectors(6, 64, 2) * torch.exp2(torch.tensor([[-60.0], [-10], [0], [10], [50], [60]]))
+    for metric in METRICS:
+        check_topk(x, q, 10, metric, 6)
+        check_topk(x, q, 10, metric, 4)
+
+
+# ---- in use -----------------------------------------------------------------------------------------------------------------------
+def test_a_store_in_use():
+    """filled in pieces, overwritten, searched, read back: as one program would"""
+    dim = 384
+    x = vectors(9000, dim, 1, torch.bfloat16)
+    table = mx4.empty(9000, dim, DEV)
+    for a in range(0, 9000, 1234):
+        mx4.write(table, x[a:a + 1234].to(DEV), first=a)
+    x[100] = x[8999]
+    mx4.write(table, x[8999:].to(DEV), torch.tensor([100], device=DEV))
+    q = x[[100, 4000]].to(DEV)
+    ids, best = mx4.topk(table, 9000, q, 3, ref.COSINE)
+    assert ids[0, :2].tolist() == [100, 8999] and best[0, 0] == best[0, 1] and ids[1, 0] == 4000
+    dense = mx4.scores(table, 9000, q, ref.COSINE)
+    picked = torch.gather(dense, 1, ids)
+    assert (picked - best).abs().max() <= 2 * (7 * 2.0 ** -22)
+    same(mx4.read(table, dim, ids[0]), ref.micro(x.double().numpy(), 4)[ids[0].cpu().numpy()])
+
+
+def test_other_streams():
+    x, q = vectors(3000, 128, 1).to(DEV), vectors(5, 128, 2).to(DEV)
+    want = mx4.topk(store_of(x), 3000, q, 10, ref.L2)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = mx4.topk(store_of(x), 3000, q, 10, ref.L2)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_and_replayed():
+    """one graph of a write, a read, scores and two searches (their workspaces apart), replayed over new inputs"""
+    n, dim = 30000, 96
+    table = store_of(vectors(n, dim, 1))
+    x, q = torch.empty(64, dim, device=DEV), torch.empty(5, dim, device=DEV)
+    slots = torch.empty(64, dtype=torch.int64, device=DEV)
+
+    def body():
+        mx4.write(table, x, slots)
+        return (mx4.read(table, dim, slots), mx4.scores(table, n, q, ref.L2), *mx4.topk(table, n, q, 10, ref.L2), *mx4.topk(table, n, q, 100, ref.IP, 4))
+
+    def fill(seed):
+        x.copy_(vectors(64, dim, seed))
+        q.copy_(vectors(5, dim, seed + 1))
+        slots.copy_(torch.randperm(n, generator=torch.Generator().manual_seed(seed))[:64])
+        slots[60:] = -1
+
+    fill(1)
+    body()
+    torch.cuda.synchronize()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = body()
+    with torch.cuda.graph(other):
+        out2 = mx4.topk(table, n, q, 10, ref.COSINE)
+    for seed in (10, 20, 30):
+        fill(seed)
+        graph.replay()
+        got = [t.clone() for t in out]
+        other.replay()
+        got += [t.clone() for t in out2]
+        torch.cuda.synchronize()
+        for a, b in zip(got, (*body(), *mx4.topk(table, n, q, 10, ref.COSINE))):
+            assert torch.equal(a, b)
+
+
+def test_results_repeat():
+    x, q = vectors(50000, 96, 1).to(DEV), vectors(70, 96, 2).to(DEV)
+    table = store_of(x)
+    first = (mx4.scores(table, 50000, q, ref.L2), *mx4.topk(table, 50000, q, 50, ref.L2))
+    for _ in range(3):
+        again = (mx4.scores(table, 50000, q, ref.L2), *mx4.topk(table, 50000, q, 50, ref.L2))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_refusals():
+    table = store_of(vectors(40, 96, 1))
+    x = vectors(4, 96, 2).to(DEV)
+    slots = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for call in (lambda: mx4.write(table, x[:, :64]), lambda: mx4.write(table, x.double()), lambda: mx4.write(table, x.cpu()),
+                 lambda: mx4.write(table, x, slots.cpu()), lambda: mx4.write(table, x, slots[:3]), lambda: mx4.write(table, x, slots.float()),
+                 lambda: mx4.write(table, x, slots, first=1), lambda: mx4.write(table, x, first=61), lambda: mx4.write(table, x, first=-1),
+                 lambda: mx4.write(table, x[0]), lambda: mx4.write(table.float(), x), lambda: mx4.write(table[:, :-128], x),
+                 lambda: mx4.write(table, x.clone().requires_grad_()), lambda: mx4.read(table, 96), lambda: mx4.read(table, 96, slots, n=3),
+                 lambda: mx4.read(table, 96, n=65), lambda: mx4.read(table, 0, n=1), lambda: mx4.read(table, 96, n=1, dtype=torch.float64),
+                 lambda: mx4.scores(table, 65, x, ref.L2), lambda: mx4.scores(table, -1, x, ref.L2), lambda: mx4.scores(table, 40, x, 3),
+                 lambda: mx4.scores(table, 40, x, ref.L2, 8), lambda: mx4.topk(table, 40, x, 0, ref.L2), lambda: mx4.topk(table, 40, x, 4097, ref.L2)):
+        with pytest.raises(ValueError):
+            call()
+    # empty ones are not errors
+    assert mx4.scores(table, 0, x, ref.L2).shape == (4, 0) and mx4.scores(table, 40, x[:0], ref.L2).shape == (0, 40)
+    ids, best = mx4.topk(table, 0, x, 3, ref.L2)
+    assert (ids == -1).all() and (best == -1).all() and mx4.topk(table, 40, x[:0], 3, ref.L2)[0].shape == (0, 3)

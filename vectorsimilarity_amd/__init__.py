@@ -6,8 +6,9 @@ Layout (only what the hot path needs):
   _capi.py         ctypes view of libvecsim_amd.so
   VecSim.py        Python surface with the reference module's names (BFParams, BFIndex, knn_query ...)
   sharded.py       multi-GPU Flat index: row shards + all-gather of per-shard partial top-K
+  mx4.py           MXFP4 row stores on torch tensors: write, read, scores, topk
 
 Importing the package does not load the native libraries; the first index does, and raises when
 they are missing.  There is no CPU implementation of any distance.
 """
-__all__ = ["VecSim", "_capi", "sharded"]
+__all__ = ["VecSim", "_capi", "mx4", "sharded"]

@@ -164,11 +164,42 @@ GPU_EXPORTS = [
     "vsgpu_scorebuf_read",
     "vsgpu_topk", "vsgpu_range", "vsgpu_scores", "vsgpu_scores_of", "vsgpu_sq8_pair_scores", "vsgpu_table_set_sq8_mean_sum_squares", "vsgpu_table_set_sq8_block_bounds", "vsgpu_stats_reset",
     "vsgpu_stats_get", "vsgpu_set_option", "vsgpu_set_poll",
+    "vsgpu_mx4_panel_bytes", "vsgpu_mx4_write", "vsgpu_mx4_read", "vsgpu_mx4_scores_workspace", "vsgpu_mx4_scores",
+    "vsgpu_mx4_topk_workspace", "vsgpu_mx4_topk",
     "vsgpu_comm_unique_id", "vsgpu_comm_create", "vsgpu_comm_destroy", "vsgpu_comm_rank", "vsgpu_comm_world",
     "vsgpu_comm_allgather", "vsgpu_comm_broadcast", "vsgpu_comm_abort", "vsgpu_comm_staged",
 ]
 
 _lib = None
+_gpu = None
+
+
+def load_gpu():
+    """libvsgpu.so itself, for callers that hold device memory (mx4.py).  The process must have ONE HIP runtime: torch brings its
+    own, so torch has to be imported before either library is loaded."""
+    global _gpu
+    if _gpu is not None:
+        return _gpu
+    load()
+    G = C.CDLL(GPU_LIB_PATH)
+    vp, sz, i = C.c_void_p, C.c_size_t, C.c_int
+    G.vsgpu_last_error.restype = C.c_char_p
+    G.vsgpu_mx4_panel_bytes.restype = sz
+    G.vsgpu_mx4_panel_bytes.argtypes = [sz]
+    G.vsgpu_mx4_write.restype = i
+    G.vsgpu_mx4_write.argtypes = [i, vp, vp, sz, sz, vp, i, sz, sz, vp, i, sz]
+    G.vsgpu_mx4_read.restype = i
+    G.vsgpu_mx4_read.argtypes = [i, vp, vp, sz, sz, vp, i, sz, sz, vp, i, sz]
+    G.vsgpu_mx4_scores_workspace.restype = sz
+    G.vsgpu_mx4_scores_workspace.argtypes = [sz, sz, i]
+    G.vsgpu_mx4_scores.restype = i
+    G.vsgpu_mx4_scores.argtypes = [i, vp, vp, sz, sz, vp, i, sz, sz, i, i, vp, sz, vp, sz]
+    G.vsgpu_mx4_topk_workspace.restype = sz
+    G.vsgpu_mx4_topk_workspace.argtypes = [sz, sz, sz, sz, i]
+    G.vsgpu_mx4_topk.restype = i
+    G.vsgpu_mx4_topk.argtypes = [i, vp, vp, sz, sz, vp, i, sz, sz, sz, i, i, vp, vp, vp, sz]
+    _gpu = G
+    return G
 
 
 def load():

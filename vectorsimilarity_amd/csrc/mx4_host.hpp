@@ -1,0 +1,14 @@
+// mx4_host.hpp -- what the MXFP4 translation unit gives the table code in vsgpu.hip.
+#pragma once
+#include "mx4_kernels.hpp"
+
+namespace vsg {
+Mx4Rows mx4_rows_of(const void *base, size_t n, size_t dim);
+int mx4_launch_write(hipStream_t s, const Mx4Write &W, int type);
+int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus);
+int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, size_t nq, const Mx4Rows &R, int bits, uint32_t tiles, char *block,
+                       float *norm, double *sq, uint32_t *zero, size_t zero_words);
+size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits);
+int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes);
+}  // namespace vsg

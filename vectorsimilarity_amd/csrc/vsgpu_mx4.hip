@@ -1,0 +1,448 @@
+// vsgpu_mx4.hip -- the MXFP4 row store of include/vsgpu.h: checks, plans and launches around mx4_kernels.hpp (gfx950).
+//
+// Nothing here allocates, waits or keeps state: every call works on the caller's device memory and stream (a captured stream
+// included), its scratch is the caller's workspace.
+#include "vsgpu_internal.hpp"
+#include "mx4_host.hpp"
+
+using namespace vsg;
+
+namespace {
+
+// the calling thread's device, put back on every way out
+struct DeviceScope {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        ok = before == device || hipSetDevice(device) == hipSuccess;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+constexpr size_t MAX_DIM = 65536, MAX_ROWS = 0xFFFFFFE0ull, QUERY_BATCH = 256;
+constexpr size_t LDS_BUDGET = 156 * 1024;
+
+int elem_size(int type) { return type == VSGPU_F32 ? 4 : (type == VSGPU_F16 || type == VSGPU_BF16 ? 2 : 0); }
+
+int compute_units(int device) {
+    static std::atomic<int> seen[64];
+    if (device < 0 || device >= 64) return 256;
+    int n = seen[device].load(std::memory_order_relaxed);
+    if (!n) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) n = 256;
+        seen[device].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+bool bad_shape(size_t n, size_t dim) { return dim == 0 || dim > MAX_DIM || n > MAX_ROWS; }
+
+}  // namespace
+
+namespace vsg {
+
+Mx4Rows mx4_rows_of(const void *base, size_t n, size_t dim) {
+    Mx4Rows r{};
+    r.base = static_cast<char *>(const_cast<void *>(base));
+    r.dim = (uint32_t)dim;
+    r.ks = mx4_steps(r.dim);
+    r.kg = mx4_groups(r.dim);
+    r.panel = mx4_panel(r.dim);
+    r.n = n;
+    return r;
+}
+
+// how a batch of at most QUERY_BATCH queries runs
+struct Plan {
+    uint32_t tiles, qt, y;       // 32-query tiles (padded to y x qt), tiles per workgroup
+    bool global_b;
+    uint32_t qtile_bytes;
+    uint64_t panels, take;       // panels of the table / of the probe
+    bool by_row;                 // the probe keeps every row's bound, not one of 16 rows
+    uint64_t minima;             // floats per query
+    uint32_t cap, slices;
+};
+static Plan plan_scan(size_t dim, size_t nq, int bits) {
+    Plan p{};
+    const uint32_t nt = (uint32_t)((nq + 31) / 32);
+    p.qtile_bytes = mx4_qtile((uint32_t)dim, bits);
+    p.qt = nt >= 3 ? 4 : nt;
+    while (p.qt > 1 && p.qt * (p.qtile_bytes + 128) > LDS_BUDGET) p.qt /= 2;
+    p.global_b = p.qtile_bytes + 128 > LDS_BUDGET;
+    p.y = (nt + p.qt - 1) / p.qt;
+    p.tiles = p.y * p.qt;
+    return p;
+}
+static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits) {
+    Plan p = plan_scan(dim, nq, bits);
+    p.panels = (n + 31) / 32;
+    // Small tables for their k: the probe covers every row.  One bound per 16 rows would put the threshold far above the k-th score.
+    p.by_row = n < 64 * k || p.panels <= 64;
+    if (p.by_row) {
+        p.take = p.panels;
+        p.minima = n;
+        p.cap = (uint32_t)std::min<size_t>(n, 4 * k + 1024);
+    } else {
+        // a probe of n / div rows leaves about k div candidates per query: div balances their exact scores against the probe's bytes
+        const double div = std::min(64.0, std::max(8.0, std::sqrt(0.15 * (double)n / ((double)nq * (double)k))));
+        p.take = std::min<uint64_t>(p.panels, std::max<uint64_t>((uint64_t)((double)p.panels / div), 2 * k));
+        p.minima = 2 * p.take;
+        p.cap = (uint32_t)std::min<uint64_t>(n, 6 * k * ((p.panels + p.take - 1) / p.take) + 1024);
+    }
+    p.slices = k <= 128 ? 32 : 8;
+    return p;
+}
+
+struct Layout {   // of the workspace
+    size_t at = 0;
+    char *base = nullptr;
+    template <typename T> T *take(size_t count) {
+        char *p = base + at;
+        at = (at + count * sizeof(T) + 255) & ~(size_t)255;
+        return reinterpret_cast<T *>(p);
+    }
+};
+struct QueryBlock {
+    char *tiles;
+    float *norm;
+    double *sq;
+};
+static QueryBlock take_queries(Layout &L, const Plan &p) {
+    QueryBlock b;
+    b.tiles = L.take<char>((size_t)p.tiles * p.qtile_bytes);
+    b.norm = L.take<float>((size_t)p.tiles * 32);
+    b.sq = L.take<double>((size_t)p.tiles * 32);
+    return b;
+}
+struct TopkBlock {
+    QueryBlock q;
+    float2 *limit;
+    uint32_t *counts, *again, *ticket;
+    uint64_t *again_limit;
+    float *minima;
+    uint2 *cand;
+    uint64_t *part;
+};
+static TopkBlock take_topk(Layout &L, const Plan &p, size_t nq, size_t k) {
+    TopkBlock b;
+    b.q = take_queries(L, p);
+    b.limit = L.take<float2>(nq);
+    b.counts = L.take<uint32_t>(nq);
+    b.again = L.take<uint32_t>(nq);
+    b.ticket = L.take<uint32_t>(nq);
+    b.again_limit = L.take<uint64_t>(nq);
+    b.minima = L.take<float>(nq * p.minima);
+    b.cand = L.take<uint2>(nq * (size_t)p.cap);
+    b.part = L.take<uint64_t>(nq * p.slices * k);
+    return b;
+}
+
+template <int BITS> static int launch_queries(hipStream_t s, const Mx4Queries &Q, uint32_t tiles, int type) {
+    const bool wide = (((uintptr_t)Q.x | Q.stride) & 15) == 0;
+    const dim3 g(tiles), b(256);
+#define MX4_CASE(T)                                                                                       \
+    if (wide) hipLaunchKernelGGL((k_mx4_queries<T, true, BITS>), g, b, 0, s, Q);                          \
+    else hipLaunchKernelGGL((k_mx4_queries<T, false, BITS>), g, b, 0, s, Q);
+    if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
+    else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
+    else { MX4_CASE(MX4_BF16) }
+#undef MX4_CASE
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, size_t nq, const Mx4Rows &R, int bits, uint32_t tiles,
+                       char *block, float *norm, double *sq, uint32_t *zero, size_t zero_words) {
+    Mx4Queries Q{static_cast<const char *>(x), stride, (uint32_t)nq, R.dim, R.ks, R.kg, block, norm, sq, zero, (uint32_t)zero_words};
+    return bits == 6 ? launch_queries<6>(s, Q, tiles, type) : launch_queries<4>(s, Q, tiles, type);
+}
+
+template <int BITS, int QT, int MODE, int NB, bool GB> static int launch_scan5(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
+    const size_t lds = (GB ? 0 : (size_t)QT * P.qtile_bytes) + QT * 128;
+    if (lds > 64 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, GB>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(QT >= 4 ? 2 : 4, (160 * 1024) / (lds + 512)));
+    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + 3) / 4, (uint64_t)cus * fit / p.y));
+    hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, GB>), dim3((unsigned)gx, p.y), dim3(256), lds, s, P);
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+template <int BITS, int QT, int MODE> static int launch_scan3(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
+    if constexpr (QT == 1) {
+        if (p.global_b) return launch_scan5<BITS, 1, MODE, 4, true>(s, P, p, cus);
+    }
+    if (P.rows.kg == 1) return launch_scan5<BITS, QT, MODE, 1, false>(s, P, p, cus);
+    return launch_scan5<BITS, QT, MODE, 4, false>(s, P, p, cus);
+}
+template <int BITS, int MODE> static int launch_scan2(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
+    switch (p.qt) {
+    case 1: return launch_scan3<BITS, 1, MODE>(s, P, p, cus);
+    case 2: return launch_scan3<BITS, 2, MODE>(s, P, p, cus);
+    default: return launch_scan3<BITS, 4, MODE>(s, P, p, cus);
+    }
+}
+template <int MODE> static int launch_scan(hipStream_t s, const Mx4Scan &P, const Plan &p, int bits, int cus) {
+    return bits == 6 ? launch_scan2<6, MODE>(s, P, p, cus) : launch_scan2<4, MODE>(s, P, p, cus);
+}
+
+int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
+    Mx4Write W = W0;
+    if (W.m == 0) return VSGPU_OK;
+    if (W.slots && W.m > 4096) {   // (up to there every workgroup looks for later owners of its slots itself)
+        const dim3 g((unsigned)((W.m + 255) / 256));
+        hipLaunchKernelGGL(k_mx4_claim, g, dim3(256), 0, s, W, 0);
+        hipLaunchKernelGGL(k_mx4_claim, g, dim3(256), 0, s, W, 1);
+        W.claimed = 1;
+    }
+    const bool wide = (((uintptr_t)W.x | W.stride) & 15) == 0;
+    const dim3 g((unsigned)((W.m + 31) / 32)), b(256);
+#define MX4_CASE(T)                                                                \
+    if (wide) hipLaunchKernelGGL((k_mx4_write<T, true>), g, b, 0, s, W);           \
+    else hipLaunchKernelGGL((k_mx4_write<T, false>), g, b, 0, s, W);
+    if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
+    else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
+    else { MX4_CASE(MX4_BF16) }
+#undef MX4_CASE
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
+    if (R.m == 0) return VSGPU_OK;
+    const uint64_t work = R.m * ((R.rows.dim + 7) / 8);
+    const dim3 g((unsigned)std::min<uint64_t>((work + 255) / 256, (uint64_t)cus * 32)), b(256);
+    if (type == VSGPU_F32) hipLaunchKernelGGL((k_mx4_read<MX4_F32>), g, b, 0, s, R);
+    else if (type == VSGPU_F16) hipLaunchKernelGGL((k_mx4_read<MX4_F16>), g, b, 0, s, R);
+    else hipLaunchKernelGGL((k_mx4_read<MX4_BF16>), g, b, 0, s, R);
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+
+size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
+    Layout L;
+    nq = std::min(nq, QUERY_BATCH);
+    take_topk(L, plan_topk(n, dim, nq, k, bits), nq, k);
+    // (a last batch of fewer queries may plan a wider probe)
+    size_t most = L.at;
+    for (size_t m : {(size_t)1, (size_t)32, (size_t)64, (size_t)128}) {
+        if (m >= nq) break;
+        Layout M;
+        take_topk(M, plan_topk(n, dim, m, k, bits), m, k);
+        most = std::max(most, M.at);
+    }
+    return most;
+}
+
+// queries of one batch -> ids / scores [nq][k] on the device
+int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes) {
+    const Plan p = plan_topk(R.n, R.dim, nq, k, bits);
+    const int cus = compute_units(device);
+    Layout L;
+    L.base = static_cast<char *>(ws);
+    const TopkBlock b = take_topk(L, p, nq, k);
+    if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
+    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.counts, nq);
+    if (rc) return rc;
+    Mx4Scan P{};
+    P.rows = R;
+    P.tiles = b.q.tiles;
+    P.qtile_bytes = p.qtile_bytes;
+    P.nq = (uint32_t)nq;
+    P.metric = (uint32_t)metric;
+    P.qnorm = b.q.norm;
+    P.n_panels = p.panels;
+    P.n_take = p.take;
+    P.minima = b.minima;
+    P.minima_stride = p.minima;
+    P.limit = b.limit;
+    P.counts = b.counts;
+    P.cand = b.cand;
+    P.cap = p.cap;
+    P.slack = mx4_slack(R.ks);
+    rc = p.by_row ? launch_scan<MX4_PROBE_ROWS>(s, P, p, bits, cus) : launch_scan<MX4_PROBE>(s, P, p, bits, cus);
+    if (rc) return rc;
+    const Mx4Threshold T{b.minima, p.minima, p.minima, (uint32_t)k, (uint32_t)metric, b.q.norm, b.q.sq, b.limit, P.slack};
+    hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
+    HIPCHK(hipGetLastError());
+    P.n_take = p.panels;
+    rc = launch_scan<MX4_FILTER>(s, P, p, bits, cus);
+    if (rc) return rc;
+    Mx4Select S{};
+    S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
+    S.nq = (uint32_t)nq;
+    S.k = (uint32_t)k;
+    S.cap = p.cap;
+    S.counts = b.counts;
+    S.cand = b.cand;
+    S.again = b.again;
+    S.again_limit = b.again_limit;
+    S.ids = ids;
+    S.scores = scores;
+    S.slices = p.slices;
+    S.part = b.part;
+    S.ticket = b.ticket;
+    const dim3 rg((unsigned)std::max<size_t>(1, std::min<size_t>((p.cap + 15) / 16, std::max<size_t>(8, (size_t)cus * 8 / nq))), (unsigned)nq);
+    if (bits == 6) hipLaunchKernelGGL((k_mx4_rerank<6>), rg, dim3(256), 0, s, S.E, b.counts, b.cand, p.cap);
+    else hipLaunchKernelGGL((k_mx4_rerank<4>), rg, dim3(256), 0, s, S.E, b.counts, b.cand, p.cap);
+    hipLaunchKernelGGL(k_mx4_select, dim3((unsigned)nq), dim3(512), 0, s, S);
+    if (bits == 6) hipLaunchKernelGGL((k_mx4_again<6>), dim3(p.slices, (unsigned)nq), dim3(512), 0, s, S);
+    else hipLaunchKernelGGL((k_mx4_again<4>), dim3(p.slices, (unsigned)nq), dim3(512), 0, s, S);
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+
+int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, int metric, int bits,
+                     float *out, size_t out_stride, void *ws, size_t ws_bytes) {
+    const Plan p = plan_scan(R.dim, nq, bits);
+    Layout L;
+    L.base = static_cast<char *>(ws);
+    const QueryBlock b = take_queries(L, p);
+    if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
+    const int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.tiles, b.norm, b.sq, nullptr, 0);
+    if (rc) return rc;
+    Mx4Scan P{};
+    P.rows = R;
+    P.tiles = b.tiles;
+    P.qtile_bytes = p.qtile_bytes;
+    P.nq = (uint32_t)nq;
+    P.metric = (uint32_t)metric;
+    P.qnorm = b.norm;
+    P.n_panels = P.n_take = (R.n + 31) / 32;
+    P.out = out;
+    P.out_stride = out_stride;
+    P.slack = mx4_slack(R.ks);
+    return launch_scan<MX4_DENSE>(s, P, p, bits, compute_units(device));
+}
+
+}  // namespace vsg
+
+// ---------------------------------------------------------------------------------------------------------------- the C entries
+static int check_table(const void *table, size_t rows, size_t dim, const char *what) {
+    if (bad_shape(rows, dim)) return fail(VSGPU_ERR_ARG, "%s: %zu rows of %zu elements (1..%zu elements, at most %zu rows)", what, rows, dim, MAX_DIM, MAX_ROWS);
+    if (rows && (!table || ((uintptr_t)table & 15))) return fail(VSGPU_ERR_ARG, "%s: the table must be 16-byte aligned device memory", what);
+    return VSGPU_OK;
+}
+static int check_device(int device) {
+    const int n = vsgpu_device_count();
+    if (n <= 0) return fail(VSGPU_ERR_NO_DEVICE, "no HIP device visible: the gfx950 kernels are the only compute path");
+    if (device < 0 || device >= n) return fail(VSGPU_ERR_ARG, "device %d out of range (0..%d)", device, n - 1);
+    return VSGPU_OK;
+}
+static int check_vectors(const void *x, int type, size_t m, size_t stride, size_t dim, const char *what) {
+    const size_t es = (size_t)elem_size(type);
+    if (!es) return fail(VSGPU_ERR_UNSUPPORTED, "%s: vectors of type %d (fp32, fp16 and bf16 only)", what, type);
+    if (m && (!x || ((uintptr_t)x & (es - 1)) || (stride & (es - 1)) || (m > 1 && stride < dim * es)))
+        return fail(VSGPU_ERR_ARG, "%s: vectors must be aligned to their elements, rows at least %zu bytes apart (stride %zu)", what, dim * es, stride);
+    return VSGPU_OK;
+}
+static int check_queries(size_t nq, int metric, int bits) {
+    if (metric < VSGPU_L2 || metric > VSGPU_COSINE) return fail(VSGPU_ERR_ARG, "metric %d", metric);
+    if (bits != 4 && bits != 6) return fail(VSGPU_ERR_ARG, "queries of %d bits (4 or 6)", bits);
+    if (nq > ((size_t)1 << 24)) return fail(VSGPU_ERR_ARG, "%zu queries in one call", nq);
+    return VSGPU_OK;
+}
+static int check_slots(const void *slots, int slot_bytes, size_t first, size_t m, size_t capacity, const char *what) {
+    if (m > 0x7FFFFFFFull) return fail(VSGPU_ERR_ARG, "%s: %zu vectors in one call", what, m);
+    if (slots ? (slot_bytes != 4 && slot_bytes != 8) || ((uintptr_t)slots & (slot_bytes - 1)) : first > capacity || m > capacity - first)
+        return fail(VSGPU_ERR_ARG, "%s: rows %zu..%zu of %zu, or slots that are not aligned 4- or 8-byte integers", what, first, first + m, capacity);
+    return VSGPU_OK;
+}
+
+extern "C" size_t vsgpu_mx4_panel_bytes(size_t dim) { return dim == 0 || dim > MAX_DIM ? 0 : mx4_panel((uint32_t)dim); }
+
+extern "C" int vsgpu_mx4_write(int device, void *stream, void *table, size_t capacity, size_t dim, const void *vectors, int type, size_t m,
+                               size_t stride, const void *slots, int slot_bytes, size_t first) {
+    int rc = check_table(table, capacity, dim, "mx4_write");
+    if (!rc) rc = check_vectors(vectors, type, m, stride, dim, "mx4_write");
+    if (!rc) rc = check_slots(slots, slot_bytes, first, m, capacity, "mx4_write");
+    if (rc || m == 0 || capacity == 0) return rc;
+    if ((rc = check_device(device))) return rc;
+    DeviceScope scope(device);
+    if (!scope.ok) return fail(VSGPU_ERR_HIP, "hipSetDevice(%d) failed", device);
+    Mx4Write W{};
+    W.rows = mx4_rows_of(table, capacity, dim);
+    W.x = static_cast<const char *>(vectors);
+    W.stride = stride;
+    W.m = m;
+    W.slots = slots;
+    W.slots64 = slot_bytes == 8;
+    W.first = first;
+    W.capacity = capacity;
+    return mx4_launch_write(static_cast<hipStream_t>(stream), W, type);
+}
+
+extern "C" int vsgpu_mx4_read(int device, void *stream, const void *table, size_t capacity, size_t dim, const void *slots, int slot_bytes, size_t first,
+                              size_t m, void *out, int type, size_t stride) {
+    int rc = check_table(table, capacity, dim, "mx4_read");
+    if (!rc) rc = check_vectors(out, type, m, stride, dim, "mx4_read");
+    if (!rc) rc = check_slots(slots, slot_bytes, first, m, capacity, "mx4_read");
+    if (rc || m == 0) return rc;
+    if ((rc = check_device(device))) return rc;
+    DeviceScope scope(device);
+    if (!scope.ok) return fail(VSGPU_ERR_HIP, "hipSetDevice(%d) failed", device);
+    Mx4Read R{};
+    R.rows = mx4_rows_of(table, capacity, dim);
+    R.out = static_cast<char *>(out);
+    R.stride = stride;
+    R.m = m;
+    R.slots = slots;
+    R.slots64 = slot_bytes == 8;
+    R.first = first;
+    R.capacity = capacity;
+    return mx4_launch_read(static_cast<hipStream_t>(stream), R, type, compute_units(device));
+}
+
+extern "C" size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits) {
+    if (bad_shape(0, dim) || (bits != 4 && bits != 6) || nq == 0) return 0;
+    Layout L;
+    take_queries(L, plan_scan(dim, std::min(nq, QUERY_BATCH), bits));
+    return L.at;
+}
+extern "C" int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq,
+                                size_t qstride, int metric, int bits, float *scores, size_t scores_stride, void *workspace, size_t workspace_bytes) {
+    int rc = check_table(table, n, dim, "mx4_scores");
+    if (!rc) rc = check_vectors(queries, type, nq, qstride, dim, "mx4_scores");
+    if (!rc) rc = check_queries(nq, metric, bits);
+    if (rc || nq == 0 || n == 0) return rc;
+    if (!scores || (nq > 1 && scores_stride < n) || !workspace || ((uintptr_t)workspace & 255))
+        return fail(VSGPU_ERR_ARG, "mx4_scores: no output, a stride below %zu, or a workspace that is not 256-byte aligned", n);
+    if ((rc = check_device(device))) return rc;
+    DeviceScope scope(device);
+    if (!scope.ok) return fail(VSGPU_ERR_HIP, "hipSetDevice(%d) failed", device);
+    const Mx4Rows R = mx4_rows_of(table, n, dim);
+    for (size_t q = 0; q < nq; q += QUERY_BATCH) {
+        rc = mx4_scores_batch(static_cast<hipStream_t>(stream), device, R, static_cast<const char *>(queries) + q * qstride, type,
+                              std::min(QUERY_BATCH, nq - q), qstride, metric, bits, scores + q * scores_stride, scores_stride, workspace, workspace_bytes);
+        if (rc) return rc;
+    }
+    return VSGPU_OK;
+}
+
+extern "C" size_t vsgpu_mx4_topk_workspace(size_t n, size_t dim, size_t nq, size_t k, int bits) {
+    if (bad_shape(n, dim) || (bits != 4 && bits != 6) || k == 0 || k > MX4_KMAX || nq == 0) return 0;
+    return mx4_topk_bytes(n, dim, nq, k, bits);
+}
+extern "C" int vsgpu_mx4_topk(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride,
+                              size_t k, int metric, int bits, int64_t *ids, float *scores, void *workspace, size_t workspace_bytes) {
+    int rc = check_table(table, n, dim, "mx4_topk");
+    if (!rc) rc = check_vectors(queries, type, nq, qstride, dim, "mx4_topk");
+    if (!rc) rc = check_queries(nq, metric, bits);
+    if (rc) return rc;
+    if (k == 0 || k > MX4_KMAX) return fail(VSGPU_ERR_UNSUPPORTED, "mx4_topk: k = %zu (1..%u)", k, MX4_KMAX);
+    if (nq == 0) return VSGPU_OK;
+    if (n == 0) return fail(VSGPU_ERR_ARG, "mx4_topk: an empty table");
+    if (!ids || !scores || !workspace || ((uintptr_t)workspace & 255))
+        return fail(VSGPU_ERR_ARG, "mx4_topk: no output, or a workspace that is not 256-byte aligned");
+    if ((rc = check_device(device))) return rc;
+    DeviceScope scope(device);
+    if (!scope.ok) return fail(VSGPU_ERR_HIP, "hipSetDevice(%d) failed", device);
+    const Mx4Rows R = mx4_rows_of(table, n, dim);
+    for (size_t q = 0; q < nq; q += QUERY_BATCH) {
+        rc = mx4_topk_batch(static_cast<hipStream_t>(stream), device, R, static_cast<const char *>(queries) + q * qstride, type,
+                            std::min(QUERY_BATCH, nq - q), qstride, k, metric, bits, ids + q * k, scores + q * k, workspace, workspace_bytes);
+        if (rc) return rc;
+    }
+    return VSGPU_OK;
+}
