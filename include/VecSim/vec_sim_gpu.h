@@ -177,6 +177,14 @@ size_t VecSimGpu_SQ8_QueryBlobSizeCentered(size_t dim, VecSimMetric metric);    
 void VecSimGpu_SQ8_QuantizeCentered(const float *vector, const float *mean, size_t dim, VecSimMetric metric, void *storage_blob);
 void VecSimGpu_SQ8_QueryBlobCentered(const float *vector, const float *mean, size_t dim, VecSimMetric metric, float *query_blob);
 
+/* ---- MXFP4 storage: rows rounded to 4 bits an element on the GPU as they are added (vsgpu.h: blocks of 32 elements share a power
+ * of two, E2M1 codes; 412 bytes a row of 768 elements, an eighth of fp32) and queries to queryBits = 6 (E2M3) or 4 (E2M1) bits.  An
+ * extension without a counterpart in the reference.  fp32, fp16 or bf16 vectors (params->type) go in and out through the ordinary
+ * calls: add, overwrite, delete, top-k, range, batch iterator, single- and multi-value.  Every score is the metric between the two
+ * rounded vectors, computed in 64 bits and rounded once to fp32; Cosine divides by the rounded vectors' norms, nothing is
+ * normalised before it is rounded.  Stored vectors read back as their values, dim fp32. */
+VecSimIndex *VecSimGpu_NewFlatMX4(const BFParams *params, int queryBits, void *logCtx);
+
 /* Stored (preprocessed) blobs of a label in internal-id order -- what the reference's Python `get_vector`
  * reads through getStoredVectorDataByLabel (bindings.cpp:201-214).  *blob_bytes receives the stored blob size;
  * returns the number of vectors written (0: unknown label, -1: cap_bytes too small / device error); with

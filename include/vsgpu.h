@@ -32,7 +32,9 @@ enum { VSGPU_F32 = 0, VSGPU_F64 = 1, VSGPU_BF16 = 2, VSGPU_F16 = 3, VSGPU_I8 = 4
        VSGPU_SQ8 = 6,
        /* the same SQ8 rows scored against FP16 query blobs {y[dim] fp16, y_sum[, y_sum_squares] FP32}: SQ8_FP16_*
         * (IP.cpp:82-144, L2.cpp:47-74, IP_AVX512F_SQ8_FP16.h: four 16-lane accumulators, scalar below dim 16) */
-       VSGPU_SQ8H = 7 };
+       VSGPU_SQ8H = 7,
+       /* MXFP4 rows (below): tables made by vsgpu_table_create_mx4 only */
+       VSGPU_MX4 = 8 };
 enum { VSGPU_L2 = 0, VSGPU_IP = 1, VSGPU_COSINE = 2 };
 /* which reference ISA tier's summation order the kernels reproduce */
 /* AVX512_FP16: as AVX512_BF16, and fp16 rows of dim >= 32 in the order of the half-ACCUMULATING kernels a gcc >= 12 build runs on an
@@ -168,6 +170,11 @@ int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size
 size_t vsgpu_mx4_topk_workspace(size_t n, size_t dim, size_t nq, size_t k, int bits);   /* 0: bad arguments */
 int vsgpu_mx4_topk(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride, size_t k,
                    int metric, int bits, int64_t *ids, float *scores, void *workspace, size_t workspace_bytes);
+/* The same rows as a table of the calls above: host vectors of `type` (VSGPU_F32, _F16 or _BF16) go in through _append and _write and
+ * are rounded on the device, queries are host vectors of that type.  _read and _read_range return the rows' VALUES as dim fp32.
+ * _topk, _range, _scores, _scores_of, _move, _truncate and views work as on other tables, with scores as in vsgpu_mx4_topk;
+ * device-resident score vectors, synthetic rows and HNSW graphs do not exist for it. */
+vsgpu_table *vsgpu_table_create_mx4(vsgpu_ctx *ctx, int type, int metric, size_t dim, int query_bits);
 
 /* ---- HNSW query loops (algorithms/hnsw/hnsw.h:530-613, 1210-1258, 1967-2084) ----
  * A device snapshot of the graph the host index built (vectors stay in the vsgpu_table): level-0

@@ -1,0 +1,203 @@
+"""GPU: the MXFP4 Flat index behind the index API (VecSim.MX4Index), against the format's definition in float64 (mx4_ref.py)."""
+import heapq
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import mx4_ref as ref
+from vectorsimilarity_amd import VecSim
+
+pytestmark = pytest.mark.gpu
+TYPES = [VecSim.VecSimType_FLOAT32, VecSim.VecSimType_FLOAT16, VecSim.VecSimType_BFLOAT16]
+TORCH = dict(zip(TYPES, (torch.float32, torch.float16, torch.bfloat16)))
+
+
+def make(dim, metric, kind=VecSim.VecSimType_FLOAT32, bits=6, multi=False):
+    p = VecSim.BFParams()
+    p.type, p.dim, p.metric, p.multi = kind, dim, metric, multi
+    return VecSim.MX4Index(p, query_bits=bits)
+
+
+def vectors(m, dim, seed, kind=VecSim.VecSimType_FLOAT32):
+    """(array as the index takes it, float64 values)"""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(m, dim, generator=g) * torch.exp(0.7 * torch.randn(dim, generator=g))).to(TORCH[kind])
+    raw = x.numpy() if kind == VecSim.VecSimType_FLOAT32 else x.view(torch.uint16).numpy()
+    return raw, x.double().numpy()
+
+
+def best(q, values, k, metric, bits, labels=None):
+    """the index's reply: the sequential heap over the rows in id order, then (score, label)"""
+    s = ref.scores(q, values, metric, bits).astype(np.float32).astype(np.float64)
+    labels = np.arange(values.shape[0]) if labels is None else labels
+    out_l, out_s = np.full((len(q), k), -1, dtype=np.int64), np.full((len(q), k), -1.0)
+    for i in range(len(q)):
+        heap = []   # (-score, -label): the top is the largest score, of equal ones the largest label
+        for v, l in zip(s[i], labels):
+            if np.isnan(v):
+                continue
+            if len(heap) < k or v < -heap[0][0]:
+                heapq.heappush(heap, (-v, -int(l)))
+                if len(heap) > k:
+                    heapq.heappop(heap)
+        got = sorted((-a, -b) for a, b in heap)
+        out_s[i, :len(got)] = [a for a, _ in got]
+        out_l[i, :len(got)] = [b for _, b in got]
+    return out_l, out_s
+
+
+def check(ix, q, q64, values, k, metric, bits, labels=None):
+    got_l, got_s = ix.knn_query(q, k)
+    want_l, want_s = best(q64, values, k, metric, bits, labels)
+    np.testing.assert_array_equal(got_l, want_l)
+    np.testing.assert_array_equal(got_s, want_s)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("metric", [ref.L2, ref.IP, ref.COSINE])
+@pytest.mark.parametrize("bits", [4, 6])
+def test_knn_range_distance_and_vectors(bits, metric, kind):
+    n, dim = 3001, 100
+    raw, x = vectors(n, dim, 1, kind)
+    q, q64 = vectors(40, dim, 2, kind)
+    ix = make(dim, metric, kind, bits)
+    ix.add_vectors(raw[:3000], np.arange(3000))
+    ix.add_vector(raw[3000], 3000)
+    values = ref.micro(x, 4)
+    for nq, k in ((1, 10), (40, 10), (3, 500), (2, 3500)):
+        check(ix, q[:nq], q64[:nq], values, k, metric, bits)
+    s = ref.scores(q64[:1], values, metric, bits)[0].astype(np.float32)
+    radius = float(max(np.sort(s)[77], 0.0))    # (a negative radius is not the API's)
+    labels, dists = ix.range_query(q[0], radius)
+    assert sorted(labels[0].tolist()) == np.flatnonzero(s <= np.float32(radius)).tolist()
+    for label in (0, 17, 3000):
+        assert np.float32(ix.get_distance_from(label, q[0])) == s[label]
+        np.testing.assert_array_equal(ix.get_vector(label), values[label:label + 1].astype(np.float32))
+    np.testing.assert_array_equal(ix.stored_rows(5, 2996)[::11], values[5:3001:11].astype(np.float32))
+    st = ix.stats()
+    assert st["scan_kernel"] == "k_mx4_scan" and st["scan_rows"] > 0
+
+
+def test_updates():
+    """overwritten, deleted (the last row moves into the hole), added again"""
+    n, dim = 2000, 70
+    raw, x = vectors(n, dim, 3)
+    q, q64 = vectors(5, dim, 4)
+    ix = make(dim, ref.L2)
+    ix.add_vectors(raw, np.arange(n))
+    values, labels = ref.micro(x, 4), np.arange(n)
+    new, new64 = vectors(3, dim, 5)
+    for i, label in enumerate((0, 1234, 1999)):
+        assert ix.add_vector(new[i], label) == 0
+        values[label] = ref.micro(new64[i:i + 1], 4)[0]
+    check(ix, q, q64, values, 10, ref.L2, 6)
+    for label in (1999, 5, 32, 1000, 0):
+        assert ix.delete_vector(label) == 1
+        at = int(np.flatnonzero(labels == label)[0])
+        values[at], labels[at] = values[-1], labels[-1]
+        values, labels = values[:-1], labels[:-1]
+        np.testing.assert_array_equal(ix.get_vector(int(labels[min(at, len(labels) - 1)])), values[min(at, len(labels) - 1)][None].astype(np.float32))
+    check(ix, q, q64, values, 20, ref.L2, 6, labels)
+    assert ix.index_size() == n - 5 and ix.delete_vector(5) == 0
+    ix.add_vector(raw[5], 5)
+    check(ix, q, q64, np.vstack([values, ref.micro(x[5:6], 4)]), 20, ref.L2, 6, np.append(labels, 5))
+
+
+def test_ties_follow_the_index_rule():
+    """equal rows under shuffled labels: more of them than the list behind the k best holds"""
+    n, dim = 5000, 64
+    raw, x = vectors(n, dim, 6)
+    raw[::2], x[::2] = raw[0], x[0]
+    labels = np.random.default_rng(0).permutation(n)
+    ix = make(dim, ref.IP)
+    ix.add_vectors(raw, labels)
+    q, q64 = raw[:1], x[:1]
+    for k in (1, 10, 700):
+        check(ix, q, q64, ref.micro(x, 4), k, ref.IP, 6, labels)
+
+
+def test_batch_iterator_gives_every_row_once_in_order():
+    n, dim = 700, 40
+    raw, x = vectors(n, dim, 7)
+    q, q64 = vectors(1, dim, 8)
+    ix = make(dim, ref.COSINE)
+    ix.add_vectors(raw, np.arange(n))
+    it, seen, scores = ix.create_batch_iterator(q), [], []
+    while it.has_next():
+        labels, dists = it.get_next_results(97, VecSim.BY_SCORE)
+        seen += labels[0].tolist()
+        scores += dists[0].tolist()
+    want_l, want_s = best(q64, ref.micro(x, 4), n, ref.COSINE, 6)
+    assert sorted(seen) == list(range(n)) and scores == want_s[0].tolist()
+
+
+def test_multi_value():
+    n, dim = 900, 48
+    raw, x = vectors(n, dim, 9)
+    q, q64 = vectors(2, dim, 10)
+    ix = make(dim, ref.L2, multi=True)
+    labels = np.arange(n) // 3
+    ix.add_vectors(raw, labels)
+    s = ref.scores(q64, ref.micro(x, 4), ref.L2, 6).astype(np.float32).reshape(2, -1, 3).min(2)
+    got_l, got_s = ix.knn_query(q, 12)
+    for i in range(2):
+        order = np.argsort(s[i], kind="stable")[:12]
+        np.testing.assert_array_equal(got_l[i], order)
+        np.testing.assert_array_equal(got_s[i], s[i][order].astype(np.float64))
+    np.testing.assert_array_equal(ix.get_vector(7), ref.micro(x, 4)[21:24].astype(np.float32))
+
+
+def test_rows_without_a_score():
+    """a zero vector and one with a NaN: not among the k best once the heap is full"""
+    n, dim = 3000, 64
+    raw, x = vectors(n, dim, 11)
+    raw[2000] = x[2000] = 0
+    raw[2500, 3] = x[2500, 3] = np.nan
+    q, q64 = vectors(4, dim, 12)
+    for metric in (ref.L2, ref.COSINE):
+        ix = make(dim, metric)
+        ix.add_vectors(raw, np.arange(n))
+        check(ix, q, q64, ref.micro(x, 4), 10, metric, 6)
+
+
+def test_large_table_and_concurrent_readers():
+    n, dim = 300000, 96
+    raw, x = vectors(n, dim, 13)
+    q, q64 = vectors(64, dim, 14)
+    ix = make(dim, ref.L2)
+    ix.add_vectors(raw, np.arange(n))
+    values = ref.micro(x, 4)
+    s = ref.scores(q64, values, ref.L2, 6).astype(np.float32)
+    order = np.argsort(s, axis=1, kind="stable")[:, :10]
+    out = [None] * 4
+
+    def reader(i):
+        for _ in range(5):
+            out[i] = ix.knn_query(q, 10)
+
+    threads = [threading.Thread(target=reader, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for labels, dists in out:
+        np.testing.assert_array_equal(labels, order)
+        np.testing.assert_array_equal(dists, np.take_along_axis(s, order, 1).astype(np.float64))
+
+
+def test_refusals():
+    for kind in (VecSim.VecSimType_FLOAT64, VecSim.VecSimType_INT8, VecSim.VecSimType_UINT8):
+        with pytest.raises(RuntimeError):
+            make(64, ref.L2, kind)
+    with pytest.raises(ValueError):
+        make(64, ref.L2, bits=8)
+    ix = make(64, ref.L2)
+    with pytest.raises(RuntimeError):
+        ix.add_synthetic(10, 1)
+    raw, _ = vectors(3, 64, 1)
+    assert ix.knn_query(raw, 2)[0].tolist() == [[-1, -1]] * 3
+    ix.add_vectors(raw, np.arange(3))
+    with pytest.raises(RuntimeError):
+        ix.add_vectors(raw, np.arange(3))

@@ -69,7 +69,7 @@ class BatchIterator:
 class VecSimIndex:
     _owned = True
 
-    def __init__(self, params, borrowed_handle=None, sq8=False, sq8_mean=None, sq8_mean_sum_squares=0.0):
+    def __init__(self, params, borrowed_handle=None, sq8=False, sq8_mean=None, sq8_mean_sum_squares=0.0, mx4_query_bits=0):
         self._lib = _capi.load()
         if borrowed_handle is not None:   # a shard of a sharded index: the owner frees it
             self._h, self._owned = borrowed_handle, False
@@ -78,6 +78,8 @@ class VecSimIndex:
             assert mean.size == params.dim
             self._h = self._lib.VecSimGpu_NewFlatSQ8Centered(C.byref(params), mean.ctypes.data_as(C.c_void_p),
                                                              float(sq8_mean_sum_squares), None)
+        elif mx4_query_bits:              # params is a BFParams here
+            self._h = self._lib.VecSimGpu_NewFlatMX4(C.byref(params), int(mx4_query_bits), None)
         elif sq8:                         # params is a BFParams here
             self._h = self._lib.VecSimGpu_NewFlatSQ8(C.byref(params), None)
         else:
@@ -490,3 +492,36 @@ def set_timeout_callback(fn):
     cb = _capi.TIMEOUT_CB(fn)
     lib.VecSim_SetTimeoutCallbackFunction(C.cast(cb, C.c_void_p))
     return cb
+
+
+class MX4Index(VecSimIndex):
+    """Flat index over MXFP4 storage (include/VecSim/vec_sim_gpu.h: VecSimGpu_NewFlatMX4): fp32, fp16 or bf16 vectors in, rounded to 4
+    bits an element on the GPU; queries rounded to query_bits = 6 or 4.  mx4.py has the same store on torch tensors."""
+
+    def __init__(self, params, query_bits=6):
+        if query_bits not in (4, 6):
+            raise ValueError("MX4Index: queries of %s bits (4 or 6)" % (query_bits,))
+        super().__init__(params, mx4_query_bits=query_bits)
+
+    def get_vector(self, label):
+        """the stored vector(s) of a label: the rounded values as float32 [n, dim]"""
+        bb = C.c_size_t(0)
+        self._lib.VecSimGpu_GetStoredVectors(self._h, int(label), None, 0, C.byref(bb))
+        cap = 64
+        while True:
+            buf = np.zeros((cap, self._dim), dtype=np.float32)
+            n = self._lib.VecSimGpu_GetStoredVectors(self._h, int(label), buf.ctypes.data_as(C.c_void_p), buf.nbytes, C.byref(bb))
+            if n >= 0:
+                return buf[:n]
+            cap *= 8
+            if cap > 1 << 20:
+                raise RuntimeError("get_vector failed")
+
+    def stored_rows(self, first_id, n, out=None):
+        """the values of internal ids [first_id, first_id + n) as float32 [n, dim]"""
+        if out is None:
+            out = np.empty((n, self._dim), dtype=np.float32)
+        got = self._lib.VecSimGpu_ReadStoredRows(self._h, int(first_id), int(n), out.ctypes.data_as(C.c_void_p), out.nbytes)
+        if got != n:
+            raise RuntimeError("stored_rows failed")
+        return out

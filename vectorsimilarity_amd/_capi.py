@@ -142,6 +142,7 @@ EXPORTS = [
     "VecSimGpu_NewFlatSQ8", "VecSimGpu_SQ8_StoredDistance", "VecSimGpu_SQ8_StorageBlobSize", "VecSimGpu_SQ8_QueryBlobSize",
     "VecSimGpu_SQ8_Quantize", "VecSimGpu_SQ8_QueryBlob", "VecSimGpu_NewFlatSQ8Centered", "VecSimGpu_SQ8_StorageBlobSizeCentered",
     "VecSimGpu_SQ8_QueryBlobSizeCentered", "VecSimGpu_SQ8_QuantizeCentered", "VecSimGpu_SQ8_QueryBlobCentered",
+    "VecSimGpu_NewFlatMX4",
     "VecSimGpu_SetDevice", "VecSimGpu_DeviceCount", "VecSimGpu_DeviceSynchronize", "VecSimGpu_LastError", "VecSimGpu_HostTier", "VecSimGpu_HostTierNote", "VecSimGpu_IndexTier", "VecSimGpu_IndexDevice", "VecSimGpu_ResetStats",
     "VecSimGpu_GetStats", "VecSimGpu_SetOption",
     "VecSimGpu_ShardedGetUniqueId", "VecSimGpu_ShardedNew", "VecSimGpu_ShardedNewWithTransport",
@@ -165,7 +166,7 @@ GPU_EXPORTS = [
     "vsgpu_topk", "vsgpu_range", "vsgpu_scores", "vsgpu_scores_of", "vsgpu_sq8_pair_scores", "vsgpu_table_set_sq8_mean_sum_squares", "vsgpu_table_set_sq8_block_bounds", "vsgpu_stats_reset",
     "vsgpu_stats_get", "vsgpu_set_option", "vsgpu_set_poll",
     "vsgpu_mx4_panel_bytes", "vsgpu_mx4_write", "vsgpu_mx4_read", "vsgpu_mx4_scores_workspace", "vsgpu_mx4_scores",
-    "vsgpu_mx4_topk_workspace", "vsgpu_mx4_topk",
+    "vsgpu_mx4_topk_workspace", "vsgpu_mx4_topk", "vsgpu_table_create_mx4",
     "vsgpu_comm_unique_id", "vsgpu_comm_create", "vsgpu_comm_destroy", "vsgpu_comm_rank", "vsgpu_comm_world",
     "vsgpu_comm_allgather", "vsgpu_comm_broadcast", "vsgpu_comm_abort", "vsgpu_comm_staged",
 ]
@@ -253,6 +254,8 @@ def load():
     L.VecSimDebugInfoIterator_Free.argtypes = [vp]
     L.VecSimGpu_NewFlatSQ8.restype = vp
     L.VecSimGpu_NewFlatSQ8.argtypes = [vp, vp]
+    L.VecSimGpu_NewFlatMX4.restype = vp
+    L.VecSimGpu_NewFlatMX4.argtypes = [vp, i, vp]
     L.VecSimGpu_SQ8_StoredDistance.restype = C.c_double
     L.VecSimGpu_SQ8_StoredDistance.argtypes = [vp, C.c_size_t, C.c_size_t]
     L.VecSimGpu_SQ8_StorageBlobSize.restype = C.c_size_t

@@ -68,6 +68,13 @@ extern "C" VecSimIndex *VecSimGpu_NewFlatSQ8(const BFParams *params, void *logCt
     if (!ix) std::fprintf(stderr, "vecsim_amd: cannot create SQ8 GPU index: %s\n", vsgpu_last_error());
     return ix;
 }
+// ---- MXFP4 storage (vec_sim_gpu.h)
+extern "C" VecSimIndex *VecSimGpu_NewFlatMX4(const BFParams *params, int queryBits, void *logCtx) {
+    if (!params) return nullptr;
+    FlatIndex *ix = FlatIndex::createMX4(*params, queryBits, logCtx);
+    if (!ix) std::fprintf(stderr, "vecsim_amd: cannot create MXFP4 GPU index: %s\n", vsgpu_last_error());
+    return ix;
+}
 extern "C" VecSimIndex *VecSimGpu_NewFlatSQ8Centered(const BFParams *params, const float *mean, float mean_sum_squares, void *logCtx) {
     if (!params || !mean) return nullptr;
     FlatIndex *ix = FlatIndex::createSQ8(*params, logCtx, mean, mean_sum_squares);

@@ -73,7 +73,7 @@ FlatIndex *FlatIndex::create(const BFParams &p, void *logCtx) {
     ix->dim_ = p.dim;
     ix->block_size_ = p.blockSize ? p.blockSize : DEFAULT_BLOCK_SIZE;
     ix->stored_bytes_ = blob_bytes(p.type, p.dim, p.metric);
-    ix->query_bytes_ = ix->stored_bytes_;
+    ix->query_bytes_ = ix->stage_bytes_ = ix->stored_bytes_;
     ix->multi_ = p.multi;
     ix->log_ctx_ = logCtx;
     ix->ctx_ = ctx;
@@ -124,7 +124,7 @@ FlatIndex *FlatIndex::createSQ8(const BFParams &p, void *logCtx, const float *me
     ix->block_size_ = p.blockSize ? p.blockSize : DEFAULT_BLOCK_SIZE;
     if (mean) ix->sq8_mean_.assign(mean, mean + p.dim);
     ix->sq8_mss_ = mean_sum_squares;
-    ix->stored_bytes_ = sq8_storage_bytes(p.dim, p.metric, mean != nullptr);
+    ix->stored_bytes_ = ix->stage_bytes_ = sq8_storage_bytes(p.dim, p.metric, mean != nullptr);
     ix->query_bytes_ = sq8_query_bytes(p.dim, p.metric, mean != nullptr, f16);
     ix->multi_ = p.multi;
     ix->log_ctx_ = logCtx;
@@ -139,6 +139,42 @@ FlatIndex *FlatIndex::createSQ8(const BFParams &p, void *logCtx, const float *me
         return nullptr;
     }
     for (size_t i = 1; i < reader_lanes(); i++) {   // extra reader lanes (best effort: without them readers take turns)
+        auto lane = std::make_unique<Lane>();
+        lane->ctx = vsgpu_ctx_create(vsgpu_ctx_device(ctx));
+        if (!lane->ctx) break;
+        lane->view = vsgpu_table_view_create(ix->table_, lane->ctx);
+        if (!lane->view) {
+            vsgpu_ctx_destroy(lane->ctx);
+            break;
+        }
+        ix->lanes_.push_back(std::move(lane));
+    }
+    return ix;
+}
+
+FlatIndex *FlatIndex::createMX4(const BFParams &p, int query_bits, void *logCtx) {
+    if (p.dim == 0 || p.metric > VecSimMetric_Cosine) return nullptr;
+    vsgpu_ctx *ctx = vsgpu_ctx_create(resolve_device());
+    if (!ctx) return nullptr;
+    vsgpu_table *table = vsgpu_table_create_mx4(ctx, (int)p.type, (int)p.metric, p.dim, query_bits);
+    if (!table) {
+        vsgpu_ctx_destroy(ctx);
+        return nullptr;
+    }
+    FlatIndex *ix = new FlatIndex();
+    ix->type_ = p.type;
+    ix->mx4_ = true;
+    ix->metric_ = p.metric;
+    ix->dim_ = p.dim;
+    ix->block_size_ = p.blockSize ? p.blockSize : DEFAULT_BLOCK_SIZE;
+    ix->stored_bytes_ = p.dim * sizeof(float);   // rows read back as values
+    ix->stage_bytes_ = ix->query_bytes_ = p.dim * type_size(p.type);
+    ix->multi_ = p.multi;
+    ix->log_ctx_ = logCtx;
+    ix->ctx_ = ctx;
+    ix->tier_ = resolve_tier();
+    ix->table_ = table;
+    for (size_t i = 1; i < reader_lanes(); i++) {   // extra reader lanes, as above
         auto lane = std::make_unique<Lane>();
         lane->ctx = vsgpu_ctx_create(vsgpu_ctx_device(ctx));
         if (!lane->ctx) break;
@@ -178,6 +214,7 @@ void FlatIndex::toStored(const void *blob, char *out) const {
 }
 void FlatIndex::toQuery(const void *query, char *out) const {
     std::memcpy(out, query, dim_ * type_size(type_));
+    if (mx4_) return;   // (rounded on the device; Cosine divides by the rounded norms)
     if (metric_ == VecSimMetric_Cosine) normalize_blob(out, dim_, type_);
     if (sq8_ && !sq8_mean_.empty()) {
         // preprocessQuery, WithNorm (preprocessors.h:574-598): L2 stores the centred query (fp16: re-rounded), IP the raw
@@ -220,6 +257,22 @@ void FlatIndex::toQuery(const void *query, char *out) const {
 
 // stored blobs and query blobs start with dim_ elements of the same kind (SQ8 storage: codes, then FP32 metadata)
 bool FlatIndex::mayScoreNaN(const char *b) const {
+    if (mx4_) {   // scores are 64-bit sums of rounded values: only an infinity or a NaN spoils them, or Cosine against a zero vector
+        bool bad = false, some = false;
+        for (size_t i = 0; i < dim_; i++) {
+            float f;
+            if (type_ == VecSimType_FLOAT32) {
+                std::memcpy(&f, b + 4 * i, 4);
+            } else {
+                uint16_t h;
+                std::memcpy(&h, b + 2 * i, 2);
+                f = type_ == VecSimType_FLOAT16 ? fp16_widen(h) : bf16_widen(h);
+            }
+            bad |= !std::isfinite(f);
+            some |= std::fabs(f) >= 1e-37f;   // (below 2^-129 everything rounds to zero)
+        }
+        return bad || (metric_ == VecSimMetric_Cosine && !some);
+    }
     if (is_int_type(type_)) {
         if (metric_ != VecSimMetric_Cosine) return false;
         float norm;  // 1 - dot / (norm_x * norm_q): a zero vector makes 0 / 0
@@ -275,7 +328,7 @@ void FlatIndex::log(const char *level, const char *fmt, ...) const {
 // ---- ingest ----
 void FlatIndex::stageRow(const void *processed) {
     const char *p = static_cast<const char *>(processed);
-    staged_.insert(staged_.end(), p, p + stored_bytes_);
+    staged_.insert(staged_.end(), p, p + stage_bytes_);
     staged_rows_++;
 }
 
@@ -317,7 +370,7 @@ int FlatIndex::addVector(const void *blob, size_t label) {
         return 0;
     }
     // appendVector (brute_force.h:175-193): preprocess for storage, next id, maps
-    if (metric_ == VecSimMetric_Cosine || sq8_) {
+    if (!mx4_ && (metric_ == VecSimMetric_Cosine || sq8_)) {
         std::vector<char> tmp(stored_bytes_);
         toStored(blob, tmp.data());
         return appendStored(tmp.data(), label);
@@ -346,7 +399,7 @@ long FlatIndex::addBulk(const void *blobs, const size_t *labels, size_t n) {
     if (!multi_)
         for (size_t i = 0; i < n; i++)
             if (label_to_id_.count(labels[i])) return -1;
-    if ((metric_ == VecSimMetric_Cosine || sq8_) && n >= 2048) {
+    if (!mx4_ && (metric_ == VecSimMetric_Cosine || sq8_) && n >= 2048) {
         // the storage preprocessing (normalise / quantise) is per row and pure: a few host threads do it, the maps and the
         // staging buffer are then filled in order.  (SQ8 10 M x 768: 82 s of single-thread quantiser otherwise.)
         std::vector<char> pre(n * stored_bytes_);
@@ -372,7 +425,7 @@ long FlatIndex::addBulk(const void *blobs, const size_t *labels, size_t n) {
 long FlatIndex::addSynthetic(size_t n, uint64_t seed) {
     // device-generated rows are stored as generated: fp Cosine would need normalisation, so only int8 Cosine
     // (norm appended by the fill kernel) is accepted among the Cosine indexes
-    if (type_ == VecSimType_FLOAT64 || type_ == VecSimType_UINT8 || multi_ || sq8_) return -1;
+    if (type_ == VecSimType_FLOAT64 || type_ == VecSimType_UINT8 || multi_ || sq8_ || mx4_) return -1;
     if (metric_ == VecSimMetric_Cosine && type_ != VecSimType_INT8) return -1;
     if (flush()) return -1;
     const size_t first = count_;

@@ -107,6 +107,8 @@ public:
     // mean != nullptr: mean-centred blobs (QuantPreprocessor<..., WithNorm = true>, L2 and IP only); mean_sum_squares is the
     // constant DistanceCalculatorWithNorm takes for its symmetric IP correction (calculator.h:204-214)
     static FlatIndex *createSQ8(const BFParams &p, void *logCtx, const float *mean = nullptr, float mean_sum_squares = 0.0f);
+    // MXFP4 storage (vsgpu.h): vectors of p.type (FLOAT32, FLOAT16, BFLOAT16) go to the device as they are and are rounded there
+    static FlatIndex *createMX4(const BFParams &p, int query_bits, void *logCtx);
     bool isSQ8() const { return sq8_; }
     // symmetric SQ8 x SQ8 distance between the stored vectors of two labels (NaN for an unknown label)
     double storedDistance(size_t label_a, size_t label_b);
@@ -190,6 +192,8 @@ private:
     mutable std::recursive_mutex gpu_mu_;
     bool multi_ = false;
     bool sq8_ = false;
+    bool mx4_ = false;
+    size_t stage_bytes_ = 0;   // a row on its way to the device: stored_bytes_, or an MXFP4 index's vector as given
     std::vector<float> sq8_mean_;   // empty: plain SQ8
     float sq8_mss_ = 0.0f;
     // fp32 vector (dim_ floats) -> stored blob / query blob of this index (Cosine: normalised first; SQ8: quantised)

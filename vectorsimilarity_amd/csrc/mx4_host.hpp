@@ -10,5 +10,13 @@ int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, si
                        float *norm, double *sq, uint32_t *zero, size_t zero_words);
 size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits);
 int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
-                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes);
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, hipEvent_t scan_begin = nullptr, hipEvent_t scan_end = nullptr);
 }  // namespace vsg
+
+// a vsgpu_table of MXFP4 rows; host pointers, every call ends with its stream drained
+struct vsgpu_table;
+int mx4_table_store(vsgpu_table *t, const void *vectors, size_t first, size_t n);   // rounds n vectors into rows first ..
+int mx4_table_move(vsgpu_table *t, size_t dst, size_t src);
+int mx4_table_values(vsgpu_table *t, size_t first, size_t n, float *out);
+int mx4_table_scores(vsgpu_table *t, const void *query, const uint32_t *ids, size_t first, size_t n, double *scores);
+int mx4_table_topk(vsgpu_table *t, const void *queries, size_t nq, size_t qstride, size_t k, size_t cap, uint32_t *ids, double *scores, uint32_t *counts);

@@ -289,6 +289,18 @@ template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Rea
     }
 }
 
+// row src into row dst of one table (swap-delete)
+static __global__ __launch_bounds__(256) void k_mx4_move(Mx4Rows R, uint64_t dst, uint64_t src) {
+    char *d = R.at(dst / 32);
+    const char *s = R.at(src / 32);
+    const uint32_t dr = (uint32_t)(dst & 31), sr = (uint32_t)(src & 31);
+    for (uint32_t i = threadIdx.x; i < R.ks * 2; i += 256)
+        reinterpret_cast<mx4_u4 *>(d)[i * 32 + dr] = reinterpret_cast<const mx4_u4 *>(s)[i * 32 + sr];
+    for (uint32_t i = threadIdx.x; i < R.kg * 2; i += 256)
+        reinterpret_cast<uint32_t *>(d + (size_t)R.ks * 1024)[i * 32 + dr] = reinterpret_cast<const uint32_t *>(s + (size_t)R.ks * 1024)[i * 32 + sr];
+    if (threadIdx.x == 0) reinterpret_cast<float *>(d + R.panel - 128)[dr] = reinterpret_cast<const float *>(s + R.panel - 128)[sr];
+}
+
 // ---------------------------------------------------------------------------------------------------------------- queries
 // the query block: q_tiles operand tiles, then per query {norm fp32}, {|q|^2 fp64}
 struct Mx4Queries {

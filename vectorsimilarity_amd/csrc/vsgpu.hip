@@ -9,6 +9,7 @@
 #include "mfma_kernels.hpp"
 #include "mfma_lowp_kernels.hpp"
 #include "iter_kernels.hpp"
+#include "mx4_host.hpp"
 
 using namespace vsg;
 
@@ -436,6 +437,27 @@ extern "C" vsgpu_table *vsgpu_table_create(vsgpu_ctx *c, int type, int metric, i
     return t;
 }
 
+// MXFP4 rows (mx4_kernels.hpp): panels of 32 rows in the same slabs; no lane table, no filter of the other types
+extern "C" vsgpu_table *vsgpu_table_create_mx4(vsgpu_ctx *c, int type, int metric, size_t dim, int query_bits) {
+    if (!c || vsgpu_mx4_panel_bytes(dim) == 0 || metric < VSGPU_L2 || metric > VSGPU_COSINE || (query_bits != 4 && query_bits != 6) ||
+        (type != VSGPU_F32 && type != VSGPU_F16 && type != VSGPU_BF16)) {
+        fail(VSGPU_ERR_ARG, "bad MXFP4 table parameters (type %d metric %d dim %zu, queries of %d bits)", type, metric, dim, query_bits);
+        return nullptr;
+    }
+    vsgpu_table *t = new vsgpu_table();
+    t->ctx = c;
+    t->type = VSGPU_MX4;
+    t->metric = metric;
+    t->dim = dim;
+    t->row_bytes = vsgpu_mx4_panel_bytes(dim) / 32;
+    t->mx4_in = type;
+    t->mx4_bits = query_bits;
+    uint32_t shift = 6;   // (two panels at least)
+    while (((size_t)2 << shift) * t->row_bytes <= (size_t)64 << 20) shift++;
+    t->slab_shift = shift;
+    return t;
+}
+
 // A view of `parent` for another context (reader lane): same rows, own stream + scratch.  The caller keeps writers away
 // while a view is in use and calls vsgpu_table_view_sync after the parent changed.
 extern "C" vsgpu_table *vsgpu_table_view_create(vsgpu_table *parent, vsgpu_ctx *ctx) {
@@ -622,6 +644,11 @@ extern "C" int vsgpu_table_append(vsgpu_table *t, const void *host_rows, size_t 
     if (t->n + n > 0xFFFFFFF0ull) return fail(VSGPU_ERR_UNSUPPORTED, "more than 2^32 rows per device table");
     int rc = grow_to(t, t->n + n);
     if (rc) return rc;
+    if (t->type == VSGPU_MX4) {
+        rc = mx4_table_store(t, host_rows, t->n, n);
+        if (!rc) t->n += n;
+        return rc;
+    }
     const size_t slab_rows = (size_t)1 << t->slab_shift;
     const char *src = (const char *)host_rows;
     size_t id = t->n, left = n;
@@ -643,6 +670,7 @@ extern "C" int vsgpu_table_append(vsgpu_table *t, const void *host_rows, size_t 
 extern "C" int vsgpu_table_write(vsgpu_table *t, size_t id, const void *host_row) {
     if (id >= t->n) return fail(VSGPU_ERR_ARG, "row %zu out of range", id);
     HIPCHK(hipSetDevice(t->ctx->device));
+    if (t->type == VSGPU_MX4) return mx4_table_store(t, host_row, id, 1);
     // same stream as the norm kernel and the queries (the ctx stream does not synchronise with the legacy stream)
     HIPCHK(hipMemcpyAsync(row_ptr(t, id), host_row, t->row_bytes, hipMemcpyHostToDevice, t->ctx->stream));
     HIPCHK(hipStreamSynchronize(t->ctx->stream));
@@ -654,6 +682,7 @@ extern "C" int vsgpu_table_move(vsgpu_table *t, size_t dst, size_t src) {
     if (dst >= t->n || src >= t->n) return fail(VSGPU_ERR_ARG, "move %zu <- %zu out of range", dst, src);
     if (dst == src) return VSGPU_OK;
     HIPCHK(hipSetDevice(t->ctx->device));
+    if (t->type == VSGPU_MX4) return mx4_table_move(t, dst, src);
     HIPCHK(hipMemcpyAsync(row_ptr(t, dst), row_ptr(t, src), t->row_bytes, hipMemcpyDeviceToDevice, t->ctx->stream));
     return update_norms(t, dst, 1);
 }
@@ -665,6 +694,7 @@ extern "C" int vsgpu_table_truncate(vsgpu_table *t, size_t new_size) {
 extern "C" int vsgpu_table_read(vsgpu_table *t, size_t id, void *host_row) {
     if (id >= t->n) return fail(VSGPU_ERR_ARG, "row %zu out of range", id);
     HIPCHK(hipSetDevice(t->ctx->device));
+    if (t->type == VSGPU_MX4) return mx4_table_values(t, id, 1, static_cast<float *>(host_row));
     HIPCHK(hipMemcpyAsync(host_row, row_ptr(t, id), t->row_bytes, hipMemcpyDeviceToHost, t->ctx->stream));
     HIPCHK(hipStreamSynchronize(t->ctx->stream));
     if (t->type == VSGPU_SQ8 || t->type == VSGPU_SQ8H)   // (the device keeps code ^ 0x80: sq8_flip_codes)
@@ -676,6 +706,7 @@ extern "C" int vsgpu_table_read(vsgpu_table *t, size_t id, void *host_row) {
 extern "C" int vsgpu_table_read_range(vsgpu_table *t, size_t first, size_t n, void *host_rows) {
     if (first + n > t->n) return fail(VSGPU_ERR_ARG, "rows [%zu, %zu) out of range", first, first + n);
     HIPCHK(hipSetDevice(t->ctx->device));
+    if (t->type == VSGPU_MX4) return mx4_table_values(t, first, n, static_cast<float *>(host_rows));
     const size_t per_slab = (size_t)1 << t->slab_shift;
     char *dst = static_cast<char *>(host_rows);
     for (size_t r = first; r < first + n;) {
@@ -691,7 +722,7 @@ extern "C" int vsgpu_table_read_range(vsgpu_table *t, size_t first, size_t n, vo
     return VSGPU_OK;
 }
 extern "C" int vsgpu_table_append_synthetic(vsgpu_table *t, size_t n, uint64_t seed) {
-    if (t->type == VSGPU_F64 || t->type == VSGPU_U8 || t->type == VSGPU_SQ8 || t->type == VSGPU_SQ8H)
+    if (t->type == VSGPU_F64 || t->type == VSGPU_U8 || t->type == VSGPU_SQ8 || t->type == VSGPU_SQ8H || t->type == VSGPU_MX4)
         return fail(VSGPU_ERR_UNSUPPORTED, "synthetic fill: fp32/bf16/fp16/int8 only");
     if (n == 0) return VSGPU_OK;
     HIPCHK(hipSetDevice(t->ctx->device));
@@ -994,6 +1025,7 @@ extern "C" int vsgpu_scores(vsgpu_table *t, const void *query, size_t first, siz
     if (first + n > t->n) return fail(VSGPU_ERR_ARG, "range [%zu,%zu) beyond table size %zu", first, first + n, t->n);
     if (n == 0) return VSGPU_OK;
     HIPCHK(hipSetDevice(t->ctx->device));
+    if (t->type == VSGPU_MX4) return mx4_table_scores(t, query, nullptr, first, n, scores);
     int rc = stage_queries(t, query, 1, 0);
     if (rc) return rc;
     // chunk so the dense buffer stays modest
@@ -1025,7 +1057,7 @@ extern "C" void vsgpu_scorebuf_destroy(vsgpu_scorebuf *b) {
 }
 extern "C" vsgpu_scorebuf *vsgpu_scorebuf_create(vsgpu_table *t, const void *query) {
     vsgpu_ctx *c = t->ctx;
-    if (t->type == VSGPU_F64 || t->n == 0 || t->n > 0xFFFFFFF0ull) return nullptr;  // fp64 scores are doubles: host path
+    if (t->type == VSGPU_F64 || t->type == VSGPU_MX4 || t->n == 0 || t->n > 0xFFFFFFF0ull) return nullptr;  // fp64 scores are doubles: host path
     if (hipSetDevice(c->device) != hipSuccess) return nullptr;
     if (stage_queries(t, query, 1, 0)) return nullptr;
     WallMarks wm;
@@ -1170,6 +1202,7 @@ extern "C" int vsgpu_scores_of(vsgpu_table *t, const void *query, const uint32_t
         if (ids[i] >= t->n) return fail(VSGPU_ERR_ARG, "row id %u beyond table size %zu", ids[i], t->n);
     vsgpu_ctx *c = t->ctx;
     HIPCHK(hipSetDevice(c->device));
+    if (t->type == VSGPU_MX4) return mx4_table_scores(t, query, ids, 0, n, scores);
     // the ids travel through the pinned staging block, behind the query image stage_queries puts at its start: no copy from
     // pageable caller memory and no synchronisation before the kernel (the HNSW batch iterator's walk calls this once per group
     // of expansions, host/hnsw_iter.cpp: one round trip per call)
@@ -1799,6 +1832,7 @@ extern "C" int vsgpu_topk(vsgpu_table *t, const void *queries, size_t nq, size_t
         return VSGPU_OK;
     }
     HIPCHK(hipSetDevice(c->device));
+    if (t->type == VSGPU_MX4) return mx4_table_topk(t, queries, nq, qstride, k, cap, ids, scores, counts);
     const size_t n = t->n;
     const bool f64 = (t->type == VSGPU_F64);
 
@@ -1952,7 +1986,7 @@ extern "C" int vsgpu_range(vsgpu_table *t, const void *query, double radius, siz
     // dense scores, threshold on the host: the comparison is `score <= radius` on the DistType value
     // (brute_force.h:305-314).  (A filtered scan is used once the table is large.)
     std::vector<Hit> hits;
-    if (t->type == VSGPU_F64 || n <= ((size_t)1 << 20)) {
+    if (t->type == VSGPU_F64 || t->type == VSGPU_MX4 || n <= ((size_t)1 << 20)) {
         std::vector<double> row(n);
         int rc = vsgpu_scores(t, query, 0, n, row.data());
         if (rc) return rc;

@@ -27,6 +27,10 @@ extern "C" vsgpu_graph *vsgpu_graph_create(vsgpu_table *t, size_t M) {
         fail(VSGPU_ERR_ARG, "graph: M must be in [2, 32] (2M neighbours are scored by one wavefront)");
         return nullptr;
     }
+    if (t->type == VSGPU_MX4) {
+        fail(VSGPU_ERR_UNSUPPORTED, "graph: no search kernel for MXFP4 rows");
+        return nullptr;
+    }
     vsgpu_graph *g = new vsgpu_graph();
     g->t = t;
     g->M = (uint32_t)M;

@@ -236,7 +236,7 @@ size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
 
 // queries of one batch -> ids / scores [nq][k] on the device
 int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
-                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes) {
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, hipEvent_t scan_begin, hipEvent_t scan_end) {
     const Plan p = plan_topk(R.n, R.dim, nq, k, bits);
     const int cus = compute_units(device);
     Layout L;
@@ -267,8 +267,10 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
     HIPCHK(hipGetLastError());
     P.n_take = p.panels;
+    if (scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
     rc = launch_scan<MX4_FILTER>(s, P, p, bits, cus);
     if (rc) return rc;
+    if (scan_end) HIPCHK(hipEventRecord(scan_end, s));
     Mx4Select S{};
     S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
     S.nq = (uint32_t)nq;
@@ -317,6 +319,171 @@ int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *qu
 }
 
 }  // namespace vsg
+
+// ---------------------------------------------------------------------------------------------------------------- tables
+static Mx4Rows rows_of(const vsgpu_table *t) {
+    Mx4Rows r = mx4_rows_of(nullptr, t->n, t->dim);
+    r.slabs = t->d_slabs;
+    r.shift = t->slab_shift - 5;
+    return r;
+}
+static size_t in_bytes(const vsgpu_table *t) { return t->dim * (size_t)elem_size(t->mx4_in); }
+constexpr size_t STAGE_BYTES = (size_t)64 << 20;
+
+int mx4_table_store(vsgpu_table *t, const void *vectors, size_t first, size_t n) {
+    vsgpu_ctx *c = t->ctx;
+    const size_t row = in_bytes(t), piece = std::max<size_t>(1, STAGE_BYTES / row);
+    for (size_t i = 0; i < n; i += piece) {
+        const size_t m = std::min(piece, n - i);
+        const int rc = ensure(c, c->dense, m * row);
+        if (rc) return rc;
+        HIPCHK(hipMemcpyAsync(c->dense.p, static_cast<const char *>(vectors) + i * row, m * row, hipMemcpyHostToDevice, c->stream));
+        Mx4Write W{};
+        W.rows = rows_of(t);
+        W.x = static_cast<const char *>(c->dense.p);
+        W.stride = row;
+        W.m = m;
+        W.first = first + i;
+        W.capacity = t->slabs.size() << t->slab_shift;
+        const int rl = mx4_launch_write(c->stream, W, t->mx4_in);
+        if (rl) return rl;
+        HIPCHK(hipStreamSynchronize(c->stream));   // (the caller's buffer is borrowed; reader lanes query on their own streams)
+    }
+    return VSGPU_OK;
+}
+int mx4_table_move(vsgpu_table *t, size_t dst, size_t src) {
+    hipLaunchKernelGGL(k_mx4_move, dim3(1), dim3(256), 0, t->ctx->stream, rows_of(t), (uint64_t)dst, (uint64_t)src);
+    HIPCHK(hipGetLastError());
+    HIPCHK(hipStreamSynchronize(t->ctx->stream));
+    return VSGPU_OK;
+}
+int mx4_table_values(vsgpu_table *t, size_t first, size_t n, float *out) {
+    vsgpu_ctx *c = t->ctx;
+    const size_t row = t->dim * 4, piece = std::max<size_t>(1, STAGE_BYTES / row);
+    for (size_t i = 0; i < n; i += piece) {
+        const size_t m = std::min(piece, n - i);
+        const int rc = ensure(c, c->dense, m * row);
+        if (rc) return rc;
+        Mx4Read R{};
+        R.rows = rows_of(t);
+        R.out = static_cast<char *>(c->dense.p);
+        R.stride = row;
+        R.m = m;
+        R.first = first + i;
+        R.capacity = t->n;
+        const int rl = mx4_launch_read(c->stream, R, VSGPU_F32, c->n_cu);
+        if (rl) return rl;
+        HIPCHK(hipMemcpyAsync(out + i * t->dim, c->dense.p, m * row, hipMemcpyDeviceToHost, c->stream));
+        HIPCHK(hipStreamSynchronize(c->stream));
+    }
+    return VSGPU_OK;
+}
+// the host's queries, packed on the device (ctx->qfrag)
+static int upload_queries(vsgpu_table *t, const void *queries, size_t nq, size_t qstride) {
+    vsgpu_ctx *c = t->ctx;
+    const size_t row = in_bytes(t), bytes = (nq * row + 15) & ~(size_t)15;
+    int rc = ensure(c, c->qfrag, bytes);
+    if (!rc) rc = ensure_pin_up(c, bytes);
+    if (rc) return rc;
+    for (size_t q = 0; q < nq; q++) memcpy(static_cast<char *>(c->pin_up) + q * row, static_cast<const char *>(queries) + q * qstride, row);
+    return upload_block(c, c->qfrag.p, c->pin_up, bytes);
+}
+int mx4_table_scores(vsgpu_table *t, const void *query, const uint32_t *ids, size_t first, size_t n, double *scores) {
+    vsgpu_ctx *c = t->ctx;
+    int rc = upload_queries(t, query, 1, 0);
+    if (rc) return rc;
+    const Mx4Rows R = rows_of(t);
+    const Plan p = plan_scan(t->dim, 1, t->mx4_bits);
+    Layout size;
+    take_queries(size, p);
+    rc = ensure(c, c->qfrag2, size.at);
+    if (rc) return rc;
+    Layout L;
+    L.base = static_cast<char *>(c->qfrag2.p);
+    const QueryBlock b = take_queries(L, p);
+    rc = mx4_launch_queries(c->stream, c->qfrag.p, t->mx4_in, in_bytes(t), 1, R, t->mx4_bits, p.tiles, b.tiles, b.norm, b.sq, nullptr, 0);
+    if (rc) return rc;
+    const Mx4Exact E{R, b.tiles, p.qtile_bytes, (uint32_t)t->metric, b.sq};
+    const size_t piece = (size_t)1 << 24;
+    for (size_t i = 0; i < n; i += piece) {
+        const size_t m = std::min(piece, n - i);
+        rc = ensure(c, c->dense, m * 4);
+        if (!rc) rc = ensure_pinned(c, m * 4);
+        if (!rc && ids) rc = ensure(c, c->ids, m * 4);
+        if (rc) return rc;
+        if (ids) HIPCHK(hipMemcpyAsync(c->ids.p, ids + i, m * 4, hipMemcpyHostToDevice, c->stream));
+        const uint32_t *d_ids = ids ? static_cast<const uint32_t *>(c->ids.p) : nullptr;
+        const dim3 g((unsigned)std::min<size_t>((m + 15) / 16, (size_t)c->n_cu * 16));
+        if (t->mx4_bits == 6) hipLaunchKernelGGL((k_mx4_exact_rows<6>), g, dim3(256), 0, c->stream, E, 1u, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
+        else hipLaunchKernelGGL((k_mx4_exact_rows<4>), g, dim3(256), 0, c->stream, E, 1u, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
+        HIPCHK(hipGetLastError());
+        HIPCHK(hipMemcpyAsync(c->pinned, c->dense.p, m * 4, hipMemcpyDeviceToHost, c->stream));
+        HIPCHK(hipStreamSynchronize(c->stream));
+        const float *src = static_cast<const float *>(c->pinned);
+        for (size_t j = 0; j < m; j++) scores[i + j] = (double)src[j];
+    }
+    return VSGPU_OK;
+}
+// vsgpu_topk's contract: every row at or below the k-th smallest score, ascending by id.  The device returns the best `take` >= k rows;
+// only when all of them are at or below the k-th score may there be more.
+int mx4_table_topk(vsgpu_table *t, const void *queries, size_t nq, size_t qstride, size_t k, size_t cap, uint32_t *ids, double *scores, uint32_t *counts) {
+    vsgpu_ctx *c = t->ctx;
+    const size_t n = t->n, kk = std::min(k, n), take = std::min(std::min(cap, n), (size_t)MX4_KMAX);
+    if (take < kk) {   // k beyond the device's lists: the caller scores every row
+        for (size_t q = 0; q < nq; q++) counts[q] = VSGPU_COUNT_OVERFLOW;
+        return VSGPU_OK;
+    }
+    const Mx4Rows R = rows_of(t);
+    const size_t row = in_bytes(t), batch = std::min(nq, QUERY_BATCH), ws = mx4_topk_bytes(n, t->dim, batch, take, t->mx4_bits);
+    const size_t ids_bytes = (batch * take * 8 + 255) & ~(size_t)255, out_bytes = ids_bytes + batch * take * 4;
+    int rc = ensure(c, c->dense, ws);
+    if (!rc) rc = ensure(c, c->sel, out_bytes);
+    if (!rc) rc = ensure_pinned(c, out_bytes);
+    if (rc) return rc;
+    for (size_t q0 = 0; q0 < nq; q0 += QUERY_BATCH) {
+        const size_t m = std::min(QUERY_BATCH, nq - q0);
+        ScanChainGuard chain(t);
+        rc = upload_queries(t, static_cast<const char *>(queries) + q0 * qstride, m, qstride);
+        if (rc) return rc;
+        chain.before_scan();
+        const bool timed = (c->opt_events & 1) != 0;
+        rc = mx4_topk_batch(c->stream, c->device, R, c->qfrag.p, t->mx4_in, m, row, take, t->metric, t->mx4_bits, static_cast<int64_t *>(c->sel.p),
+                            reinterpret_cast<float *>(static_cast<char *>(c->sel.p) + ids_bytes), c->dense.p, c->dense.cap, timed ? c->ev_a : nullptr,
+                            timed ? c->ev_b : nullptr);
+        if (rc) return rc;
+        chain.submitted();
+        HIPCHK(hipMemcpyAsync(c->pinned, c->sel.p, out_bytes, hipMemcpyDeviceToHost, c->stream));
+        HIPCHK(hipStreamSynchronize(c->stream));
+        if (c->poll && c->poll(c->poll_user)) return VSGPU_ERR_TIMEOUT;
+        account_scan(c, t, n, 1, "k_mx4_scan");
+        const int64_t *rid = static_cast<const int64_t *>(c->pinned);
+        const float *rsc = reinterpret_cast<const float *>(static_cast<const char *>(c->pinned) + ids_bytes);
+        std::vector<std::pair<uint32_t, double>> hits;
+        for (size_t q = 0; q < m; q++) {
+            hits.clear();
+            for (size_t i = 0; i < take && rid[q * take + i] >= 0; i++) hits.emplace_back((uint32_t)rid[q * take + i], (double)rsc[q * take + i]);
+            c->stats.candidates += hits.size();
+            size_t keep = hits.size();
+            if (hits.size() > kk) {
+                const double T = hits[kk - 1].second;
+                keep = kk;
+                while (keep < hits.size() && hits[keep].second <= T) keep++;
+            }
+            if (keep == take && take < n && keep > 0 && hits[keep - 1].second <= hits[std::min(kk, keep) - 1].second) {
+                counts[q0 + q] = VSGPU_COUNT_OVERFLOW;   // ties may go on behind the list
+                continue;
+            }
+            hits.resize(keep);
+            std::sort(hits.begin(), hits.end());
+            counts[q0 + q] = (uint32_t)keep;
+            for (size_t i = 0; i < keep; i++) {
+                ids[(q0 + q) * cap + i] = hits[i].first;
+                scores[(q0 + q) * cap + i] = hits[i].second;
+            }
+        }
+    }
+    return VSGPU_OK;
+}
 
 // ---------------------------------------------------------------------------------------------------------------- the C entries
 static int check_table(const void *table, size_t rows, size_t dim, const char *what) {
