@@ -27,6 +27,9 @@ typedef float mx4_f16 __attribute__((ext_vector_type(16)));
 typedef float mx4_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int mx4_u4 __attribute__((ext_vector_type(4)));
 typedef unsigned int mx4_u2 __attribute__((ext_vector_type(2)));
+typedef unsigned int mx4_u6 __attribute__((ext_vector_type(6)));
+typedef float mx4_f2 __attribute__((ext_vector_type(2)));
+typedef float mx4_f32 __attribute__((ext_vector_type(32)));
 
 enum { MX4_F32 = 0, MX4_BF16 = 2, MX4_F16 = 3 };   // VSGPU_F32, _BF16, _F16
 enum { MX4_L2 = 0, MX4_IP = 1, MX4_COSINE = 2 };
@@ -100,10 +103,10 @@ __device__ __forceinline__ int mx4_scale(const float v[32], float &inv) {
     inv = __uint_as_float((uint32_t)(254 - byte) << 23);   // 2^(127 - byte): the exponent field 254 - byte is 2..254
     return byte;
 }
-// four dwords of E2M1 codes; returns sum (2 x)^2.  The conversion rounds to nearest even and saturates, as the format asks
-// (checked against the definition at every tie and border)
-__device__ __forceinline__ int mx4_codes4(const float v[32], float inv, bool bad, mx4_u4 &out) {
-    int ss = 0;
+// four dwords of E2M1 codes; returns sum x^2 of the rounded elements (multiples of 1/4 below 2^11: exact).  The conversion rounds to
+// nearest even and saturates, as the format asks (checked against the definition at every tie and border)
+__device__ __forceinline__ float mx4_codes4(const float v[32], float inv, bool bad, mx4_u4 &out) {
+    float ss = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         uint32_t d = 0;
@@ -112,35 +115,27 @@ __device__ __forceinline__ int mx4_codes4(const float v[32], float inv, bool bad
         d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[8 * w + 4] * inv, v[8 * w + 5] * inv, 1.f, 2);
         d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[8 * w + 6] * inv, v[8 * w + 7] * inv, 1.f, 3);
         out[w] = bad ? 0u : d;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t c = (out[w] >> (4 * j)) & 7u;
-            const int twice = c < 2 ? (int)c : (int)((2u | (c & 1u)) << ((c >> 1) - 1));   // 0 1 2 3 4 6 8 12
-            ss += twice * twice;
-        }
+        const mx4_f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(out[w], 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(out[w], 1.f, 1);
+        const mx4_f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(out[w], 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(out[w], 1.f, 3);
+        ss = __fmaf_rn(a[0], a[0], __fmaf_rn(a[1], a[1], __fmaf_rn(b[0], b[0], __fmaf_rn(b[1], b[1], ss))));
+        ss = __fmaf_rn(c[0], c[0], __fmaf_rn(c[1], c[1], __fmaf_rn(e[0], e[0], __fmaf_rn(e[1], e[1], ss))));
     }
     return ss;
 }
-// six dwords of E2M3 codes; returns sum (8 x)^2
-__device__ __forceinline__ int mx4_codes6(const float v[32], float inv, bool bad, uint32_t out[6]) {
-    uint32_t w[6] = {0, 0, 0, 0, 0, 0};
-    int ss = 0;
+// six dwords of E2M3 codes; returns sum x^2 (multiples of 1/64 below 2^11: exact).  The instruction interleaves its two sources;
+// it is given the even and the odd elements, clamped to the largest value
+__device__ __forceinline__ float mx4_codes6(const float v[32], float inv, bool bad, mx4_u6 &out) {
+    mx4_f16 even, odd;
 #pragma unroll
-    for (int j = 0; j < 32; j++) {
-        const float m = fminf(fabsf(v[j] * inv), 7.5f);
-        // steps of 1/8 below 2, 1/4 below 4, 1/2 above: rounding to the step, ties to even
-        const float up = m < 2.f ? 8.f : (m < 4.f ? 4.f : 2.f);
-        const int eighths = bad ? 0 : (int)(__builtin_rintf(m * up) * (8.f / up));
-        ss += eighths * eighths;
-        // eighths -> code: below 16 the number itself, then exponent and three digits
-        const uint32_t mag = eighths < 16 ? (uint32_t)eighths : (eighths < 32 ? 16u + (((uint32_t)eighths - 16u) >> 1) : 24u + (((uint32_t)eighths - 32u) >> 2));
-        const uint32_t c = mag | (__float_as_uint(v[j]) >> 31 << 5);
-        const int bit = 6 * j;
-        w[bit / 32] |= c << (bit % 32);
-        if (bit % 32 > 26) w[bit / 32 + 1] |= c >> (32 - bit % 32);
+    for (int j = 0; j < 16; j++) {
+        even[j] = bad ? 0.f : fminf(fmaxf(v[2 * j] * inv, -7.5f), 7.5f);
+        odd[j] = bad ? 0.f : fminf(fmaxf(v[2 * j + 1] * inv, -7.5f), 7.5f);
     }
+    out = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, 1.f);
+    const mx4_f32 r = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(out, 1.f);
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 6; i++) out[i] = bad ? 0u : w[i];
+    for (int j = 0; j < 32; j++) ss = __fmaf_rn(r[j], r[j], ss);
     return ss;
 }
 
@@ -170,13 +165,13 @@ static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) 
     if (pass == 0) __hip_atomic_store(norm, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     else atomicMax(norm, 0x80000000u | (uint32_t)i);
 }
-// One workgroup takes 32 vectors, its waves every fourth k-step; a lane rounds one block (half, row) by itself, so neither the
-// maximum nor the codes cross lanes.
-template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_write(Mx4Write W) {
-    __shared__ double part[4][64];
+// One workgroup takes 32 vectors, its waves (up to 16) the k-steps in turn; a lane rounds one block (half, row) by itself, so neither
+// the maximum nor the codes cross lanes.
+template <int T, bool WIDE> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
+    __shared__ double part[16][64];
     __shared__ int64_t slot_s[32];
     __shared__ int lost_s[32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, row = lane & 31, half = lane >> 5;
     const uint64_t i0 = (uint64_t)blockIdx.x * 32;
     if (threadIdx.x < 32) {
         const uint64_t i = i0 + threadIdx.x;
@@ -191,8 +186,8 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
         lost_s[threadIdx.x] = 0;
     }
     __syncthreads();
-    if (W.slots && !W.claimed) {   // few vectors: a later vector with the same slot takes it
-        for (uint64_t j = i0 + threadIdx.x; j < W.m; j += 256) {
+    if (W.slots && !W.claimed && W.m > 1) {   // few vectors: a later vector with the same slot takes it
+        for (uint64_t j = i0 + threadIdx.x; j < W.m; j += blockDim.x) {
             const int64_t s = mx4_slot(W.slots, W.slots64, j, W.first);
             if (s < 0) continue;
             for (int r = 0; r < 32 && i0 + r < j; r++)
@@ -207,7 +202,7 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
         char *panel = W.rows.at((uint64_t)slot / 32);
         const int at = (int)(slot & 31) + 32 * half;
         const int esz = T == MX4_F32 ? 4 : 2;
-        for (uint32_t s = wave; s < W.rows.ks; s += 4) {
+        for (uint32_t s = wave; s < W.rows.ks; s += waves) {
             const int have = (int)W.rows.dim - (int)(2 * s + half) * 32;
             float v[32], inv;
             if (have > 0) mx4_load32<T, WIDE>(x + (size_t)(2 * s + half) * 32 * esz, have, v);
@@ -217,8 +212,8 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
             }
             const int byte = mx4_scale(v, inv);
             mx4_u4 codes;
-            const int sq = mx4_codes4(v, inv, byte == 255, codes);
-            ss += byte == 255 ? __builtin_nan("") : (double)sq * mx4_pow2(2 * (byte - 128));   // (2x)^2 / 4
+            const float sq = mx4_codes4(v, inv, byte == 255, codes);
+            ss += byte == 255 ? __builtin_nan("") : (double)sq * mx4_pow2(2 * (byte - 127));
             *reinterpret_cast<mx4_u4 *>(panel + (size_t)s * 1024 + at * 16) = codes;
             panel[(size_t)W.rows.ks * 1024 + (s >> 2) * 256 + at * 4 + (s & 3)] = (char)byte;
         }
@@ -227,8 +222,7 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
     __syncthreads();
     if (threadIdx.x < 32 && slot >= 0) {
         double t = 0;
-#pragma unroll
-        for (int w = 0; w < 4; w++) t += part[w][lane] + part[w][lane + 32];
+        for (int w = 0; w < waves; w++) t += part[w][lane] + part[w][lane + 32];
         float nrm = (float)sqrt(t);
         if (!(nrm == nrm)) nrm = __uint_as_float(0x7FC00000u);
         *(reinterpret_cast<float *>(W.rows.at((uint64_t)slot / 32) + W.rows.panel - 128) + (slot & 31)) = nrm;
@@ -245,13 +239,6 @@ struct Mx4Read {
     int slots64;
     uint64_t first, capacity;
 };
-template <int T> __device__ __forceinline__ void mx4_store1(char *o, size_t i, float v) {
-    if constexpr (T == MX4_F32) reinterpret_cast<float *>(o)[i] = v;
-    else if constexpr (T == MX4_F16) reinterpret_cast<_Float16 *>(o)[i] = (_Float16)v;
-    else {   // E2M1 values have two digits: bf16 holds them exactly, its subnormals the smallest blocks'
-        reinterpret_cast<uint16_t *>(o)[i] = (uint16_t)(__float_as_uint(v) >> 16);
-    }
-}
 // 2^(byte - 127) in fp32 (byte 0: subnormal; 255: NaN)
 __device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
     return byte == 255 ? __uint_as_float(0x7FC00000u) : (byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23));
@@ -261,13 +248,14 @@ __device__ __forceinline__ float mx4_code_value(uint32_t c) {   // c: 4 bits
     const float v = m < 2 ? 0.5f * (float)m : (float)((2u | (m & 1u)) << ((m >> 1) - 1)) * 0.5f;
     return c & 8u ? -v : v;
 }
-// A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so the stores of a wave are contiguous.
-template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R) {
-    const uint32_t per_row = (R.rows.dim + 7) / 8;
-    const uint64_t total = R.m * per_row;
-    for (uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (uint64_t)gridDim.x * 256) {
-        const uint64_t i = t / per_row;
-        const uint32_t piece = (uint32_t)(t - i * per_row), e = piece * 8;
+// A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  A
+// workgroup takes `rows` whole rows (rows * per_row < 2^16: the division is one multiplication, by ceil(2^32 / per_row)).
+template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t recip) {
+    const uint64_t i0 = (uint64_t)blockIdx.x * rows;
+    const uint32_t work = (uint32_t)min((uint64_t)rows, R.m - i0) * per_row;
+    for (uint32_t t = threadIdx.x; t < work; t += 256) {
+        const uint32_t r = __umulhi(t, recip), piece = t - r * per_row, e = piece * 8;
+        const uint64_t i = i0 + r;
         const int64_t s = mx4_slot(R.slots, R.slots64, i, R.first);
         float v[8];
         if (s < 0 || (uint64_t)s >= R.capacity) {
@@ -279,16 +267,40 @@ template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Rea
             const uint32_t step = e / 64, half = (e / 32) & 1, at = (uint32_t)(s & 31) + 32 * half;
             const uint32_t codes = *reinterpret_cast<const uint32_t *>(panel + (size_t)step * 1024 + at * 16 + (e & 31) / 2);
             const float sc = mx4_scale_value((uint8_t)panel[(size_t)R.rows.ks * 1024 + (step >> 2) * 256 + at * 4 + (step & 3)]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = mx4_code_value((codes >> (4 * j)) & 15u) * sc;
+            const mx4_f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 1);
+            const mx4_f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
+            v[0] = a[0] * sc, v[1] = a[1] * sc, v[2] = b[0] * sc, v[3] = b[1] * sc, v[4] = c[0] * sc, v[5] = c[1] * sc, v[6] = d[0] * sc, v[7] = d[1] * sc;
         }
         char *o = R.out + i * R.stride;
+        if constexpr (T == MX4_F32) {
+            float *of = reinterpret_cast<float *>(o) + e;
+            if (WIDE && e + 8 <= R.rows.dim) {
+                *reinterpret_cast<mx4_f4 *>(of) = mx4_f4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<mx4_f4 *>(of + 4) = mx4_f4{v[4], v[5], v[6], v[7]};
+            } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (e + j < R.rows.dim) mx4_store1<T>(o, e + j, v[j]);
+                for (int j = 0; j < 8; j++)
+                    if (e + j < R.rows.dim) of[j] = v[j];
+            }
+        } else {
+            // E2M1 values have two digits: bf16 holds them exactly, its subnormals the smallest blocks'
+            uint16_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[j] = T == MX4_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : (uint16_t)(__float_as_uint(v[j]) >> 16);
+            uint16_t *oh = reinterpret_cast<uint16_t *>(o) + e;
+            if (WIDE && e + 8 <= R.rows.dim) {
+                mx4_u4 w;
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = (uint32_t)h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+                *reinterpret_cast<mx4_u4 *>(oh) = w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (e + j < R.rows.dim) oh[j] = h[j];
+            }
+        }
     }
 }
-
 // row src into row dst of one table (swap-delete)
 static __global__ __launch_bounds__(256) void k_mx4_move(Mx4Rows R, uint64_t dst, uint64_t src) {
     char *d = R.at(dst / 32);
@@ -313,16 +325,16 @@ struct Mx4Queries {
     uint32_t *zero;      // words to clear for the kernels behind this one
     uint32_t zero_words;
 };
-template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(256) void k_mx4_queries(Mx4Queries Q) {
-    __shared__ double part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 31, half = lane >> 5;
+template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) void k_mx4_queries(Mx4Queries Q) {
+    __shared__ double part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, row = lane & 31, half = lane >> 5;
     const uint32_t q = blockIdx.x * 32 + row;
     char *tile = Q.tiles + (size_t)blockIdx.x * mx4_qtile(Q.dim, BITS);
     char *scales = tile + (size_t)Q.ks * (BITS == 6 ? 1536 : 1024);
     const int esz = T == MX4_F32 ? 4 : 2;
-    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < Q.zero_words; i += gridDim.x * 256) Q.zero[i] = 0;
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < Q.zero_words; i += gridDim.x * blockDim.x) Q.zero[i] = 0;
     double ss = 0;
-    for (uint32_t s = wave; s < Q.kg * 4; s += 4) {
+    for (uint32_t s = wave; s < Q.kg * 4; s += waves) {
         char *sc = scales + (s >> 2) * 256 + lane * 4 + (s & 3);
         if (s >= Q.ks) {
             *sc = 0;
@@ -336,9 +348,9 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(256) v
             for (int j = 0; j < 32; j++) v[j] = 0.f;
         }
         const int byte = mx4_scale(v, inv);
-        int sq;
+        float sq;
         if constexpr (BITS == 6) {
-            uint32_t w[6];
+            mx4_u6 w;
             sq = mx4_codes6(v, inv, byte == 255, w);
             *reinterpret_cast<mx4_u4 *>(tile + (size_t)s * 1024 + lane * 16) = mx4_u4{w[0], w[1], w[2], w[3]};
             *reinterpret_cast<mx4_u2 *>(tile + (size_t)Q.ks * 1024 + (size_t)s * 512 + lane * 8) = mx4_u2{w[4], w[5]};
@@ -348,14 +360,13 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(256) v
             *reinterpret_cast<mx4_u4 *>(tile + (size_t)s * 1024 + lane * 16) = w;
         }
         *sc = (char)byte;
-        ss += byte == 255 ? __builtin_nan("") : (double)sq * mx4_pow2(2 * (byte - (BITS == 6 ? 130 : 128)));
+        ss += byte == 255 ? __builtin_nan("") : (double)sq * mx4_pow2(2 * (byte - 127));
     }
     part[wave][lane] = ss;
     __syncthreads();
     if (threadIdx.x < 32) {
         double t = 0;
-#pragma unroll
-        for (int w = 0; w < 4; w++) t += part[w][lane] + part[w][lane + 32];
+        for (int w = 0; w < waves; w++) t += part[w][lane] + part[w][lane + 32];
         Q.sq[q] = t;
         Q.norm[q] = (float)sqrt(t);
     }
@@ -366,27 +377,56 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(256) v
 // so far within 2^-22 of what it adds up (measured 2^-23.4); eight more of the same for the rounded norms and the comparison's own
 // arithmetic, and twice all of it.
 __host__ __device__ inline float mx4_slack(uint32_t ks) { return (float)(ks + 8) * 4.76837158203125e-7f; }
-constexpr float MX4_EPS = 1.9073486328125e-6f;   // 2^-19, of |q|^2 + |x|^2 (L2): the same for sums of squares
+constexpr float MX4_EPS = 1.9073486328125e-6f;    // 2^-19, of |q|^2 + |x|^2 (L2): the same for sums of squares
+constexpr float MX4_STEP = 9.5367431640625e-7f;   // 2^-20: what rounding a score to fp32 may move it, and more
+constexpr float MX4_TINY = 1e-36f;                // L2 scores below it: fp32 has no digits left to rank them by
+constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: the product of the norms may leave fp32
 
 enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
+constexpr uint32_t MX4_SEGMENTS = 32;             // a query's candidate list: one counter for every panel modulo 32
+constexpr uint32_t MX4_QUEUE = 256;               // survivors a wave collects in LDS before they go out
+struct Mx4Cand {
+    uint32_t row;
+    float low, up;                // bounds of its score
+    uint32_t pad;
+};
 struct Mx4Scan {
     Mx4Rows rows;
-    const char *tiles;           // this launch's query tiles start at blockIdx.y * QT
+    const char *tiles;            // this launch's query tiles start at blockIdx.y * QT
     uint32_t qtile_bytes;
     uint32_t nq, metric;
     const float *qnorm;
     // which panels: n_take of them, number i is i * n_panels / n_take
     uint64_t n_panels, n_take;
-    float *minima;               // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row
+    float *minima;                // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row
     uint64_t minima_stride;
-    const float2 *limit;         // FILTER: {alpha, beta} of each query
-    uint32_t *counts;            // FILTER
-    uint2 *cand;
-    uint32_t cap;
-    float *out;                  // DENSE: [nq][out_stride]
+    const float2 *limit;          // FILTER: {alpha, beta} of each query
+    uint32_t *counts;             // FILTER: [nq][MX4_SEGMENTS]
+    Mx4Cand *cand;                // [nq][MX4_SEGMENTS][segment]
+    uint32_t segment;
+    float *out;                   // DENSE: [nq][out_stride]
     uint64_t out_stride;
     float slack;
 };
+
+// the score's bounds from a matrix-core dot and the two norms
+__device__ __forceinline__ void mx4_bounds(uint32_t metric, float d, float x, float y, float slack, float &low, float &up) {
+    float s, e;
+    if (metric == MX4_L2) {
+        const float sum = __fmaf_rn(x, x, y * y);
+        s = __fmaf_rn(-2.f, d, sum);
+        e = __fmaf_rn(2.f * slack * x, y, __fmaf_rn(MX4_EPS, sum, MX4_TINY));
+    } else if (metric == MX4_IP) {
+        s = 1.f - d;
+        e = __fmaf_rn(slack * x, y, MX4_STEP * fmaxf(1.f, fabsf(s)));
+    } else {
+        s = 1.f - d / x / y;
+        e = slack + MX4_STEP;
+        if (x < MX4_SHORT || y < MX4_SHORT) s = 1.f, e = 1.001f;
+    }
+    low = s - e;
+    up = s + e;
+}
 
 // one operand pair and its scales; the table is the A operand (results: a lane one query, its registers 16 rows) or, for dense
 // scores, the B operand (a lane one row: stores along a query's line)
@@ -424,11 +464,21 @@ __device__ __forceinline__ void mx4_step(mx4_f16 *acc, const Mx4Chunk &c, const 
         acc[q] = mx4_mma<BITS, SWAP, I>(t, f, acc[q], c.sc, sq[q]);
     }
 }
+// a candidate into its query's list (segments of counters: one counter would make all waves wait in line for it)
+__device__ __forceinline__ void mx4_admit(const Mx4Scan &P, uint32_t q, uint32_t row, float d, float x, float y) {
+    const uint32_t seg = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
+    const uint32_t at = atomicAdd(&P.counts[seg], 1u);
+    if (at < P.segment) {
+        Mx4Cand c{row, 0.f, 0.f, 0u};
+        mx4_bounds(P.metric, d, x, y, P.slack, c.low, c.up);
+        P.cand[(size_t)seg * P.segment + at] = c;
+    }
+}
 
 // A wave takes whole panels, one after the other, every wave of the grid in turn; the queries' operands stay in LDS.  NB chunks of
 // the panel (256 elements each) are in flight: chunk g of the next panel is requested as soon as chunk g of this one has gone into
 // the matrix cores.  Panels of more than 4 chunks go through the same four buffers several times.
-template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launch_bounds__(256) void k_mx4_scan(Mx4Scan P) {
+template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launch_bounds__(256, 2) void k_mx4_scan(Mx4Scan P) {
     extern __shared__ char shared[];
     constexpr bool SWAP = MODE == MX4_DENSE;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
@@ -437,15 +487,22 @@ template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launc
     // (rows too wide for that, GB: the operands are read from the query block itself, through the caches)
     const char *lds = GB ? P.tiles + (size_t)blockIdx.y * QT * P.qtile_bytes : shared;
     float *yn_s = reinterpret_cast<float *>(shared + (GB ? 0 : QT * P.qtile_bytes));
+    float *yr_s = yn_s + QT * 32;   // 1 / |q|
+    mx4_u4 *queue = reinterpret_cast<mx4_u4 *>(yr_s + QT * 32) + wave * MX4_QUEUE;   // FILTER: {query, row, dot, |x|}
+    uint32_t queued = 0;
     if constexpr (!GB) {
         const mx4_u4 *src = reinterpret_cast<const mx4_u4 *>(P.tiles + (size_t)blockIdx.y * QT * P.qtile_bytes);
         const uint32_t n16 = QT * P.qtile_bytes / 16;
         for (uint32_t i = threadIdx.x; i < n16; i += 256) reinterpret_cast<mx4_u4 *>(shared)[i] = src[i];
     }
-    for (uint32_t i = threadIdx.x; i < QT * 32; i += 256) yn_s[i] = P.qnorm[q0 + i];   // (padded to whole tiles)
+    for (uint32_t i = threadIdx.x; i < QT * 32; i += 256) {
+        const float y = P.qnorm[q0 + i];   // (padded to whole tiles)
+        yn_s[i] = y;
+        yr_s[i] = 1.f / y;
+    }
     __syncthreads();
     const uint32_t sc_at = ks * (BITS == 6 ? 1536 : 1024);
-    float alpha[QT], beta[QT], qn[QT];
+    float alpha[QT], beta[QT], qn[QT], qr[QT];
 #pragma unroll
     for (int q = 0; q < QT; q++) {
         const uint32_t me = q0 + q * 32 + col;
@@ -455,11 +512,24 @@ template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launc
             beta[q] = l.y;
         }
         qn[q] = yn_s[q * 32 + col];
+        if constexpr (MODE == MX4_PROBE || MODE == MX4_PROBE_ROWS) qr[q] = yr_s[q * 32 + col];
+    }
+    bool shorts = false;   // DENSE, Cosine: queries whose reciprocal norm is no use
+    if constexpr (MODE == MX4_DENSE) {
+        for (int i = 0; i < QT * 32; i++) shorts |= yn_s[i] < MX4_SHORT && yn_s[i] > 0.f;
     }
     const uint64_t W = (uint64_t)gridDim.x * 4;
     uint64_t w = (uint64_t)blockIdx.x * 4 + wave;
     if (w >= P.n_take) return;
     const auto panel_of = [&](uint64_t i) { return P.n_take == P.n_panels ? i : i * P.n_panels / P.n_take; };
+    // the wave's queue, 64 survivors at a time
+    const auto flush = [&]() {
+        for (uint32_t i = lane; i < queued; i += 64) {
+            const mx4_u4 e = queue[i];
+            mx4_admit(P, e[0], e[1], __uint_as_float(e[2]), __uint_as_float(e[3]), yn_s[e[0] - q0]);
+        }
+        queued = 0;
+    };
     Mx4Chunk buf[NB];
     const char *panel = P.rows.at(panel_of(w));
 #pragma unroll
@@ -500,46 +570,77 @@ template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launc
         const uint64_t row0 = p * 32;
         if constexpr (MODE == MX4_DENSE) {
             const uint64_t row = row0 + col;
+            float *line = P.out + (q0 + 4 * half) * P.out_stride + row;
+            const float *yl = yn_s + 4 * half;
+            const float c0 = P.metric == MX4_L2 ? nx * nx : 1.f, rx = 1.f / nx;
+            const bool divide = P.metric == MX4_COSINE && (shorts || __any(nx < MX4_SHORT && nx > 0.f));
+            const bool whole = row0 + 32 <= P.rows.n && q0 + QT * 32 <= P.nq;
 #pragma unroll
             for (int q = 0; q < QT; q++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const uint32_t me = q0 + q * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    const float yn = yn_s[q * 32 + 8 * (v >> 2) + 4 * half + (v & 3)];
-                    float s;
-                    if (P.metric == MX4_L2) s = __fmaf_rn(-2.f, acc[q][v], __fmaf_rn(nx, nx, yn * yn));
-                    else if (P.metric == MX4_IP) s = 1.f - acc[q][v];
-                    else s = 1.f - acc[q][v] / nx / yn;
-                    if (me < P.nq && row < P.rows.n) P.out[me * P.out_stride + row] = s;
+                for (int i = 0; i < 4; i++) {
+                    const mx4_f4 y4 = *reinterpret_cast<const mx4_f4 *>(yl + q * 32 + 8 * i), r4 = *reinterpret_cast<const mx4_f4 *>(yl + (QT + q) * 32 + 8 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float d = acc[q][4 * i + j], y = y4[j];
+                        float s;
+                        if (P.metric == MX4_L2) s = __fmaf_rn(-2.f, d, __fmaf_rn(y, y, c0));
+                        else if (P.metric == MX4_IP) s = 1.f - d;
+                        else if (!divide) s = 1.f - d * rx * r4[j];
+                        else s = 1.f - d / nx / y;
+                        const uint32_t me = q * 32 + 8 * i + j;
+                        if (whole || (q0 + me + 4 * half < P.nq && row < P.rows.n)) __builtin_nontemporal_store(s, line);
+                        line += j < 3 ? P.out_stride : 5 * P.out_stride;
+                    }
                 }
         } else if constexpr (MODE == MX4_FILTER) {
-            // emitted when the score may be at or below the query's threshold: dot >= alpha |x| + beta + (L2: |x|^2 / 2)
+            // a survivor when its score may be at or below the query's threshold: dot >= alpha |x| + beta + (L2: |x|^2 / 2)
             float base[16];
 #pragma unroll
             for (int v = 0; v < 16; v++) {
                 const float x = nrm[v >> 2][v & 3];
                 base[v] = P.metric == MX4_L2 ? 0.5f * (1.f - MX4_EPS) * x * x : 0.f;
-                if (P.metric == MX4_COSINE && !(x > 0.f)) base[v] = __uint_as_float(0x7F800000u);   // no direction: score NaN
+                if (P.metric == MX4_COSINE && x < MX4_SHORT) base[v] = x > 0.f ? -__uint_as_float(0x7F800000u) : __uint_as_float(0x7F800000u);   // (zero: score NaN)
             }
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 bool any = false;
 #pragma unroll
                 for (int v = 0; v < 16; v++) any |= acc[q][v] >= __fmaf_rn(alpha[q], nrm[v >> 2][v & 3], base[v] + beta[q]);
-                if (any) {
+                if (__any(any)) {
                     const uint32_t me = q0 + q * 32 + col;
+                    uint32_t total = 0;
 #pragma unroll
                     for (int v = 0; v < 16; v++) {
+                        const bool hit = acc[q][v] >= __fmaf_rn(alpha[q], nrm[v >> 2][v & 3], base[v] + beta[q]);
+                        total += __builtin_popcountll(__ballot(hit));
+                    }
+                    if (queued + total > MX4_QUEUE) flush();
+                    const bool direct = total > MX4_QUEUE;   // a panel full of survivors
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const float x = nrm[v >> 2][v & 3], d = acc[q][v];
                         const uint64_t row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
-                        if (acc[q][v] >= __fmaf_rn(alpha[q], nrm[v >> 2][v & 3], base[v] + beta[q]) && row < P.rows.n) {
-                            const uint32_t at = atomicAdd(&P.counts[me], 1u);
-                            if (at < P.cap) P.cand[(size_t)me * P.cap + at].x = (uint32_t)row;
+                        const bool hit = d >= __fmaf_rn(alpha[q], x, base[v] + beta[q]) && row < P.rows.n;
+                        const uint64_t b = __ballot(hit);
+                        if (b == 0) continue;
+                        if (direct) {
+                            if (hit) mx4_admit(P, me, (uint32_t)row, d, x, qn[q]);
+                        } else {
+                            if (hit) queue[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u))] =
+                                mx4_u4{me, (uint32_t)row, __float_as_uint(d), __float_as_uint(x)};
+                            queued += __builtin_popcountll(b);
                         }
                     }
                 }
             }
         } else {
             const float inf = __uint_as_float(0x7F800000u);
+            float rx[16];
+            if (P.metric == MX4_COSINE) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) rx[v] = __builtin_amdgcn_rcpf(nrm[v >> 2][v & 3]);
+            }
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 const uint32_t me = q0 + q * 32 + col;
@@ -548,10 +649,13 @@ template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launc
                 for (int v = 0; v < 16; v++) {
                     const float x = nrm[v >> 2][v & 3], d = acc[q][v];
                     const uint64_t row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    float u;   // an upper bound of the score
-                    if (P.metric == MX4_L2) u = __fmaf_rn(2.f * P.slack * qn[q], x, __fmaf_rn(-2.f, d, (1.f + MX4_EPS) * (x * x + qn[q] * qn[q])));
-                    else if (P.metric == MX4_IP) u = __fmaf_rn(P.slack * qn[q], x, 1.f - d);
-                    else u = 1.f - d / x / qn[q] + P.slack;
+                    float u;   // an upper bound of the score (mx4_bounds, with reciprocals: two more roundings, in the slack)
+                    if (P.metric == MX4_L2) u = __fmaf_rn(2.f * P.slack * qn[q], x, __fmaf_rn(-2.f, d, __fmaf_rn(1.f + MX4_EPS, __fmaf_rn(x, x, qn[q] * qn[q]), MX4_TINY)));
+                    else if (P.metric == MX4_IP) u = __fmaf_rn(P.slack * qn[q], x, 1.f - d) + MX4_STEP * fmaxf(1.f, fabsf(1.f - d));
+                    else {
+                        u = 1.f - d * rx[v] * qr[q] + (P.slack + MX4_STEP);
+                        if (x < MX4_SHORT || qn[q] < MX4_SHORT) u = x > 0.f ? 2.001f : inf;
+                    }
                     if (row >= P.rows.n || !(u == u)) u = inf;
                     if constexpr (MODE == MX4_PROBE_ROWS) {
                         if (me < P.nq && row < P.rows.n) P.minima[me * P.minima_stride + row] = u;
@@ -565,6 +669,7 @@ template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launc
         }
         panel = next;
     }
+    if constexpr (MODE == MX4_FILTER) flush();
 }
 
 // ---------------------------------------------------------------------------------------------------------------- threshold
@@ -573,38 +678,59 @@ __device__ __forceinline__ uint32_t mx4_key(float f) {   // order-preserving; Na
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float mx4_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
-struct Mx4Threshold {
-    const float *minima;
-    uint64_t stride, count;
-    uint32_t k, metric;
-    const float *qnorm;
-    const double *qsq;
-    float2 *limit;
-    float slack;
+constexpr uint32_t MX4_KEY_INF = 0xFF800000u;   // key of infinity: not counted
+constexpr uint32_t MX4_BINS = 2048;
+struct Mx4Bins {   // shared
+    uint32_t hist[MX4_BINS];
+    uint32_t lo, hi, pick, left, in;
 };
-// tau = the k-th smallest upper bound (each of different rows, so at least k rows are at or below it), then what the filter compares
-// against.  The score of a row is rounded to fp32 before rows are compared: half a step of it more.
-static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t pick_s, left_s;
-    const uint32_t q = blockIdx.x;
-    const float *m = T.minima + q * T.stride;
-    uint32_t prefix = 0, mask = 0, need = T.k;
-    const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-    const bool all = T.k > T.count;
-    for (int pass = 0; pass < 3 && !all; pass++) {
-        const uint32_t bins = 1u << bits[pass];
-        for (uint32_t i = threadIdx.x; i < bins; i += 1024) hist[i] = 0;
+// A number at or above the k-th smallest of n keys, and close to it (MX4_KEY_INF: fewer than k of them are finite).  Bins of equal
+// width between the smallest and the largest key, then inside the bin of the k-th; a bin of few keys is near enough.  All threads.
+template <typename F> __device__ __forceinline__ uint32_t mx4_kth(Mx4Bins &B, uint64_t n, uint32_t k, F key_of) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        B.lo = 0xFFFFFFFFu;
+        B.hi = 0;
+    }
+    __syncthreads();
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint32_t key = key_of(i);
+        if (key < MX4_KEY_INF) {
+            lo = min(lo, key);
+            hi = max(hi, key);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor(lo, o));
+        hi = max(hi, (uint32_t)__shfl_xor(hi, o));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        atomicMin(&B.lo, lo);
+        atomicMax(&B.hi, hi);
+    }
+    __syncthreads();
+    lo = B.lo;
+    hi = B.hi;
+    if (lo > hi) return MX4_KEY_INF;
+    uint32_t need = k;
+    for (int pass = 0; pass < 4; pass++) {
+        // bins of 2^shift keys from lo on
+        const uint32_t range = hi - lo;
+        const int shift = range < MX4_BINS ? 0 : 32 - __builtin_clz(range) - 11;
+        for (uint32_t i = threadIdx.x; i < MX4_BINS; i += blockDim.x) B.hist[i] = 0;
+        if (threadIdx.x == 0) B.pick = 0xFFFFFFFFu;
         __syncthreads();
-        for (uint64_t i = threadIdx.x; i < T.count; i += 1024) {
-            const uint32_t key = mx4_key(m[i]);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shifts[pass]) & (bins - 1)], 1u);
+        for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
+            const uint32_t key = key_of(i);
+            if (key >= lo && key <= hi && key < MX4_KEY_INF) atomicAdd(&B.hist[(key - lo) >> shift], 1u);
         }
         __syncthreads();
-        if (threadIdx.x < 64) {   // one wave finds the bin of the need-th: bins / 64 each, then the lane's own
-            const uint32_t each = bins / 64, b0 = threadIdx.x * each;
+        if (threadIdx.x < 64) {   // one wave: 32 bins a lane, then the lane's own
+            const uint32_t b0 = threadIdx.x * (MX4_BINS / 64);
             uint32_t sum = 0;
-            for (uint32_t i = 0; i < each; i++) sum += hist[b0 + i];
+            for (uint32_t i = 0; i < MX4_BINS / 64; i++) sum += B.hist[b0 + i];
             uint32_t before = sum;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -614,34 +740,57 @@ static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
             before -= sum;
             if (before < need && need <= before + sum) {
                 uint32_t i = 0;
-                while (before + hist[b0 + i] < need) before += hist[b0 + i++];
-                pick_s = b0 + i;
-                left_s = need - before;
+                while (before + B.hist[b0 + i] < need) before += B.hist[b0 + i++];
+                B.pick = b0 + i;
+                B.left = need - before;
+                B.in = B.hist[b0 + i];
             }
         }
         __syncthreads();
-        prefix |= pick_s << shifts[pass];
-        mask |= (bins - 1) << shifts[pass];
-        need = left_s;
+        const uint32_t pick = B.pick, left = B.left, in = B.in;
         __syncthreads();
+        if (pick == 0xFFFFFFFFu) return MX4_KEY_INF;   // fewer than k finite keys
+        hi = min(hi, lo + (pick << shift) + ((1u << shift) - 1));
+        lo = lo + (pick << shift);
+        need = left;
+        if (shift == 0 || in <= 8 + k / 16) break;
     }
+    return hi;
+}
+struct Mx4Threshold {
+    const float *minima;
+    uint64_t stride, count;
+    uint32_t k, metric;
+    const float *qnorm;
+    const double *qsq;
+    float2 *limit;
+    float slack;
+};
+// a Cosine query of norm zero, or one that holds an infinity or a NaN: every score is NaN
+__device__ __forceinline__ bool mx4_dead(uint32_t metric, double sq) { return !(sq == sq) || (metric == MX4_COSINE && sq == 0); }
+// tau = a little above the k-th smallest upper bound (each of different rows, so at least k rows are at or below it), then what the
+// filter compares against
+static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
+    __shared__ Mx4Bins bins;
+    const uint32_t q = blockIdx.x;
+    const float *m = T.minima + q * T.stride;
+    const uint32_t key = T.k > T.count ? MX4_KEY_INF : mx4_kth(bins, T.count, T.k, [&](uint64_t i) { return mx4_key(m[i]); });
     if (threadIdx.x) return;
     const float inf = __uint_as_float(0x7F800000u);
-    const float tau = all ? inf : mx4_unkey(prefix), yn = T.qnorm[q];
+    const float tau = mx4_unkey(key), yn = T.qnorm[q];
     float2 l;
     if (T.metric == MX4_L2) {
         l.x = -T.slack * yn;
-        l.y = 0.5f * ((1.f - MX4_EPS) * yn * yn - (tau + MX4_EPS * fabsf(tau)));
+        l.y = 0.5f * ((1.f - MX4_EPS) * yn * yn - (tau + MX4_EPS * fabsf(tau)) - 2.f * MX4_TINY);
     } else if (T.metric == MX4_IP) {
         l.x = -T.slack * yn;
-        l.y = 1.f - tau - 9.5367431640625e-7f * fmaxf(1.f, fabsf(tau));   // 2^-20
+        l.y = 1.f - tau - MX4_STEP * fmaxf(1.f, fabsf(tau));
     } else {
-        l.x = ((1.f - tau) - T.slack - 9.5367431640625e-7f) * yn;
-        l.y = 0.f;
+        l.x = ((1.f - tau) - T.slack - MX4_STEP) * yn;
+        l.y = yn < MX4_SHORT ? -inf : 0.f;
     }
     if (tau == inf) l = make_float2(0.f, -inf);
-    const double sq = T.qsq[q];
-    if (!(sq == sq) || (T.metric == MX4_COSINE && sq == 0)) l = make_float2(0.f, inf);   // every score is NaN
+    if (mx4_dead(T.metric, T.qsq[q])) l = make_float2(0.f, inf);
     T.limit[q] = l;
 }
 
@@ -706,15 +855,6 @@ template <int BITS> __device__ __forceinline__ float mx4_exact_score(const Mx4Ex
         xx += __shfl_xor(xx, o);
     }
     return mx4_final(E.metric, dot, xx, E.qsq[q]);
-}
-// the filter's candidates, scored exactly in place
-template <int BITS> static __global__ __launch_bounds__(256) void k_mx4_rerank(Mx4Exact E, const uint32_t *counts, uint2 *cand, uint32_t cap) {
-    const uint32_t q = blockIdx.y, n = min(counts[q], cap);
-    for (uint32_t i = (blockIdx.x * 256 + threadIdx.x) / MX4_LANES; i < n; i += gridDim.x * (256 / MX4_LANES)) {
-        uint2 *c = cand + (size_t)q * cap + i;
-        const float s = mx4_exact_score<BITS>(E, q, c->x);
-        if (threadIdx.x % MX4_LANES == 0) c->y = __float_as_uint(s);
-    }
 }
 // rows first .. first + m - 1, or ids[0 .. m)
 template <int BITS> static __global__ __launch_bounds__(256) void k_mx4_exact_rows(Mx4Exact E, uint32_t nq, const uint32_t *ids, uint64_t first, uint64_t m, float *out) {
@@ -781,9 +921,9 @@ __device__ __forceinline__ void mx4_keep_add(const Mx4Keep &K, uint64_t key, uin
 }
 struct Mx4Select {
     Mx4Exact E;
-    uint32_t nq, k, cap;
-    const uint32_t *counts;
-    const uint2 *cand;
+    uint32_t nq, k, segment;
+    const uint32_t *counts;     // [nq][MX4_SEGMENTS]
+    const Mx4Cand *cand;
     uint32_t *again;            // [nq]: 1 = the list did not hold the answer: k_mx4_again
     uint64_t *again_limit;      // [nq] ... which then needs nothing above this
     int64_t *ids;               // [nq][k]
@@ -800,30 +940,80 @@ __device__ __forceinline__ void mx4_emit(const Mx4Select &S, uint32_t q, const u
         S.scores[(size_t)q * S.k + i] = key == MX4_NONE ? -1.f : mx4_unkey((uint32_t)(key >> 32));
     }
 }
-static __global__ __launch_bounds__(512) void k_mx4_select(Mx4Select S) {
+// One workgroup a query: of its candidates only those whose lower bound is at or below the k-th smallest upper bound (little more
+// than k) are scored exactly, 16 lanes a row; then sorted.
+constexpr uint32_t MX4_FINISH = 1024;
+template <int BITS> static __global__ __launch_bounds__(1024) void k_mx4_finish(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];
-    __shared__ uint32_t n_s;
+    __shared__ Mx4Bins bins;
+    __shared__ uint32_t rows_s[2 * MX4_FINISH];
+    __shared__ uint32_t first_s[MX4_SEGMENTS + 1], n_s, rows_n;
     __shared__ uint64_t limit_s;
-    const uint32_t q = blockIdx.x, found = S.counts[q], n = min(found, S.cap);
+    __shared__ int over_s;
+    const uint32_t q = blockIdx.x;
     const Mx4Keep K{keys, &n_s, &limit_s, S.k};
-    if (threadIdx.x == 0) {
-        n_s = 0;
-        limit_s = MX4_NONE;
-    }
-    for (uint32_t i0 = 0; i0 < n; i0 += 512) {
-        const uint32_t i = i0 + threadIdx.x;
-        uint64_t key = MX4_NONE;
-        if (i < n) {
-            const uint2 c = S.cand[(size_t)q * S.cap + i];
-            key = mx4_pack(__uint_as_float(c.y), c.x);
+    if (threadIdx.x < 64) {
+        const uint32_t c = threadIdx.x < MX4_SEGMENTS ? S.counts[q * MX4_SEGMENTS + threadIdx.x] : 0;
+        const bool over = c > S.segment;
+        uint32_t sum = min(c, S.segment);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(sum, o);
+            if ((int)threadIdx.x >= o) sum += t;
         }
-        mx4_keep_add(K, key, 512);
+        if (threadIdx.x < MX4_SEGMENTS) first_s[threadIdx.x + 1] = sum;
+        const bool any = __any(over);
+        if (threadIdx.x == 0) {
+            first_s[0] = 0;
+            n_s = 0;
+            rows_n = 0;
+            limit_s = MX4_NONE;
+            over_s = any;
+        }
+    }
+    __syncthreads();
+    const uint32_t n = first_s[MX4_SEGMENTS];
+    const auto at = [&](uint32_t i) -> const Mx4Cand & {   // candidate i of all segments
+        uint32_t seg = 0;
+#pragma unroll
+        for (uint32_t step = MX4_SEGMENTS / 2; step; step >>= 1)
+            if (first_s[seg + step] <= i) seg += step;
+        return S.cand[((size_t)q * MX4_SEGMENTS + seg) * S.segment + (i - first_s[seg])];
+    };
+    uint32_t key = MX4_KEY_INF;
+    if (n > S.k) key = mx4_kth(bins, n, S.k, [&](uint64_t i) {
+        const float up = at((uint32_t)i).up;
+        return up == up ? mx4_key(up) : MX4_KEY_INF;
+    });
+    const float most = mx4_unkey(key);
+    // rows worth an exact score, collected and scored MX4_FINISH at a time
+    const auto score = [&]() {
+        __syncthreads();
+        const uint32_t m = rows_n;
+        for (uint32_t i0 = 0; i0 < m; i0 += MX4_FINISH / MX4_LANES) {
+            const uint32_t i = i0 + threadIdx.x / MX4_LANES;
+            const uint32_t row = rows_s[min(i, m - 1)];
+            const float s = mx4_exact_score<BITS>(S.E, q, row);
+            mx4_keep_add(K, threadIdx.x % MX4_LANES == 0 && i < m ? mx4_pack(s, row) : MX4_NONE, MX4_FINISH / MX4_LANES);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) rows_n = 0;
+        __syncthreads();
+    };
+    for (uint32_t i0 = 0; i0 < n; i0 += MX4_FINISH) {
+        const uint32_t i = i0 + threadIdx.x;
+        if (i < n) {
+            const Mx4Cand c = at(i);
+            if (!(c.low > most)) rows_s[atomicAdd(&rows_n, 1u)] = c.row;
+        }
+        __syncthreads();
+        const bool full = rows_n > MX4_FINISH || i0 + MX4_FINISH >= n;   // (the same for all threads)
+        if (full) score();
+        else __syncthreads();
     }
     mx4_keep_cut(K);
     const uint32_t got = n_s;
-    const double sq = S.E.qsq[q];
-    const bool dead = !(sq == sq) || (S.E.metric == MX4_COSINE && sq == 0);   // every score is NaN
-    const bool again = !dead && (found > S.cap || got < min((uint64_t)S.k, S.E.rows.n));
+    const bool again = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || got < min((uint64_t)S.k, S.E.rows.n));
     if (threadIdx.x == 0) {
         S.again[q] = again;
         S.ticket[q] = 0;
@@ -832,46 +1022,49 @@ static __global__ __launch_bounds__(512) void k_mx4_select(Mx4Select S) {
     mx4_emit(S, q, keys, got);
 }
 // Queries whose candidates overflowed (many rows as near as the k-th), or were fewer than k: every row scored exactly, `slices`
-// workgroups a query, the last one joins their lists.  It only ever reads memory of its own query and waits for nobody.
+// workgroups a query, the last one joins their lists.  It only ever reads memory of its own query and waits for nobody.  The grid
+// is slices x groups: a group takes every groups-th query, so that the usual case -- nobody's list overflowed -- is a short launch.
 template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ uint32_t n_s, last_s;
     __shared__ uint64_t limit_s;
-    const uint32_t q = blockIdx.y;
-    if (!S.again[q]) return;
-    const Mx4Keep K{keys, &n_s, &limit_s, S.k};
-    if (threadIdx.x == 0) {
-        n_s = 0;
-        limit_s = S.again_limit[q] + 1;
+    for (uint32_t q = blockIdx.y; q < S.nq; q += gridDim.y) {
+        if (!S.again[q]) continue;
+        const Mx4Keep K{keys, &n_s, &limit_s, S.k};
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            n_s = 0;
+            limit_s = S.again_limit[q] + 1;
+        }
+        const uint64_t n = S.E.rows.n, per = (n + S.slices - 1) / S.slices, a = min(n, per * blockIdx.x), b = min(n, a + per);
+        const uint32_t at_once = 512 / MX4_LANES;
+        for (uint64_t r0 = a; r0 < b; r0 += at_once) {
+            const uint64_t row = r0 + threadIdx.x / MX4_LANES;
+            const float s = mx4_exact_score<BITS>(S.E, q, min(row, n - 1));
+            mx4_keep_add(K, threadIdx.x % MX4_LANES == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
+        }
+        mx4_keep_cut(K);
+        uint64_t *mine = S.part + ((size_t)q * S.slices + blockIdx.x) * S.k;
+        for (uint32_t i = threadIdx.x; i < S.k; i += 512) __hip_atomic_store(&mine[i], i < n_s ? keys[i] : MX4_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) last_s = atomicAdd(&S.ticket[q], 1u) == S.slices - 1;
+        __syncthreads();
+        if (!last_s) continue;
+        __threadfence();
+        if (threadIdx.x == 0) {
+            n_s = 0;
+            limit_s = MX4_NONE;
+        }
+        const uint64_t total = (uint64_t)S.slices * S.k;
+        const uint64_t *all = S.part + (size_t)q * total;
+        for (uint64_t i0 = 0; i0 < total; i0 += 512) {
+            const uint64_t i = i0 + threadIdx.x;
+            mx4_keep_add(K, i < total ? __hip_atomic_load(&all[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE, 512);
+        }
+        mx4_keep_cut(K);
+        mx4_emit(S, q, keys, n_s);
     }
-    const uint64_t n = S.E.rows.n, per = (n + S.slices - 1) / S.slices, a = min(n, per * blockIdx.x), b = min(n, a + per);
-    const uint32_t at_once = 512 / MX4_LANES;
-    for (uint64_t r0 = a; r0 < b; r0 += at_once) {
-        const uint64_t row = r0 + threadIdx.x / MX4_LANES;
-        const float s = mx4_exact_score<BITS>(S.E, q, min(row, n - 1));
-        mx4_keep_add(K, threadIdx.x % MX4_LANES == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
-    }
-    mx4_keep_cut(K);
-    uint64_t *mine = S.part + ((size_t)q * S.slices + blockIdx.x) * S.k;
-    for (uint32_t i = threadIdx.x; i < S.k; i += 512) __hip_atomic_store(&mine[i], i < n_s ? keys[i] : MX4_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last_s = atomicAdd(&S.ticket[q], 1u) == S.slices - 1;
-    __syncthreads();
-    if (!last_s) return;
-    __threadfence();
-    if (threadIdx.x == 0) {
-        n_s = 0;
-        limit_s = MX4_NONE;
-    }
-    const uint64_t total = (uint64_t)S.slices * S.k;
-    const uint64_t *all = S.part + (size_t)q * total;
-    for (uint64_t i0 = 0; i0 < total; i0 += 512) {
-        const uint64_t i = i0 + threadIdx.x;
-        mx4_keep_add(K, i < total ? __hip_atomic_load(&all[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE, 512);
-    }
-    mx4_keep_cut(K);
-    mx4_emit(S, q, keys, n_s);
 }
 
 }  // namespace vsg

@@ -23,7 +23,7 @@ struct DeviceScope {
 };
 
 constexpr size_t MAX_DIM = 65536, MAX_ROWS = 0xFFFFFFE0ull, QUERY_BATCH = 256;
-constexpr size_t LDS_BUDGET = 156 * 1024;
+constexpr size_t LDS_BUDGET = 160 * 1024 - 4 * MX4_QUEUE * 16;   // for the queries' operands; the rest is the filter's queues
 
 int elem_size(int type) { return type == VSGPU_F32 ? 4 : (type == VSGPU_F16 || type == VSGPU_BF16 ? 2 : 0); }
 
@@ -63,15 +63,15 @@ struct Plan {
     uint64_t panels, take;       // panels of the table / of the probe
     bool by_row;                 // the probe keeps every row's bound, not one of 16 rows
     uint64_t minima;             // floats per query
-    uint32_t cap, slices;
+    uint32_t segment, slices;    // candidates a list segment holds; workgroups per query that k_mx4_again may need
 };
 static Plan plan_scan(size_t dim, size_t nq, int bits) {
     Plan p{};
     const uint32_t nt = (uint32_t)((nq + 31) / 32);
     p.qtile_bytes = mx4_qtile((uint32_t)dim, bits);
     p.qt = nt >= 3 ? 4 : nt;
-    while (p.qt > 1 && p.qt * (p.qtile_bytes + 128) > LDS_BUDGET) p.qt /= 2;
-    p.global_b = p.qtile_bytes + 128 > LDS_BUDGET;
+    while (p.qt > 1 && p.qt * (p.qtile_bytes + 256) > LDS_BUDGET) p.qt /= 2;
+    p.global_b = p.qtile_bytes + 256 > LDS_BUDGET;
     p.y = (nt + p.qt - 1) / p.qt;
     p.tiles = p.y * p.qt;
     return p;
@@ -81,17 +81,20 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits) {
     p.panels = (n + 31) / 32;
     // Small tables for their k: the probe covers every row.  One bound per 16 rows would put the threshold far above the k-th score.
     p.by_row = n < 64 * k || p.panels <= 64;
+    uint64_t expected;   // candidates
     if (p.by_row) {
         p.take = p.panels;
         p.minima = n;
-        p.cap = (uint32_t)std::min<size_t>(n, 4 * k + 1024);
+        expected = k;
     } else {
-        // a probe of n / div rows leaves about k div candidates per query: div balances their exact scores against the probe's bytes
+        // a probe of n / div rows leaves about k div candidates per query: div balances its bytes against what they cost
         const double div = std::min(64.0, std::max(8.0, std::sqrt(0.15 * (double)n / ((double)nq * (double)k))));
-        p.take = std::min<uint64_t>(p.panels, std::max<uint64_t>((uint64_t)((double)p.panels / div), 2 * k));
+        p.take = std::min<uint64_t>(p.panels, std::max<uint64_t>((uint64_t)((double)p.panels / div), 4 * k));
         p.minima = 2 * p.take;
-        p.cap = (uint32_t)std::min<uint64_t>(n, 6 * k * ((p.panels + p.take - 1) / p.take) + 1024);
+        expected = k * ((p.panels + p.take - 1) / p.take);
     }
+    // four times a segment's share: panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one
+    p.segment = (uint32_t)std::min<uint64_t>((n + MX4_SEGMENTS * 32 - 1) / (MX4_SEGMENTS * 32) * 32, expected * 4 / MX4_SEGMENTS + 64);
     p.slices = k <= 128 ? 32 : 8;
     return p;
 }
@@ -123,26 +126,26 @@ struct TopkBlock {
     uint32_t *counts, *again, *ticket;
     uint64_t *again_limit;
     float *minima;
-    uint2 *cand;
+    Mx4Cand *cand;
     uint64_t *part;
 };
 static TopkBlock take_topk(Layout &L, const Plan &p, size_t nq, size_t k) {
     TopkBlock b;
     b.q = take_queries(L, p);
     b.limit = L.take<float2>(nq);
-    b.counts = L.take<uint32_t>(nq);
+    b.counts = L.take<uint32_t>(nq * MX4_SEGMENTS);
     b.again = L.take<uint32_t>(nq);
     b.ticket = L.take<uint32_t>(nq);
     b.again_limit = L.take<uint64_t>(nq);
     b.minima = L.take<float>(nq * p.minima);
-    b.cand = L.take<uint2>(nq * (size_t)p.cap);
+    b.cand = L.take<Mx4Cand>(nq * (size_t)p.segment * MX4_SEGMENTS);
     b.part = L.take<uint64_t>(nq * p.slices * k);
     return b;
 }
 
 template <int BITS> static int launch_queries(hipStream_t s, const Mx4Queries &Q, uint32_t tiles, int type) {
     const bool wide = (((uintptr_t)Q.x | Q.stride) & 15) == 0;
-    const dim3 g(tiles), b(256);
+    const dim3 g(tiles), b(64 * std::min(16u, Q.kg * 4));
 #define MX4_CASE(T)                                                                                       \
     if (wide) hipLaunchKernelGGL((k_mx4_queries<T, true, BITS>), g, b, 0, s, Q);                          \
     else hipLaunchKernelGGL((k_mx4_queries<T, false, BITS>), g, b, 0, s, Q);
@@ -160,7 +163,7 @@ int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, si
 }
 
 template <int BITS, int QT, int MODE, int NB, bool GB> static int launch_scan5(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
-    const size_t lds = (GB ? 0 : (size_t)QT * P.qtile_bytes) + QT * 128;
+    const size_t lds = (GB ? 0 : (size_t)QT * P.qtile_bytes) + QT * 256 + (MODE == MX4_FILTER ? 4 * MX4_QUEUE * 16 : 0);
     if (lds > 64 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, GB>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(QT >= 4 ? 2 : 4, (160 * 1024) / (lds + 512)));
@@ -197,7 +200,7 @@ int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
         W.claimed = 1;
     }
     const bool wide = (((uintptr_t)W.x | W.stride) & 15) == 0;
-    const dim3 g((unsigned)((W.m + 31) / 32)), b(256);
+    const dim3 g((unsigned)((W.m + 31) / 32)), b(64 * std::min(16u, W.rows.ks));
 #define MX4_CASE(T)                                                                \
     if (wide) hipLaunchKernelGGL((k_mx4_write<T, true>), g, b, 0, s, W);           \
     else hipLaunchKernelGGL((k_mx4_write<T, false>), g, b, 0, s, W);
@@ -210,11 +213,19 @@ int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
 }
 int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
     if (R.m == 0) return VSGPU_OK;
-    const uint64_t work = R.m * ((R.rows.dim + 7) / 8);
-    const dim3 g((unsigned)std::min<uint64_t>((work + 255) / 256, (uint64_t)cus * 32)), b(256);
-    if (type == VSGPU_F32) hipLaunchKernelGGL((k_mx4_read<MX4_F32>), g, b, 0, s, R);
-    else if (type == VSGPU_F16) hipLaunchKernelGGL((k_mx4_read<MX4_F16>), g, b, 0, s, R);
-    else hipLaunchKernelGGL((k_mx4_read<MX4_BF16>), g, b, 0, s, R);
+    const uint32_t per_row = (R.rows.dim + 7) / 8, recip = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
+    // about 1024 threads' work a workgroup, fewer rows when there are not enough of them to fill the chip
+    uint64_t rows = std::max<uint64_t>(1, 1024 / per_row);
+    rows = std::max<uint64_t>(std::min<uint64_t>(rows, R.m / ((uint64_t)cus * 8)), std::max<uint64_t>(1, std::min<uint64_t>(256 / per_row, R.m)));
+    const bool wide = (((uintptr_t)R.out | R.stride) & 15) == 0;
+    const dim3 g((unsigned)((R.m + rows - 1) / rows)), b(256);
+#define MX4_CASE(T)                                                                                                           \
+    if (wide) hipLaunchKernelGGL((k_mx4_read<T, true>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);                       \
+    else hipLaunchKernelGGL((k_mx4_read<T, false>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);
+    if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
+    else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
+    else { MX4_CASE(MX4_BF16) }
+#undef MX4_CASE
     HIPCHK(hipGetLastError());
     return VSGPU_OK;
 }
@@ -243,7 +254,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     L.base = static_cast<char *>(ws);
     const TopkBlock b = take_topk(L, p, nq, k);
     if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
-    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.counts, nq);
+    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.counts, nq * MX4_SEGMENTS);
     if (rc) return rc;
     Mx4Scan P{};
     P.rows = R;
@@ -259,7 +270,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.limit = b.limit;
     P.counts = b.counts;
     P.cand = b.cand;
-    P.cap = p.cap;
+    P.segment = p.segment;
     P.slack = mx4_slack(R.ks);
     rc = p.by_row ? launch_scan<MX4_PROBE_ROWS>(s, P, p, bits, cus) : launch_scan<MX4_PROBE>(s, P, p, bits, cus);
     if (rc) return rc;
@@ -275,7 +286,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
     S.nq = (uint32_t)nq;
     S.k = (uint32_t)k;
-    S.cap = p.cap;
+    S.segment = p.segment;
     S.counts = b.counts;
     S.cand = b.cand;
     S.again = b.again;
@@ -285,12 +296,14 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.slices = p.slices;
     S.part = b.part;
     S.ticket = b.ticket;
-    const dim3 rg((unsigned)std::max<size_t>(1, std::min<size_t>((p.cap + 15) / 16, std::max<size_t>(8, (size_t)cus * 8 / nq))), (unsigned)nq);
-    if (bits == 6) hipLaunchKernelGGL((k_mx4_rerank<6>), rg, dim3(256), 0, s, S.E, b.counts, b.cand, p.cap);
-    else hipLaunchKernelGGL((k_mx4_rerank<4>), rg, dim3(256), 0, s, S.E, b.counts, b.cand, p.cap);
-    hipLaunchKernelGGL(k_mx4_select, dim3((unsigned)nq), dim3(512), 0, s, S);
-    if (bits == 6) hipLaunchKernelGGL((k_mx4_again<6>), dim3(p.slices, (unsigned)nq), dim3(512), 0, s, S);
-    else hipLaunchKernelGGL((k_mx4_again<4>), dim3(p.slices, (unsigned)nq), dim3(512), 0, s, S);
+    const dim3 ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
+    if (bits == 6) {
+        hipLaunchKernelGGL((k_mx4_finish<6>), dim3((unsigned)nq), dim3(MX4_FINISH), 0, s, S);
+        hipLaunchKernelGGL((k_mx4_again<6>), ag, dim3(512), 0, s, S);
+    } else {
+        hipLaunchKernelGGL((k_mx4_finish<4>), dim3((unsigned)nq), dim3(MX4_FINISH), 0, s, S);
+        hipLaunchKernelGGL((k_mx4_again<4>), ag, dim3(512), 0, s, S);
+    }
     HIPCHK(hipGetLastError());
     return VSGPU_OK;
 }
