@@ -1,8 +1,17 @@
 // mx4_host.hpp -- what the MXFP4 translation unit gives the table code in vsgpu.hip.
 #pragma once
-#include "mx4_kernels.hpp"
+#include "mx4_common.hpp"
 
 namespace vsg {
+struct Mx4Write;
+struct Mx4Read;
+enum { MX4_SHARED = 0, MX4_GLOBAL = 1, MX4_REGS = 2 };   // where a scan's waves take the queries' operands from
+struct Mx4ScanShape {
+    int src, cus;
+    uint32_t qt, y;   // query tiles a wave, workgroups side by side (each with groups x qt tiles)
+};
+int mx4_scan4(hipStream_t s, int mode, const Mx4Scan &P, const Mx4ScanShape &shape);
+int mx4_scan6(hipStream_t s, int mode, const Mx4Scan &P, const Mx4ScanShape &shape);
 Mx4Rows mx4_rows_of(const void *base, size_t n, size_t dim);
 int mx4_launch_write(hipStream_t s, const Mx4Write &W, int type);
 int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus);

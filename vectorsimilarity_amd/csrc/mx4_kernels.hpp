@@ -1,57 +1,9 @@
-// mx4_kernels.hpp -- rows in the OCP microscaling format MXFP4: writing, reading back, scoring, the k best (gfx950).
-//
-// The arithmetic.  A block of 32 elements shares E = clamp(floor(log2 max|x|) - 2, -127, 125); its elements are E2M1 codes of
-// x 2^-E, nearest with ties to even, saturating at 6.  The scale byte is E + 127; a block that holds an infinity or a NaN has
-// byte 255 and is NaN as a whole.  Queries are rounded the same way to E2M1 (4 bits) or E2M3 (6 bits, saturating at 7.5).
-//   dot(q, x) = sum_blocks 2^(Eq + Ex) sum_j q_j x_j      IP 1 - dot    L2 |q|^2 + |x|^2 - 2 dot    Cosine 1 - dot / (|q| |x|)
-// (|.| of the rounded vectors).  A block's inner sum is a multiple of 1/16 below 2^11, so it is exact in fp32, whatever the order.
-// E2M3 and not E4M3 for the finer queries: at a block's own scale both keep four digits of its larger elements, the matrix
-// instruction takes six-bit operands at the four-bit rate, and it adds their products without loss (measured over random blocks:
-// within 2^-23.4 of sum|q x|, where E4M3 products came back up to 3e-4 of the largest product off).
-//
-// The layout.  32 rows form a panel, laid out as v_mfma_scale_f32_32x32x64_f8f6f4 takes its operand, so that a wave's load of one
-// k-step (64 elements of 32 rows) is one contiguous KiB straight into registers, without a pass through LDS:
-//   codes  [ks = ceil(dim / 64)][half][row][16 bytes]    element j of block 2 step + half in byte j / 2, low nibble first
-//   scales [kg = ceil(ks / 4)][half][row][4 bytes]       byte i: k-step 4 group + i; one dword feeds four instructions (opsel)
-//   norms  [32] fp32                                     |x|, rounded once from 64 bits; the sign bit is free (k_mx4_claim)
-// 768 elements: 412 bytes a row.
+// mx4_kernels.hpp -- MXFP4 rows: writing, reading back, rounding queries, exact scores, the k best (mx4_common.hpp has the format;
+// mx4_scan_kernels.hpp the passes over the table).
 #pragma once
-#include <hip/hip_runtime.h>
-#include <stdint.h>
+#include "mx4_common.hpp"
 
 namespace vsg {
-
-typedef int mx4_i4 __attribute__((ext_vector_type(4)));
-typedef int mx4_i8 __attribute__((ext_vector_type(8)));
-typedef float mx4_f16 __attribute__((ext_vector_type(16)));
-typedef float mx4_f4 __attribute__((ext_vector_type(4)));
-typedef unsigned int mx4_u4 __attribute__((ext_vector_type(4)));
-typedef unsigned int mx4_u2 __attribute__((ext_vector_type(2)));
-typedef unsigned int mx4_u6 __attribute__((ext_vector_type(6)));
-typedef float mx4_f2 __attribute__((ext_vector_type(2)));
-typedef float mx4_f32 __attribute__((ext_vector_type(32)));
-
-enum { MX4_F32 = 0, MX4_BF16 = 2, MX4_F16 = 3 };   // VSGPU_F32, _BF16, _F16
-enum { MX4_L2 = 0, MX4_IP = 1, MX4_COSINE = 2 };
-
-__host__ __device__ inline uint32_t mx4_steps(uint32_t dim) { return (dim + 63) / 64; }
-__host__ __device__ inline uint32_t mx4_groups(uint32_t dim) { return (mx4_steps(dim) + 3) / 4; }
-__host__ __device__ inline uint32_t mx4_panel(uint32_t dim) { return mx4_steps(dim) * 1024 + mx4_groups(dim) * 256 + 128; }
-// a 32-query tile of the query block: operand bytes of every k-step (16 a lane; E2M3: 8 more a lane behind all of them), scales
-__host__ __device__ inline uint32_t mx4_qtile(uint32_t dim, int bits) { return mx4_steps(dim) * (bits == 6 ? 1536 : 1024) + mx4_groups(dim) * 256; }
-
-// where rows are: one block of panels, or slabs of 2^shift panels each
-struct Mx4Rows {
-    char *base;
-    char *const *slabs;
-    uint32_t shift;
-    uint32_t dim, ks, kg, panel;
-    uint64_t n;
-    __device__ char *at(uint64_t p) const {
-        if (slabs) return slabs[p >> shift] + (p & ((1u << shift) - 1)) * (size_t)panel;
-        return base + p * panel;
-    }
-};
 
 __device__ __forceinline__ double mx4_pow2(int e) {   // 2^e, |e| <= 1000
     return __longlong_as_double((long long)(e + 1023) << 52);
@@ -372,306 +324,6 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) 
     }
 }
 
-// ---------------------------------------------------------------------------------------------------------------- scan
-// How far a matrix-core dot may be from the exact one, over |q| |x|: each of the ks instructions adds its 64 products to the sum
-// so far within 2^-22 of what it adds up (measured 2^-23.4); eight more of the same for the rounded norms and the comparison's own
-// arithmetic, and twice all of it.
-__host__ __device__ inline float mx4_slack(uint32_t ks) { return (float)(ks + 8) * 4.76837158203125e-7f; }
-constexpr float MX4_EPS = 1.9073486328125e-6f;    // 2^-19, of |q|^2 + |x|^2 (L2): the same for sums of squares
-constexpr float MX4_STEP = 9.5367431640625e-7f;   // 2^-20: what rounding a score to fp32 may move it, and more
-constexpr float MX4_TINY = 1e-36f;                // L2 scores below it: fp32 has no digits left to rank them by
-constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: the product of the norms may leave fp32
-
-enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
-constexpr uint32_t MX4_SEGMENTS = 32;             // a query's candidate list: one counter for every panel modulo 32
-constexpr uint32_t MX4_QUEUE = 256;               // survivors a wave collects in LDS before they go out
-struct Mx4Cand {
-    uint32_t row;
-    float low, up;                // bounds of its score
-    uint32_t pad;
-};
-struct Mx4Scan {
-    Mx4Rows rows;
-    const char *tiles;            // this launch's query tiles start at blockIdx.y * QT
-    uint32_t qtile_bytes;
-    uint32_t nq, metric;
-    const float *qnorm;
-    // which panels: n_take of them, number i is i * n_panels / n_take
-    uint64_t n_panels, n_take;
-    float *minima;                // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row
-    uint64_t minima_stride;
-    const float2 *limit;          // FILTER: {alpha, beta} of each query
-    uint32_t *counts;             // FILTER: [nq][MX4_SEGMENTS]
-    Mx4Cand *cand;                // [nq][MX4_SEGMENTS][segment]
-    uint32_t segment;
-    float *out;                   // DENSE: [nq][out_stride]
-    uint64_t out_stride;
-    float slack;
-};
-
-// the score's bounds from a matrix-core dot and the two norms
-__device__ __forceinline__ void mx4_bounds(uint32_t metric, float d, float x, float y, float slack, float &low, float &up) {
-    float s, e;
-    if (metric == MX4_L2) {
-        const float sum = __fmaf_rn(x, x, y * y);
-        s = __fmaf_rn(-2.f, d, sum);
-        e = __fmaf_rn(2.f * slack * x, y, __fmaf_rn(MX4_EPS, sum, MX4_TINY));
-    } else if (metric == MX4_IP) {
-        s = 1.f - d;
-        e = __fmaf_rn(slack * x, y, MX4_STEP * fmaxf(1.f, fabsf(s)));
-    } else {
-        s = 1.f - d / x / y;
-        e = slack + MX4_STEP;
-        if (x < MX4_SHORT || y < MX4_SHORT) s = 1.f, e = 1.001f;
-    }
-    low = s - e;
-    up = s + e;
-}
-
-// one operand pair and its scales; the table is the A operand (results: a lane one query, its registers 16 rows) or, for dense
-// scores, the B operand (a lane one row: stores along a query's line)
-template <int BITS, bool SWAP, int I> __device__ __forceinline__ mx4_f16 mx4_mma(mx4_i8 t, mx4_i8 q, mx4_f16 c, int st, int sq) {
-    constexpr int FQ = BITS == 6 ? 2 : 4;
-    if constexpr (SWAP) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(q, t, c, FQ, 4, I, sq, I, st);
-    else return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(t, q, c, 4, FQ, I, st, I, sq);
-}
-struct Mx4Chunk {   // four k-steps of a panel
-    mx4_i4 a[4];
-    int sc;
-};
-__device__ __forceinline__ void mx4_fetch(Mx4Chunk &c, const char *panel, uint32_t g, uint32_t ks, int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t s = min(4 * g + i, ks - 1);   // (past the last step: the same bytes again, never used)
-        c.a[i] = __builtin_nontemporal_load(reinterpret_cast<const mx4_i4 *>(panel + (size_t)s * 1024) + lane);
-    }
-    c.sc = __builtin_nontemporal_load(reinterpret_cast<const int *>(panel + (size_t)ks * 1024 + g * 256) + lane);
-}
-template <int BITS, bool SWAP, int QT, int I>
-__device__ __forceinline__ void mx4_step(mx4_f16 *acc, const Mx4Chunk &c, const char *lds, uint32_t g, uint32_t ks, uint32_t qtile_bytes, const int *sq, int lane) {
-    const uint32_t s = 4 * g + I;
-    mx4_i8 t{c.a[I][0], c.a[I][1], c.a[I][2], c.a[I][3], 0, 0, 0, 0};
-#pragma unroll
-    for (int q = 0; q < QT; q++) {
-        const char *b = lds + q * qtile_bytes;
-        const mx4_i4 lo = reinterpret_cast<const mx4_i4 *>(b + s * 1024)[lane];
-        mx4_i8 f{lo[0], lo[1], lo[2], lo[3], 0, 0, 0, 0};
-        if constexpr (BITS == 6) {
-            const mx4_u2 hi = reinterpret_cast<const mx4_u2 *>(b + ks * 1024 + s * 512)[lane];
-            f[4] = (int)hi[0];
-            f[5] = (int)hi[1];
-        }
-        acc[q] = mx4_mma<BITS, SWAP, I>(t, f, acc[q], c.sc, sq[q]);
-    }
-}
-// a candidate into its query's list (segments of counters: one counter would make all waves wait in line for it)
-__device__ __forceinline__ void mx4_admit(const Mx4Scan &P, uint32_t q, uint32_t row, float d, float x, float y) {
-    const uint32_t seg = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
-    const uint32_t at = atomicAdd(&P.counts[seg], 1u);
-    if (at < P.segment) {
-        Mx4Cand c{row, 0.f, 0.f, 0u};
-        mx4_bounds(P.metric, d, x, y, P.slack, c.low, c.up);
-        P.cand[(size_t)seg * P.segment + at] = c;
-    }
-}
-
-// A wave takes whole panels, one after the other, every wave of the grid in turn; the queries' operands stay in LDS.  NB chunks of
-// the panel (256 elements each) are in flight: chunk g of the next panel is requested as soon as chunk g of this one has gone into
-// the matrix cores.  Panels of more than 4 chunks go through the same four buffers several times.
-template <int BITS, int QT, int MODE, int NB, bool GB> static __global__ __launch_bounds__(256, 2) void k_mx4_scan(Mx4Scan P) {
-    extern __shared__ char shared[];
-    constexpr bool SWAP = MODE == MX4_DENSE;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const uint32_t q0 = blockIdx.y * QT * 32;
-    const uint32_t ks = P.rows.ks, kg = P.rows.kg;
-    // (rows too wide for that, GB: the operands are read from the query block itself, through the caches)
-    const char *lds = GB ? P.tiles + (size_t)blockIdx.y * QT * P.qtile_bytes : shared;
-    float *yn_s = reinterpret_cast<float *>(shared + (GB ? 0 : QT * P.qtile_bytes));
-    float *yr_s = yn_s + QT * 32;   // 1 / |q|
-    mx4_u4 *queue = reinterpret_cast<mx4_u4 *>(yr_s + QT * 32) + wave * MX4_QUEUE;   // FILTER: {query, row, dot, |x|}
-    uint32_t queued = 0;
-    if constexpr (!GB) {
-        const mx4_u4 *src = reinterpret_cast<const mx4_u4 *>(P.tiles + (size_t)blockIdx.y * QT * P.qtile_bytes);
-        const uint32_t n16 = QT * P.qtile_bytes / 16;
-        for (uint32_t i = threadIdx.x; i < n16; i += 256) reinterpret_cast<mx4_u4 *>(shared)[i] = src[i];
-    }
-    for (uint32_t i = threadIdx.x; i < QT * 32; i += 256) {
-        const float y = P.qnorm[q0 + i];   // (padded to whole tiles)
-        yn_s[i] = y;
-        yr_s[i] = 1.f / y;
-    }
-    __syncthreads();
-    const uint32_t sc_at = ks * (BITS == 6 ? 1536 : 1024);
-    float alpha[QT], beta[QT], qn[QT], qr[QT];
-#pragma unroll
-    for (int q = 0; q < QT; q++) {
-        const uint32_t me = q0 + q * 32 + col;
-        if constexpr (MODE == MX4_FILTER) {
-            const float2 l = me < P.nq ? P.limit[me] : make_float2(0.f, __uint_as_float(0x7F800000u));
-            alpha[q] = l.x;
-            beta[q] = l.y;
-        }
-        qn[q] = yn_s[q * 32 + col];
-        if constexpr (MODE == MX4_PROBE || MODE == MX4_PROBE_ROWS) qr[q] = yr_s[q * 32 + col];
-    }
-    bool shorts = false;   // DENSE, Cosine: queries whose reciprocal norm is no use
-    if constexpr (MODE == MX4_DENSE) {
-        for (int i = 0; i < QT * 32; i++) shorts |= yn_s[i] < MX4_SHORT && yn_s[i] > 0.f;
-    }
-    const uint64_t W = (uint64_t)gridDim.x * 4;
-    uint64_t w = (uint64_t)blockIdx.x * 4 + wave;
-    if (w >= P.n_take) return;
-    const auto panel_of = [&](uint64_t i) { return P.n_take == P.n_panels ? i : i * P.n_panels / P.n_take; };
-    // the wave's queue, 64 survivors at a time
-    const auto flush = [&]() {
-        for (uint32_t i = lane; i < queued; i += 64) {
-            const mx4_u4 e = queue[i];
-            mx4_admit(P, e[0], e[1], __uint_as_float(e[2]), __uint_as_float(e[3]), yn_s[e[0] - q0]);
-        }
-        queued = 0;
-    };
-    Mx4Chunk buf[NB];
-    const char *panel = P.rows.at(panel_of(w));
-#pragma unroll
-    for (int g = 0; g < NB; g++)
-        if (g < (int)kg) mx4_fetch(buf[g], panel, g, ks, lane);
-    for (; w < P.n_take; w += W) {
-        const uint64_t p = panel_of(w), wn = w + W;
-        const char *next = wn < P.n_take ? P.rows.at(panel_of(wn)) : panel;   // (at the end: this panel again, never used)
-        mx4_f16 acc[QT];
-#pragma unroll
-        for (int q = 0; q < QT; q++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) acc[q][v] = 0.f;
-        mx4_f4 nrm[4];
-        float nx = 0.f;
-        if constexpr (SWAP) nx = reinterpret_cast<const float *>(panel + P.rows.panel - 128)[col];
-        else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) nrm[i] = reinterpret_cast<const mx4_f4 *>(panel + P.rows.panel - 128)[2 * i + half];
-        }
-        for (uint32_t g0 = 0; g0 < kg; g0 += NB) {
-#pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const uint32_t g = g0 + j;
-                if (g >= kg) break;
-                int sq[QT];
-#pragma unroll
-                for (int q = 0; q < QT; q++) sq[q] = reinterpret_cast<const int *>(lds + q * P.qtile_bytes + sc_at + g * 256)[lane];
-                mx4_step<BITS, SWAP, QT, 0>(acc, buf[j], lds, g, ks, P.qtile_bytes, sq, lane);
-                if (4 * g + 1 < ks) mx4_step<BITS, SWAP, QT, 1>(acc, buf[j], lds, g, ks, P.qtile_bytes, sq, lane);
-                if (4 * g + 2 < ks) mx4_step<BITS, SWAP, QT, 2>(acc, buf[j], lds, g, ks, P.qtile_bytes, sq, lane);
-                if (4 * g + 3 < ks) mx4_step<BITS, SWAP, QT, 3>(acc, buf[j], lds, g, ks, P.qtile_bytes, sq, lane);
-                // the buffer's next contents: NB chunks on in this panel, or the chunk of the next panel that it takes
-                if (g + NB < kg) mx4_fetch(buf[j], panel, g + NB, ks, lane);
-                else mx4_fetch(buf[j], next, j, ks, lane);
-            }
-        }
-        const uint64_t row0 = p * 32;
-        if constexpr (MODE == MX4_DENSE) {
-            const uint64_t row = row0 + col;
-            float *line = P.out + (q0 + 4 * half) * P.out_stride + row;
-            const float *yl = yn_s + 4 * half;
-            const float c0 = P.metric == MX4_L2 ? nx * nx : 1.f, rx = 1.f / nx;
-            const bool divide = P.metric == MX4_COSINE && (shorts || __any(nx < MX4_SHORT && nx > 0.f));
-            const bool whole = row0 + 32 <= P.rows.n && q0 + QT * 32 <= P.nq;
-#pragma unroll
-            for (int q = 0; q < QT; q++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const mx4_f4 y4 = *reinterpret_cast<const mx4_f4 *>(yl + q * 32 + 8 * i), r4 = *reinterpret_cast<const mx4_f4 *>(yl + (QT + q) * 32 + 8 * i);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float d = acc[q][4 * i + j], y = y4[j];
-                        float s;
-                        if (P.metric == MX4_L2) s = __fmaf_rn(-2.f, d, __fmaf_rn(y, y, c0));
-                        else if (P.metric == MX4_IP) s = 1.f - d;
-                        else if (!divide) s = 1.f - d * rx * r4[j];
-                        else s = 1.f - d / nx / y;
-                        const uint32_t me = q * 32 + 8 * i + j;
-                        if (whole || (q0 + me + 4 * half < P.nq && row < P.rows.n)) __builtin_nontemporal_store(s, line);
-                        line += j < 3 ? P.out_stride : 5 * P.out_stride;
-                    }
-                }
-        } else if constexpr (MODE == MX4_FILTER) {
-            // a survivor when its score may be at or below the query's threshold: dot >= alpha |x| + beta + (L2: |x|^2 / 2)
-            float base[16];
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float x = nrm[v >> 2][v & 3];
-                base[v] = P.metric == MX4_L2 ? 0.5f * (1.f - MX4_EPS) * x * x : 0.f;
-                if (P.metric == MX4_COSINE && x < MX4_SHORT) base[v] = x > 0.f ? -__uint_as_float(0x7F800000u) : __uint_as_float(0x7F800000u);   // (zero: score NaN)
-            }
-#pragma unroll
-            for (int q = 0; q < QT; q++) {
-                bool any = false;
-#pragma unroll
-                for (int v = 0; v < 16; v++) any |= acc[q][v] >= __fmaf_rn(alpha[q], nrm[v >> 2][v & 3], base[v] + beta[q]);
-                if (__any(any)) {
-                    const uint32_t me = q0 + q * 32 + col;
-                    uint32_t total = 0;
-#pragma unroll
-                    for (int v = 0; v < 16; v++) {
-                        const bool hit = acc[q][v] >= __fmaf_rn(alpha[q], nrm[v >> 2][v & 3], base[v] + beta[q]);
-                        total += __builtin_popcountll(__ballot(hit));
-                    }
-                    if (queued + total > MX4_QUEUE) flush();
-                    const bool direct = total > MX4_QUEUE;   // a panel full of survivors
-#pragma unroll
-                    for (int v = 0; v < 16; v++) {
-                        const float x = nrm[v >> 2][v & 3], d = acc[q][v];
-                        const uint64_t row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
-                        const bool hit = d >= __fmaf_rn(alpha[q], x, base[v] + beta[q]) && row < P.rows.n;
-                        const uint64_t b = __ballot(hit);
-                        if (b == 0) continue;
-                        if (direct) {
-                            if (hit) mx4_admit(P, me, (uint32_t)row, d, x, qn[q]);
-                        } else {
-                            if (hit) queue[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u))] =
-                                mx4_u4{me, (uint32_t)row, __float_as_uint(d), __float_as_uint(x)};
-                            queued += __builtin_popcountll(b);
-                        }
-                    }
-                }
-            }
-        } else {
-            const float inf = __uint_as_float(0x7F800000u);
-            float rx[16];
-            if (P.metric == MX4_COSINE) {
-#pragma unroll
-                for (int v = 0; v < 16; v++) rx[v] = __builtin_amdgcn_rcpf(nrm[v >> 2][v & 3]);
-            }
-#pragma unroll
-            for (int q = 0; q < QT; q++) {
-                const uint32_t me = q0 + q * 32 + col;
-                float best = inf;
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const float x = nrm[v >> 2][v & 3], d = acc[q][v];
-                    const uint64_t row = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    float u;   // an upper bound of the score (mx4_bounds, with reciprocals: two more roundings, in the slack)
-                    if (P.metric == MX4_L2) u = __fmaf_rn(2.f * P.slack * qn[q], x, __fmaf_rn(-2.f, d, __fmaf_rn(1.f + MX4_EPS, __fmaf_rn(x, x, qn[q] * qn[q]), MX4_TINY)));
-                    else if (P.metric == MX4_IP) u = __fmaf_rn(P.slack * qn[q], x, 1.f - d) + MX4_STEP * fmaxf(1.f, fabsf(1.f - d));
-                    else {
-                        u = 1.f - d * rx[v] * qr[q] + (P.slack + MX4_STEP);
-                        if (x < MX4_SHORT || qn[q] < MX4_SHORT) u = x > 0.f ? 2.001f : inf;
-                    }
-                    if (row >= P.rows.n || !(u == u)) u = inf;
-                    if constexpr (MODE == MX4_PROBE_ROWS) {
-                        if (me < P.nq && row < P.rows.n) P.minima[me * P.minima_stride + row] = u;
-                    }
-                    best = fminf(best, u);
-                }
-                if constexpr (MODE == MX4_PROBE) {
-                    if (me < P.nq) P.minima[me * P.minima_stride + 2 * w + half] = best;
-                }
-            }
-        }
-        panel = next;
-    }
-    if constexpr (MODE == MX4_FILTER) flush();
-}
-
 // ---------------------------------------------------------------------------------------------------------------- threshold
 __device__ __forceinline__ uint32_t mx4_key(float f) {   // order-preserving; NaN is never passed
     const uint32_t u = __float_as_uint(f);
@@ -770,11 +422,21 @@ struct Mx4Threshold {
 __device__ __forceinline__ bool mx4_dead(uint32_t metric, double sq) { return !(sq == sq) || (metric == MX4_COSINE && sq == 0); }
 // tau = a little above the k-th smallest upper bound (each of different rows, so at least k rows are at or below it), then what the
 // filter compares against
+constexpr uint32_t MX4_STAGED = 16384;
 static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
     __shared__ Mx4Bins bins;
+    __shared__ uint32_t staged[MX4_STAGED];   // (up to 2^14 bounds are read once)
     const uint32_t q = blockIdx.x;
     const float *m = T.minima + q * T.stride;
-    const uint32_t key = T.k > T.count ? MX4_KEY_INF : mx4_kth(bins, T.count, T.k, [&](uint64_t i) { return mx4_key(m[i]); });
+    uint32_t key = MX4_KEY_INF;
+    if (T.k <= T.count) {
+        if (T.count <= MX4_STAGED) {
+            for (uint32_t i = threadIdx.x; i < T.count; i += 1024) staged[i] = mx4_key(m[i]);
+            key = mx4_kth(bins, T.count, T.k, [&](uint64_t i) { return staged[i]; });
+        } else {
+            key = mx4_kth(bins, T.count, T.k, [&](uint64_t i) { return mx4_key(m[i]); });
+        }
+    }
     if (threadIdx.x) return;
     const float inf = __uint_as_float(0x7F800000u);
     const float tau = mx4_unkey(key), yn = T.qnorm[q];
@@ -801,13 +463,10 @@ struct Mx4Exact {
     uint32_t qtile_bytes, metric;
     const double *qsq;
 };
-__device__ __forceinline__ float mx4_code6(const uint32_t *w, int j) {   // element j of six dwords
-    const int bit = 6 * j;
-    uint32_t c = w[bit / 32] >> (bit % 32);
-    if (bit % 32 > 26) c |= w[bit / 32 + 1] << (32 - bit % 32);
-    const uint32_t m = c & 31u;
-    const float v = m < 16 ? (float)m : (m < 24 ? (float)(2 * m - 16) : (float)(4 * m - 64));
-    return (c & 32u ? -v : v) * 0.125f;
+template <typename F> __device__ __forceinline__ void mx4_unpack8(uint32_t codes, F use) {   // eight E2M1 elements
+    const mx4_f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 1);
+    const mx4_f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
+    use(0, a[0]), use(1, a[1]), use(2, b[0]), use(3, b[1]), use(4, c[0]), use(5, c[1]), use(6, d[0]), use(7, d[1]);
 }
 // this lane's share of a row's sums: blocks first, first + by, ...   In a block the sums are whole numbers (of 1/16): exact.
 template <int BITS> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact &E, const char *tile, uint32_t col, const char *panel, uint32_t r,
@@ -821,20 +480,21 @@ template <int BITS> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact 
         const uint32_t bx = (uint8_t)panel[(size_t)E.rows.ks * 1024 + (s >> 2) * 256 + ra * 4 + (s & 3)];
         const mx4_u4 lo = *reinterpret_cast<const mx4_u4 *>(tile + (size_t)s * 1024 + qa * 16);
         const uint32_t bq = (uint8_t)tile[(size_t)E.rows.ks * (BITS == 6 ? 1536 : 1024) + (s >> 2) * 256 + qa * 4 + (s & 3)];
-        uint32_t w[6] = {lo[0], lo[1], lo[2], lo[3], 0, 0};
+        float d = 0, sq = 0;
+        mx4_f32 qv;
         if constexpr (BITS == 6) {
             const mx4_u2 hi = *reinterpret_cast<const mx4_u2 *>(tile + (size_t)E.rows.ks * 1024 + (size_t)s * 512 + qa * 8);
-            w[4] = hi[0];
-            w[5] = hi[1];
-        }
-        float d = 0, sq = 0;
+            qv = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(mx4_u6{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1]}, 1.f);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const float xv = mx4_code_value((x[j / 8] >> (4 * (j % 8))) & 15u);
-            const float qv = BITS == 6 ? mx4_code6(w, j) : mx4_code_value((w[j / 8] >> (4 * (j % 8))) & 15u);
-            d = __fmaf_rn(xv, qv, d);
-            sq = __fmaf_rn(xv, xv, sq);
+            for (int w = 0; w < 4; w++) mx4_unpack8(lo[w], [&](int j, float v) { qv[8 * w + j] = v; });
         }
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            mx4_unpack8(x[w], [&](int j, float v) {
+                d = __fmaf_rn(v, qv[8 * w + j], d);
+                sq = __fmaf_rn(v, v, sq);
+            });
         const double nan = __builtin_nan("");
         dot += bx == 255 || bq == 255 ? nan : (double)d * mx4_pow2((int)bx + (int)bq - 254);
         xx += bx == 255 ? nan : (double)sq * mx4_pow2(2 * (int)bx - 254);
@@ -845,23 +505,23 @@ __device__ __forceinline__ float mx4_final(uint32_t metric, double dot, double x
     if (metric == MX4_L2) return (float)(qq + xx - 2.0 * dot);
     return (float)(1.0 - dot / (sqrt(qq) * sqrt(xx)));
 }
-constexpr int MX4_LANES = 16;   // lanes on one row in the exact kernels
-template <int BITS> __device__ __forceinline__ float mx4_exact_score(const Mx4Exact &E, uint32_t q, uint64_t row) {
+// lanes on one row: one for each of its blocks, 4 to 32
+__host__ __device__ inline uint32_t mx4_row_lanes(uint32_t ks) { return ks <= 2 ? 4u : (ks <= 4 ? 8u : (ks <= 8 ? 16u : 32u)); }
+template <int BITS> __device__ __forceinline__ float mx4_exact_score(const Mx4Exact &E, uint32_t q, uint64_t row, uint32_t lanes) {
     double dot, xx;
-    mx4_row_sums<BITS>(E, E.tiles + (size_t)(q >> 5) * E.qtile_bytes, q & 31, E.rows.at(row >> 5), (uint32_t)(row & 31), threadIdx.x % MX4_LANES, MX4_LANES, dot, xx);
-#pragma unroll
-    for (int o = MX4_LANES / 2; o; o >>= 1) {
+    mx4_row_sums<BITS>(E, E.tiles + (size_t)(q >> 5) * E.qtile_bytes, q & 31, E.rows.at(row >> 5), (uint32_t)(row & 31), threadIdx.x & (lanes - 1), lanes, dot, xx);
+    for (int o = (int)lanes / 2; o; o >>= 1) {
         dot += __shfl_xor(dot, o);
         xx += __shfl_xor(xx, o);
     }
     return mx4_final(E.metric, dot, xx, E.qsq[q]);
 }
 // rows first .. first + m - 1, or ids[0 .. m)
-template <int BITS> static __global__ __launch_bounds__(256) void k_mx4_exact_rows(Mx4Exact E, uint32_t nq, const uint32_t *ids, uint64_t first, uint64_t m, float *out) {
-    const uint32_t q = blockIdx.y;
-    for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / MX4_LANES; i < m; i += (uint64_t)gridDim.x * (256 / MX4_LANES)) {
-        const float s = mx4_exact_score<BITS>(E, q, ids ? ids[i] : first + i);
-        if (threadIdx.x % MX4_LANES == 0) out[q * m + i] = s;
+template <int BITS> static __global__ __launch_bounds__(256) void k_mx4_exact_rows(Mx4Exact E, const uint32_t *ids, uint64_t first, uint64_t m, float *out) {
+    const uint32_t lanes = mx4_row_lanes(E.rows.ks), at_once = 256 / lanes, me = threadIdx.x / lanes;
+    for (uint64_t i = (uint64_t)blockIdx.x * at_once + me; i < m; i += (uint64_t)gridDim.x * at_once) {
+        const float s = mx4_exact_score<BITS>(E, 0, ids ? ids[i] : first + i, lanes);
+        if ((threadIdx.x & (lanes - 1)) == 0) out[i] = s;
     }
 }
 
@@ -924,6 +584,8 @@ struct Mx4Select {
     uint32_t nq, k, segment;
     const uint32_t *counts;     // [nq][MX4_SEGMENTS]
     const Mx4Cand *cand;
+    const float *minima, *qnorm;   // DENSE: [nq][n] upper bounds
+    float slack;
     uint32_t *again;            // [nq]: 1 = the list did not hold the answer: k_mx4_again
     uint64_t *again_limit;      // [nq] ... which then needs nothing above this
     int64_t *ids;               // [nq][k]
@@ -941,11 +603,14 @@ __device__ __forceinline__ void mx4_emit(const Mx4Select &S, uint32_t q, const u
     }
 }
 // One workgroup a query: of its candidates only those whose lower bound is at or below the k-th smallest upper bound (little more
-// than k) are scored exactly, 16 lanes a row; then sorted.
+// than k) are scored exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds
+// the probe's.
 constexpr uint32_t MX4_FINISH = 1024;
-template <int BITS> static __global__ __launch_bounds__(1024) void k_mx4_finish(Mx4Select S) {
+constexpr uint32_t MX4_LISTED = 6144;   // candidates kept in LDS; more are read from memory every time
+template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k_mx4_finish(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ Mx4Bins bins;
+    __shared__ uint32_t up_s[MX4_LISTED];   // keys of the upper bounds
     __shared__ uint32_t rows_s[2 * MX4_FINISH];
     __shared__ uint32_t first_s[MX4_SEGMENTS + 1], n_s, rows_n;
     __shared__ uint64_t limit_s;
@@ -953,9 +618,13 @@ template <int BITS> static __global__ __launch_bounds__(1024) void k_mx4_finish(
     const uint32_t q = blockIdx.x;
     const Mx4Keep K{keys, &n_s, &limit_s, S.k};
     if (threadIdx.x < 64) {
-        const uint32_t c = threadIdx.x < MX4_SEGMENTS ? S.counts[q * MX4_SEGMENTS + threadIdx.x] : 0;
-        const bool over = c > S.segment;
-        uint32_t sum = min(c, S.segment);
+        bool over = false;
+        uint32_t sum = 0;
+        if (!DENSE && threadIdx.x < MX4_SEGMENTS) {
+            sum = S.counts[q * MX4_SEGMENTS + threadIdx.x];
+            over = sum > S.segment;
+            sum = min(sum, S.segment);
+        }
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t t = __shfl_up(sum, o);
@@ -972,48 +641,69 @@ template <int BITS> static __global__ __launch_bounds__(1024) void k_mx4_finish(
         }
     }
     __syncthreads();
-    const uint32_t n = first_s[MX4_SEGMENTS];
-    const auto at = [&](uint32_t i) -> const Mx4Cand & {   // candidate i of all segments
+    const uint32_t n = DENSE ? (uint32_t)S.E.rows.n : first_s[MX4_SEGMENTS];
+    const auto listed = [&](uint32_t i) -> const Mx4Cand & {   // candidate i of all segments
         uint32_t seg = 0;
 #pragma unroll
         for (uint32_t step = MX4_SEGMENTS / 2; step; step >>= 1)
             if (first_s[seg + step] <= i) seg += step;
         return S.cand[((size_t)q * MX4_SEGMENTS + seg) * S.segment + (i - first_s[seg])];
     };
-    uint32_t key = MX4_KEY_INF;
-    if (n > S.k) key = mx4_kth(bins, n, S.k, [&](uint64_t i) {
-        const float up = at((uint32_t)i).up;
+    const auto up_key = [&](uint64_t i) {
+        const float up = DENSE ? S.minima[(size_t)q * S.E.rows.n + i] : listed((uint32_t)i).up;
         return up == up ? mx4_key(up) : MX4_KEY_INF;
-    });
-    const float most = mx4_unkey(key);
-    // rows worth an exact score, collected and scored MX4_FINISH at a time
-    const auto score = [&]() {
-        __syncthreads();
-        const uint32_t m = rows_n;
-        for (uint32_t i0 = 0; i0 < m; i0 += MX4_FINISH / MX4_LANES) {
-            const uint32_t i = i0 + threadIdx.x / MX4_LANES;
-            const uint32_t row = rows_s[min(i, m - 1)];
-            const float s = mx4_exact_score<BITS>(S.E, q, row);
-            mx4_keep_add(K, threadIdx.x % MX4_LANES == 0 && i < m ? mx4_pack(s, row) : MX4_NONE, MX4_FINISH / MX4_LANES);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) rows_n = 0;
-        __syncthreads();
     };
+    uint32_t key = MX4_KEY_INF;
+    if (n > S.k) {
+        if (n <= MX4_LISTED) {
+            for (uint32_t i = threadIdx.x; i < n; i += MX4_FINISH) up_s[i] = up_key(i);
+            key = mx4_kth(bins, n, S.k, [&](uint64_t i) { return up_s[i]; });
+        } else {
+            key = mx4_kth(bins, n, S.k, up_key);
+        }
+    }
+    const float most = mx4_unkey(key);
+    // rows worth an exact score, collected and scored MX4_FINISH or more at a time
+    const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
     for (uint32_t i0 = 0; i0 < n; i0 += MX4_FINISH) {
         const uint32_t i = i0 + threadIdx.x;
         if (i < n) {
-            const Mx4Cand c = at(i);
-            if (!(c.low > most)) rows_s[atomicAdd(&rows_n, 1u)] = c.row;
+            uint32_t row = i;
+            float low;
+            if constexpr (DENSE) {
+                const float up = S.minima[(size_t)q * S.E.rows.n + i], y = S.qnorm[q];
+                const float x = reinterpret_cast<const float *>(S.E.rows.at(i / 32) + S.E.rows.panel - 128)[i & 31];
+                low = mx4_low(S.E.metric, up, x, y, S.slack);
+            } else {
+                const Mx4Cand &c = listed(i);
+                row = c.row;
+                low = c.low;
+            }
+            if (!(low > most)) rows_s[atomicAdd(&rows_n, 1u)] = row;
         }
         __syncthreads();
-        const bool full = rows_n > MX4_FINISH || i0 + MX4_FINISH >= n;   // (the same for all threads)
-        if (full) score();
-        else __syncthreads();
+        const uint32_t m = rows_n;
+        if (m <= MX4_FINISH && i0 + MX4_FINISH < n) {   // (the same for all threads)
+            __syncthreads();
+            continue;
+        }
+        if (n_s + m > MX4_KEEP) mx4_keep_cut(K);
+        const uint32_t base = n_s;
+        for (uint32_t r = threadIdx.x / lanes; r < m; r += at_once) {
+            const float s = mx4_exact_score<BITS>(S.E, q, rows_s[r], lanes);
+            if ((threadIdx.x & (lanes - 1)) == 0) keys[base + r] = mx4_pack(s, rows_s[r]);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            n_s = base + m;
+            rows_n = 0;
+        }
+        __syncthreads();
     }
     mx4_keep_cut(K);
-    const uint32_t got = n_s;
-    const bool again = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || got < min((uint64_t)S.k, S.E.rows.n));
+    uint32_t got = n_s;
+    while (got && keys[got - 1] == MX4_NONE) got--;   // NaN scores
+    const bool again = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || (!DENSE && got < min((uint64_t)S.k, S.E.rows.n)));
     if (threadIdx.x == 0) {
         S.again[q] = again;
         S.ticket[q] = 0;
@@ -1037,11 +727,11 @@ template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx
             limit_s = S.again_limit[q] + 1;
         }
         const uint64_t n = S.E.rows.n, per = (n + S.slices - 1) / S.slices, a = min(n, per * blockIdx.x), b = min(n, a + per);
-        const uint32_t at_once = 512 / MX4_LANES;
+        const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = 512 / lanes;
         for (uint64_t r0 = a; r0 < b; r0 += at_once) {
-            const uint64_t row = r0 + threadIdx.x / MX4_LANES;
-            const float s = mx4_exact_score<BITS>(S.E, q, min(row, n - 1));
-            mx4_keep_add(K, threadIdx.x % MX4_LANES == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
+            const uint64_t row = r0 + threadIdx.x / lanes;
+            const float s = mx4_exact_score<BITS>(S.E, q, min(row, n - 1), lanes);
+            mx4_keep_add(K, (threadIdx.x & (lanes - 1)) == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
         }
         mx4_keep_cut(K);
         uint64_t *mine = S.part + ((size_t)q * S.slices + blockIdx.x) * S.k;

@@ -4,6 +4,7 @@
 // included), its scratch is the caller's workspace.
 #include "vsgpu_internal.hpp"
 #include "mx4_host.hpp"
+#include "mx4_kernels.hpp"
 
 using namespace vsg;
 
@@ -57,30 +58,44 @@ Mx4Rows mx4_rows_of(const void *base, size_t n, size_t dim) {
 
 // how a batch of at most QUERY_BATCH queries runs
 struct Plan {
-    uint32_t tiles, qt, y;       // 32-query tiles (padded to y x qt), tiles per workgroup
-    bool global_b;
+    uint32_t tiles;              // 32-query tiles, padded to what the workgroups take
+    uint32_t groups;             // waves that share a panel
+    Mx4ScanShape shape;
     uint32_t qtile_bytes;
     uint64_t panels, take;       // panels of the table / of the probe
     bool by_row;                 // the probe keeps every row's bound, not one of 16 rows
+    bool dense;                  // ... and those bounds are the candidate list: no threshold, no second pass
     uint64_t minima;             // floats per query
     uint32_t segment, slices;    // candidates a list segment holds; workgroups per query that k_mx4_again may need
 };
-static Plan plan_scan(size_t dim, size_t nq, int bits) {
+static Plan plan_scan(size_t dim, size_t nq, int bits, int cus) {
     Plan p{};
     const uint32_t nt = (uint32_t)((nq + 31) / 32);
     p.qtile_bytes = mx4_qtile((uint32_t)dim, bits);
-    p.qt = nt >= 3 ? 4 : nt;
-    while (p.qt > 1 && p.qt * (p.qtile_bytes + 256) > LDS_BUDGET) p.qt /= 2;
-    p.global_b = p.qtile_bytes + 256 > LDS_BUDGET;
-    p.y = (nt + p.qt - 1) / p.qt;
-    p.tiles = p.y * p.qt;
+    p.shape.cus = cus;
+    p.groups = 1;
+    if (nt > 2 && dim <= 1024) {
+        p.shape.src = MX4_REGS;
+        p.shape.qt = 2;
+        p.groups = std::min(4u, (nt + 1) / 2);
+    } else if (p.qtile_bytes + 256 > LDS_BUDGET) {
+        p.shape.src = MX4_GLOBAL;
+        p.shape.qt = 1;
+    } else {
+        p.shape.src = MX4_SHARED;
+        p.shape.qt = nt >= 2 && 2 * (p.qtile_bytes + 256) <= LDS_BUDGET ? 2 : 1;
+    }
+    const uint32_t each = p.groups * p.shape.qt;
+    p.shape.y = (nt + each - 1) / each;
+    p.tiles = p.shape.y * each;
     return p;
 }
-static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits) {
-    Plan p = plan_scan(dim, nq, bits);
+static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int cus) {
+    Plan p = plan_scan(dim, nq, bits, cus);
     p.panels = (n + 31) / 32;
     // Small tables for their k: the probe covers every row.  One bound per 16 rows would put the threshold far above the k-th score.
-    p.by_row = n < 64 * k || p.panels <= 64;
+    p.dense = n <= MX4_LISTED;
+    p.by_row = p.dense || n < 64 * k;
     uint64_t expected;   // candidates
     if (p.by_row) {
         p.take = p.panels;
@@ -162,32 +177,8 @@ int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, si
     return bits == 6 ? launch_queries<6>(s, Q, tiles, type) : launch_queries<4>(s, Q, tiles, type);
 }
 
-template <int BITS, int QT, int MODE, int NB, bool GB> static int launch_scan5(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
-    const size_t lds = (GB ? 0 : (size_t)QT * P.qtile_bytes) + QT * 256 + (MODE == MX4_FILTER ? 4 * MX4_QUEUE * 16 : 0);
-    if (lds > 64 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, GB>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(QT >= 4 ? 2 : 4, (160 * 1024) / (lds + 512)));
-    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + 3) / 4, (uint64_t)cus * fit / p.y));
-    hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, GB>), dim3((unsigned)gx, p.y), dim3(256), lds, s, P);
-    HIPCHK(hipGetLastError());
-    return VSGPU_OK;
-}
-template <int BITS, int QT, int MODE> static int launch_scan3(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
-    if constexpr (QT == 1) {
-        if (p.global_b) return launch_scan5<BITS, 1, MODE, 4, true>(s, P, p, cus);
-    }
-    if (P.rows.kg == 1) return launch_scan5<BITS, QT, MODE, 1, false>(s, P, p, cus);
-    return launch_scan5<BITS, QT, MODE, 4, false>(s, P, p, cus);
-}
-template <int BITS, int MODE> static int launch_scan2(hipStream_t s, const Mx4Scan &P, const Plan &p, int cus) {
-    switch (p.qt) {
-    case 1: return launch_scan3<BITS, 1, MODE>(s, P, p, cus);
-    case 2: return launch_scan3<BITS, 2, MODE>(s, P, p, cus);
-    default: return launch_scan3<BITS, 4, MODE>(s, P, p, cus);
-    }
-}
-template <int MODE> static int launch_scan(hipStream_t s, const Mx4Scan &P, const Plan &p, int bits, int cus) {
-    return bits == 6 ? launch_scan2<6, MODE>(s, P, p, cus) : launch_scan2<4, MODE>(s, P, p, cus);
+static int launch_scan(hipStream_t s, int mode, const Mx4Scan &P, const Plan &p, int bits) {
+    return bits == 6 ? mx4_scan6(s, mode, P, p.shape) : mx4_scan4(s, mode, P, p.shape);
 }
 
 int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
@@ -233,13 +224,13 @@ int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
 size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
     Layout L;
     nq = std::min(nq, QUERY_BATCH);
-    take_topk(L, plan_topk(n, dim, nq, k, bits), nq, k);
+    take_topk(L, plan_topk(n, dim, nq, k, bits, 256), nq, k);
     // (a last batch of fewer queries may plan a wider probe)
     size_t most = L.at;
     for (size_t m : {(size_t)1, (size_t)32, (size_t)64, (size_t)128}) {
         if (m >= nq) break;
         Layout M;
-        take_topk(M, plan_topk(n, dim, m, k, bits), m, k);
+        take_topk(M, plan_topk(n, dim, m, k, bits, 256), m, k);
         most = std::max(most, M.at);
     }
     return most;
@@ -248,8 +239,8 @@ size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
 // queries of one batch -> ids / scores [nq][k] on the device
 int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
                    int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, hipEvent_t scan_begin, hipEvent_t scan_end) {
-    const Plan p = plan_topk(R.n, R.dim, nq, k, bits);
     const int cus = compute_units(device);
+    const Plan p = plan_topk(R.n, R.dim, nq, k, bits, cus);
     Layout L;
     L.base = static_cast<char *>(ws);
     const TopkBlock b = take_topk(L, p, nq, k);
@@ -260,6 +251,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.rows = R;
     P.tiles = b.q.tiles;
     P.qtile_bytes = p.qtile_bytes;
+    P.groups = p.groups;
     P.nq = (uint32_t)nq;
     P.metric = (uint32_t)metric;
     P.qnorm = b.q.norm;
@@ -272,15 +264,18 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.cand = b.cand;
     P.segment = p.segment;
     P.slack = mx4_slack(R.ks);
-    rc = p.by_row ? launch_scan<MX4_PROBE_ROWS>(s, P, p, bits, cus) : launch_scan<MX4_PROBE>(s, P, p, bits, cus);
+    if (p.dense && scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
+    rc = launch_scan(s, p.by_row ? MX4_PROBE_ROWS : MX4_PROBE, P, p, bits);
     if (rc) return rc;
-    const Mx4Threshold T{b.minima, p.minima, p.minima, (uint32_t)k, (uint32_t)metric, b.q.norm, b.q.sq, b.limit, P.slack};
-    hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
-    HIPCHK(hipGetLastError());
-    P.n_take = p.panels;
-    if (scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
-    rc = launch_scan<MX4_FILTER>(s, P, p, bits, cus);
-    if (rc) return rc;
+    if (!p.dense) {
+        const Mx4Threshold T{b.minima, p.minima, p.minima, (uint32_t)k, (uint32_t)metric, b.q.norm, b.q.sq, b.limit, P.slack};
+        hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
+        HIPCHK(hipGetLastError());
+        P.n_take = p.panels;
+        if (scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
+        rc = launch_scan(s, MX4_FILTER, P, p, bits);
+        if (rc) return rc;
+    }
     if (scan_end) HIPCHK(hipEventRecord(scan_end, s));
     Mx4Select S{};
     S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
@@ -296,12 +291,18 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.slices = p.slices;
     S.part = b.part;
     S.ticket = b.ticket;
-    const dim3 ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
-    if (bits == 6) {
-        hipLaunchKernelGGL((k_mx4_finish<6>), dim3((unsigned)nq), dim3(MX4_FINISH), 0, s, S);
+    S.minima = b.minima;
+    S.qnorm = b.q.norm;
+    S.slack = P.slack;
+    const dim3 fg((unsigned)nq), ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
+    if (p.dense) {
+        if (bits == 6) hipLaunchKernelGGL((k_mx4_finish<6, true>), fg, dim3(MX4_FINISH), 0, s, S);
+        else hipLaunchKernelGGL((k_mx4_finish<4, true>), fg, dim3(MX4_FINISH), 0, s, S);
+    } else if (bits == 6) {
+        hipLaunchKernelGGL((k_mx4_finish<6, false>), fg, dim3(MX4_FINISH), 0, s, S);
         hipLaunchKernelGGL((k_mx4_again<6>), ag, dim3(512), 0, s, S);
     } else {
-        hipLaunchKernelGGL((k_mx4_finish<4>), dim3((unsigned)nq), dim3(MX4_FINISH), 0, s, S);
+        hipLaunchKernelGGL((k_mx4_finish<4, false>), fg, dim3(MX4_FINISH), 0, s, S);
         hipLaunchKernelGGL((k_mx4_again<4>), ag, dim3(512), 0, s, S);
     }
     HIPCHK(hipGetLastError());
@@ -310,7 +311,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
 
 int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, int metric, int bits,
                      float *out, size_t out_stride, void *ws, size_t ws_bytes) {
-    const Plan p = plan_scan(R.dim, nq, bits);
+    const Plan p = plan_scan(R.dim, nq, bits, compute_units(device));
     Layout L;
     L.base = static_cast<char *>(ws);
     const QueryBlock b = take_queries(L, p);
@@ -321,6 +322,7 @@ int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *qu
     P.rows = R;
     P.tiles = b.tiles;
     P.qtile_bytes = p.qtile_bytes;
+    P.groups = p.groups;
     P.nq = (uint32_t)nq;
     P.metric = (uint32_t)metric;
     P.qnorm = b.norm;
@@ -328,7 +330,7 @@ int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *qu
     P.out = out;
     P.out_stride = out_stride;
     P.slack = mx4_slack(R.ks);
-    return launch_scan<MX4_DENSE>(s, P, p, bits, compute_units(device));
+    return launch_scan(s, MX4_DENSE, P, p, bits);
 }
 
 }  // namespace vsg
@@ -406,7 +408,7 @@ int mx4_table_scores(vsgpu_table *t, const void *query, const uint32_t *ids, siz
     int rc = upload_queries(t, query, 1, 0);
     if (rc) return rc;
     const Mx4Rows R = rows_of(t);
-    const Plan p = plan_scan(t->dim, 1, t->mx4_bits);
+    const Plan p = plan_scan(t->dim, 1, t->mx4_bits, c->n_cu);
     Layout size;
     take_queries(size, p);
     rc = ensure(c, c->qfrag2, size.at);
@@ -427,8 +429,8 @@ int mx4_table_scores(vsgpu_table *t, const void *query, const uint32_t *ids, siz
         if (ids) HIPCHK(hipMemcpyAsync(c->ids.p, ids + i, m * 4, hipMemcpyHostToDevice, c->stream));
         const uint32_t *d_ids = ids ? static_cast<const uint32_t *>(c->ids.p) : nullptr;
         const dim3 g((unsigned)std::min<size_t>((m + 15) / 16, (size_t)c->n_cu * 16));
-        if (t->mx4_bits == 6) hipLaunchKernelGGL((k_mx4_exact_rows<6>), g, dim3(256), 0, c->stream, E, 1u, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
-        else hipLaunchKernelGGL((k_mx4_exact_rows<4>), g, dim3(256), 0, c->stream, E, 1u, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
+        if (t->mx4_bits == 6) hipLaunchKernelGGL((k_mx4_exact_rows<6>), g, dim3(256), 0, c->stream, E, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
+        else hipLaunchKernelGGL((k_mx4_exact_rows<4>), g, dim3(256), 0, c->stream, E, d_ids, (uint64_t)(first + i), (uint64_t)m, (float *)c->dense.p);
         HIPCHK(hipGetLastError());
         HIPCHK(hipMemcpyAsync(c->pinned, c->dense.p, m * 4, hipMemcpyDeviceToHost, c->stream));
         HIPCHK(hipStreamSynchronize(c->stream));
@@ -577,7 +579,7 @@ extern "C" int vsgpu_mx4_read(int device, void *stream, const void *table, size_
 extern "C" size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits) {
     if (bad_shape(0, dim) || (bits != 4 && bits != 6) || nq == 0) return 0;
     Layout L;
-    take_queries(L, plan_scan(dim, std::min(nq, QUERY_BATCH), bits));
+    take_queries(L, plan_scan(dim, std::min(nq, QUERY_BATCH), bits, 256));
     return L.at;
 }
 extern "C" int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq,
