@@ -148,7 +148,8 @@ int vsgpu_table_set_sq8_block_bounds(vsgpu_table *t, const float bounds[8]);
  *
  * A table of capacity rows is ceil(capacity / 32) panels of vsgpu_mx4_panel_bytes(dim) bytes, 16-byte aligned; a panel holds 32
  * rows: codes [ceil(dim / 64)][half][row][16 bytes] (block 2 step + half, element j in byte j / 2, low nibble first), scale bytes
- * [ceil(dim / 256)][half][row][4] (byte i: step 4 group + i), row norms [32] fp32.  Zero bytes are zero rows. */
+ * [ceil(dim / 256)][half][row][4] (byte i: step 4 group + i; zero past the
+ * last step), row norms [32] fp32.  Zero bytes are zero rows. */
 size_t vsgpu_mx4_panel_bytes(size_t dim);   /* 0: dim is not in 1 .. 65536 */
 /* m vectors (VSGPU_F32, _F16 or _BF16; `stride` bytes apart) into slots[0 .. m) (device integers of slot_bytes = 4 or 8 bytes), or
  * into rows first .. first + m - 1 when slots is NULL.  A negative slot is padding: its vector is skipped; so is one whose slot is

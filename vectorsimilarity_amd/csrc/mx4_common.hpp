@@ -38,8 +38,9 @@ enum { MX4_L2 = 0, MX4_IP = 1, MX4_COSINE = 2 };
 __host__ __device__ inline uint32_t mx4_steps(uint32_t dim) { return (dim + 63) / 64; }
 __host__ __device__ inline uint32_t mx4_groups(uint32_t dim) { return (mx4_steps(dim) + 3) / 4; }
 __host__ __device__ inline uint32_t mx4_panel(uint32_t dim) { return mx4_steps(dim) * 1024 + mx4_groups(dim) * 256 + 128; }
-// a 32-query tile of the query block: operand bytes of every k-step (16 a lane; E2M3: 8 more a lane behind all of them), scales
-__host__ __device__ inline uint32_t mx4_qtile(uint32_t dim, int bits) { return mx4_steps(dim) * (bits == 6 ? 1536 : 1024) + mx4_groups(dim) * 256; }
+// a 32-query tile of the query block: operand bytes of every k-step (16 a lane; E2M3: 8 more a lane behind all of them), scales.
+// Whole groups of four steps, zero beyond the last one: a scan multiplies whole groups (the rows' scale bytes there are zero too)
+__host__ __device__ inline uint32_t mx4_qtile(uint32_t dim, int bits) { return mx4_groups(dim) * (bits == 6 ? 4 * 1536 + 256 : 4 * 1024 + 256); }
 
 // where rows are: one block of panels, or slabs of 2^shift panels each
 struct Mx4Rows {
@@ -48,6 +49,12 @@ struct Mx4Rows {
     uint32_t shift;
     uint32_t dim, ks, kg, panel;
     uint64_t n;
+    // p the same for the whole wave: the slab's address comes through the scalar cache, apart from the loads in flight
+    __device__ __forceinline__ uint64_t uniform_at(uint64_t p) const {
+        if (!slabs) return reinterpret_cast<uint64_t>(base) + p * panel;
+        typedef const __attribute__((address_space(4))) uint64_t *Scalar;
+        return ((Scalar)(uintptr_t)slabs)[p >> shift] + (p & ((1u << shift) - 1)) * (size_t)panel;
+    }
     __device__ char *at(uint64_t p) const {
         if (slabs) return slabs[p >> shift] + (p & ((1u << shift) - 1)) * (size_t)panel;
         return base + p * panel;
@@ -79,8 +86,8 @@ struct Mx4Scan {
     uint32_t nq, metric;
     uint32_t groups;              // waves that share a panel, each with its own query tiles
     const float *qnorm;
-    // which panels: n_take of them, number i is i * n_panels / n_take
-    uint64_t n_panels, n_take;
+    uint64_t n_take;              // panels: all of them, or for a probe number i is (i * every) >> 24
+    uint64_t every;
     float *minima;                // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row
     uint64_t minima_stride;
     const float2 *limit;          // FILTER: {alpha, beta} of each query

@@ -167,7 +167,10 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(1024) void k_mx4
             const float sq = mx4_codes4(v, inv, byte == 255, codes);
             ss += byte == 255 ? __builtin_nan("") : (double)sq * mx4_pow2(2 * (byte - 127));
             *reinterpret_cast<mx4_u4 *>(panel + (size_t)s * 1024 + at * 16) = codes;
-            panel[(size_t)W.rows.ks * 1024 + (s >> 2) * 256 + at * 4 + (s & 3)] = (char)byte;
+            char *scale = panel + (size_t)W.rows.ks * 1024 + (s >> 2) * 256 + at * 4 + (s & 3);
+            *scale = (char)byte;
+            if (s + 1 == W.rows.ks)   // the group's bytes past the last step: zero (mx4_qtile)
+                for (uint32_t i = (s & 3) + 1; i < 4; i++) *++scale = 0;
         }
     }
     part[wave][lane] = ss;
@@ -282,16 +285,12 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, row = lane & 31, half = lane >> 5;
     const uint32_t q = blockIdx.x * 32 + row;
     char *tile = Q.tiles + (size_t)blockIdx.x * mx4_qtile(Q.dim, BITS);
-    char *scales = tile + (size_t)Q.ks * (BITS == 6 ? 1536 : 1024);
+    char *scales = tile + (size_t)Q.kg * (BITS == 6 ? 4 * 1536 : 4 * 1024);
     const int esz = T == MX4_F32 ? 4 : 2;
     for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < Q.zero_words; i += gridDim.x * blockDim.x) Q.zero[i] = 0;
     double ss = 0;
     for (uint32_t s = wave; s < Q.kg * 4; s += waves) {
         char *sc = scales + (s >> 2) * 256 + lane * 4 + (s & 3);
-        if (s >= Q.ks) {
-            *sc = 0;
-            continue;
-        }
         const int have = q < Q.nq ? (int)Q.dim - (int)(2 * s + half) * 32 : 0;
         float v[32], inv;
         if (have > 0) mx4_load32<T, WIDE>(Q.x + q * Q.stride + (size_t)(2 * s + half) * 32 * esz, have, v);
@@ -305,7 +304,7 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) 
             mx4_u6 w;
             sq = mx4_codes6(v, inv, byte == 255, w);
             *reinterpret_cast<mx4_u4 *>(tile + (size_t)s * 1024 + lane * 16) = mx4_u4{w[0], w[1], w[2], w[3]};
-            *reinterpret_cast<mx4_u2 *>(tile + (size_t)Q.ks * 1024 + (size_t)s * 512 + lane * 8) = mx4_u2{w[4], w[5]};
+            *reinterpret_cast<mx4_u2 *>(tile + (size_t)Q.kg * 4096 + (size_t)s * 512 + lane * 8) = mx4_u2{w[4], w[5]};
         } else {
             mx4_u4 w;
             sq = mx4_codes4(v, inv, byte == 255, w);
@@ -479,11 +478,11 @@ template <int BITS> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact 
         const mx4_u4 x = *reinterpret_cast<const mx4_u4 *>(panel + (size_t)s * 1024 + ra * 16);
         const uint32_t bx = (uint8_t)panel[(size_t)E.rows.ks * 1024 + (s >> 2) * 256 + ra * 4 + (s & 3)];
         const mx4_u4 lo = *reinterpret_cast<const mx4_u4 *>(tile + (size_t)s * 1024 + qa * 16);
-        const uint32_t bq = (uint8_t)tile[(size_t)E.rows.ks * (BITS == 6 ? 1536 : 1024) + (s >> 2) * 256 + qa * 4 + (s & 3)];
+        const uint32_t bq = (uint8_t)tile[(size_t)E.rows.kg * (BITS == 6 ? 4 * 1536 : 4 * 1024) + (s >> 2) * 256 + qa * 4 + (s & 3)];
         float d = 0, sq = 0;
         mx4_f32 qv;
         if constexpr (BITS == 6) {
-            const mx4_u2 hi = *reinterpret_cast<const mx4_u2 *>(tile + (size_t)E.rows.ks * 1024 + (size_t)s * 512 + qa * 8);
+            const mx4_u2 hi = *reinterpret_cast<const mx4_u2 *>(tile + (size_t)E.rows.kg * 4096 + (size_t)s * 512 + qa * 8);
             qv = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(mx4_u6{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1]}, 1.f);
         } else {
 #pragma unroll

@@ -12,7 +12,7 @@ template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hi
     if (lds > 64 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     // as many workgroups as stay resident; few panels: fewer, so that a wave's start is not most of its work
-    const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(mx4_scan_waves(BITS, QT, NB, SRC), (160 * 1024) / (lds + 512)));
+    const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(mx4_scan_waves(BITS, QT, MODE, NB, SRC), (160 * 1024) / (lds + 512)));
     const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + abreast - 1) / abreast, (uint64_t)shape.cus * fit / shape.y));
     hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, SRC>), dim3((unsigned)gx, shape.y), dim3(64 * waves), lds, s, P);
     HIPCHK(hipGetLastError());

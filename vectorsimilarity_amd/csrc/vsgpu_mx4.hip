@@ -255,8 +255,8 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.nq = (uint32_t)nq;
     P.metric = (uint32_t)metric;
     P.qnorm = b.q.norm;
-    P.n_panels = p.panels;
     P.n_take = p.take;
+    P.every = (p.panels << 24) / p.take;   // (2^27 panels at most)
     P.minima = b.minima;
     P.minima_stride = p.minima;
     P.limit = b.limit;
@@ -326,7 +326,7 @@ int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *qu
     P.nq = (uint32_t)nq;
     P.metric = (uint32_t)metric;
     P.qnorm = b.norm;
-    P.n_panels = P.n_take = (R.n + 31) / 32;
+    P.n_take = (R.n + 31) / 32;
     P.out = out;
     P.out_stride = out_stride;
     P.slack = mx4_slack(R.ks);
