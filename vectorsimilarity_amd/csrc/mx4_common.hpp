@@ -73,7 +73,7 @@ constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: 
 
 enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
 constexpr uint32_t MX4_SEGMENTS = 32;             // a query's candidate list: one counter for every panel modulo 32
-constexpr uint32_t MX4_QUEUE = 256;               // survivors a wave collects in LDS before they go out
+constexpr uint32_t MX4_QUEUE = 128;               // survivors a wave collects in LDS before they go out
 struct Mx4Cand {
     uint32_t row;
     float low, up;                // bounds of its score

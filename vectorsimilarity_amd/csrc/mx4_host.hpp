@@ -5,7 +5,7 @@
 namespace vsg {
 struct Mx4Write;
 struct Mx4Read;
-enum { MX4_SHARED = 0, MX4_GLOBAL = 1, MX4_REGS = 2 };   // where a scan's waves take the queries' operands from
+enum { MX4_SHARED = 0, MX4_GLOBAL = 1, MX4_REGS = 2, MX4_RING = 3 };   // where the queries' operands are; RING: k_mx4_ring, or REGS for what it does not do
 struct Mx4ScanShape {
     int src, cus;
     uint32_t qt, y;   // query tiles a wave, workgroups side by side (each with groups x qt tiles)

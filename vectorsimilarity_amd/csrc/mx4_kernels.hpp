@@ -448,7 +448,7 @@ static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
         l.y = 1.f - tau - MX4_STEP * fmaxf(1.f, fabsf(tau));
     } else {
         l.x = ((1.f - tau) - T.slack - MX4_STEP) * yn;
-        l.y = yn < MX4_SHORT ? -inf : 0.f;
+        l.y = yn < MX4_SHORT ? -inf : 1e-42f;   // (0: a zero vector's dot is 0, and its score NaN)
     }
     if (tau == inf) l = make_float2(0.f, -inf);
     if (mx4_dead(T.metric, T.qsq[q])) l = make_float2(0.f, inf);

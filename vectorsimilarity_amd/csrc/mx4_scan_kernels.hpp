@@ -44,17 +44,105 @@ template <int BITS> struct Mx4Operand {
         else return mx4_i8{lo[0], lo[1], lo[2], lo[3], 0, 0, 0, 0};
     }
 };
-// a candidate into its query's list (segments of counters: one counter would make all waves wait in line for it)
-__device__ __forceinline__ void mx4_admit(const Mx4Scan &P, uint32_t q, uint32_t row, float d, float x, float y) {
-    const uint32_t seg = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
-    const uint32_t at = atomicAdd(&P.counts[seg], 1u);
-    if (at < P.segment) {
-        Mx4Cand c{row, 0.f, 0.f, 0u};
-        mx4_bounds(P.metric, d, x, y, P.slack, c.low, c.up);
-        P.cand[(size_t)seg * P.segment + at] = c;
+// A wave's survivors, collected in LDS and sent to their queries' lists 64 at a time: the returning atomic of a list's counter takes
+// microseconds, and a wave that waited for each by itself would do little else.  A list has 32 counters (every panel modulo 32), one
+// would make all waves wait in line.
+struct Mx4Queue {
+    mx4_u4 *slots;       // [MX4_QUEUE], LDS: {query, row, dot}
+    uint32_t n;
+    // norm[q]: |q|
+    __device__ __forceinline__ void flush(const Mx4Scan &P, const float *norm, int lane) {
+        for (uint32_t i = lane; i < n; i += 64) {
+            const mx4_u4 e = slots[i];
+            const uint32_t q = e[0], row = e[1], list = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
+            const float x = reinterpret_cast<const float *>(P.rows.at(row >> 5) + P.rows.panel - 128)[row & 31];
+            const uint32_t at = atomicAdd(&P.counts[list], 1u);
+            if (at < P.segment) {
+                Mx4Cand c{row, 0.f, 0.f, 0u};
+                mx4_bounds(P.metric, __uint_as_float(e[2]), x, norm[q], P.slack, c.low, c.up);
+                P.cand[(size_t)list * P.segment + at] = c;
+            }
+        }
+        n = 0;
     }
+    // mask: this lane's survivors among its 16 rows (bit v: dot d[v], row row0 + 8 (v / 4) + 4 half + v % 4)
+    __device__ __forceinline__ void push(const Mx4Scan &P, const float *norm, int lane, uint32_t q, uint32_t row0, uint32_t mask, const mx4_f16 &d) {
+        for (;;) {
+            const uint64_t b = __ballot(mask != 0);
+            if (b == 0) break;
+            if (n > MX4_QUEUE - 64) flush(P, norm, lane);
+            if (mask != 0) {
+                const int v = __builtin_ctz(mask);
+                float dot = d[0];
+#pragma unroll
+                for (int i = 1; i < 16; i++) dot = v == i ? d[i] : dot;
+                const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
+                slots[at] = mx4_u4{q, row0 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3), __float_as_uint(dot), 0u};
+                mask &= mask - 1;
+            }
+            n += __builtin_popcountll(b);
+        }
+    }
+};
+// What a row's dot is held against: f(dot, row) >= beta when the row's score may be at or below the query's threshold
+// (k_mx4_threshold).  L2 dot + slack |q| |x| - |x|^2 / 2,  IP dot + slack |q| |x|,  Cosine dot - least cosine x |q| |x|
+template <int M> __device__ __forceinline__ float mx4_held(float d, float x, float alpha) {
+    const float f = __fmaf_rn(-alpha, x, d);
+    if constexpr (M == MX4_L2) return __fmaf_rn(x * (-0.5f * (1.f - MX4_EPS)), x, f);
+    else return f;
+}
+// this lane's survivors.  Cosine: vectors too short for fp32 arithmetic go on to the exact one, zero vectors (score NaN) do not
+template <int M> __device__ __forceinline__ uint32_t mx4_survivors(const mx4_f16 &d, const mx4_f16 &x, float alpha, float beta) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        bool hit = mx4_held<M>(d[v], x[v], alpha) >= beta;
+        if constexpr (M == MX4_COSINE) hit |= x[v] < MX4_SHORT && x[v] > 0.f && beta < __uint_as_float(0x7F800000u);
+        mask |= hit ? 1u << v : 0u;
+    }
+    return mask;
+}
+// rows at or behind n do not count: bit v is row first + 8 (v / 4) + v % 4
+__device__ __forceinline__ uint32_t mx4_rows_below(uint64_t first, uint64_t n) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int v = 0; v < 16; v++) mask |= first + 8 * (v >> 2) + (v & 3) < n ? 1u << v : 0u;
+    return mask;
+}
+// PROBE: smaller is nearer, then the upper bound (mx4_bounds, a reciprocal's rounding in the slack) of the smallest.  h is per row
+template <int M> __device__ __forceinline__ float mx4_probe_row(float x, bool none) {
+    const float inf = __uint_as_float(0x7F800000u), nan = __uint_as_float(0x7FC00000u);
+    if constexpr (M == MX4_L2) return none ? inf : (1.f + MX4_EPS) * x * x;
+    else if constexpr (M == MX4_IP) return none ? inf : 0.f;
+    else return none || x < MX4_SHORT ? nan : __builtin_amdgcn_rcpf(x);
+}
+template <int M> __device__ __forceinline__ float mx4_probe_value(float d, float x, float h, float c) {   // c = slack |q|
+    if constexpr (M == MX4_L2) return __fmaf_rn(2.f * c, x, __fmaf_rn(-2.f, d, h));
+    else if constexpr (M == MX4_IP) return __fmaf_rn(c, x, h - d);
+    else return -d * h;
+}
+template <int M> __device__ __forceinline__ float mx4_probe_bound(float best, float y, float ry, float slack) {
+    const float inf = __uint_as_float(0x7F800000u);
+    float u;
+    if constexpr (M == MX4_L2) u = best + __fmaf_rn((1.f + MX4_EPS) * y, y, MX4_TINY);
+    else if constexpr (M == MX4_IP) u = 1.f + best, u = u + MX4_STEP * fmaxf(1.f, fabsf(u));
+    else u = y < MX4_SHORT ? inf : __fmaf_rn(best, ry, 1.f + slack + MX4_STEP);
+    return u == u ? u : inf;
 }
 
+// The ring of k_mx4_ring: the workgroup's four waves bring every panel into LDS together, a KiB at a time in turn, and `stages` panels
+// are under way or in use.  Constants by the chunks of a panel (codes, scales, norms in whole KiB); the stages fill the LDS beside the queues.
+constexpr int mx4_ring_pieces(int nb) { return (4 * nb * 1024 + nb * 256 + 128 + 1023) / 1024; }
+constexpr int mx4_ring_stages(int nb) { return nb == 1 ? 16 : (nb == 2 ? 15 : (nb == 3 ? 10 : 7)); }
+constexpr int mx4_ring_bytes(int nb) { return mx4_ring_stages(nb) * mx4_ring_pieces(nb) * 1024; }
+constexpr int MX4_RING_WAVES = 4;
+// 16 bytes a lane from base + offset to LDS (lds: the wave's first byte), without passing through registers
+__device__ __forceinline__ void mx4_to_lds(uint32_t lds, uint32_t offset, uint64_t base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+template <int N> __device__ __forceinline__ void mx4_wait_loads() {   // until at most N of the wave's memory operations are under way
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 // registers of a wave, about: what its operands, sums and panel in flight need
 constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
     const int regs = (src == MX4_REGS ? qt * nb * (bits == 6 ? 25 : 17) : qt * 12) + qt * 16 + nb * 17 + (mode == MX4_DENSE ? 60 : 105);
@@ -65,23 +153,23 @@ constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
 // 4 chunks go through the same four buffers several times.  The queries' operands (SRC) are
 //   up to 64 queries          in LDS, read per k-step: the registers hold more of the table in flight instead
 //   more, rows to 1024        in registers: LDS could not feed the matrix cores (1.5 KiB a tile and step against 32 cycles of matrix
-//                             work on each of four SIMDs), so a wave keeps two tiles and `groups` waves take the same panels, which
-//                             then come from the CU's own cache
+//                             work on each of four SIMDs), so a wave keeps one or two tiles and the waves take the same panels, through
+//                             LDS (RING) or, where stores are most of the traffic (DENSE), each by itself through the CU's cache (REGS)
 //   rows beyond the LDS       in global memory, through the caches
 template <int BITS, int QT, int MODE, int NB, int SRC>
 static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)) void k_mx4_scan(Mx4Scan P) {
     extern __shared__ char shared[];
     constexpr bool SWAP = MODE == MX4_DENSE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-    const uint32_t groups = SRC == MX4_REGS ? P.groups : 1, group = SRC == MX4_REGS ? wave % groups : 0;
+    constexpr bool HELD = SRC == MX4_REGS;   // operands in registers
+    const uint32_t groups = HELD ? P.groups : 1, group = HELD ? wave % groups : 0;
     const uint32_t block_q0 = blockIdx.y * groups * QT * 32, q0 = block_q0 + group * QT * 32;
-    const uint32_t ks = P.rows.ks, kg = SRC == MX4_REGS ? NB : P.rows.kg;
+    const uint32_t ks = P.rows.ks, kg = HELD ? NB : P.rows.kg;
     const char *tiles = P.tiles + (size_t)(q0 / 32) * P.qtile_bytes;
     const char *lds = SRC == MX4_SHARED ? shared : tiles;
     const uint32_t block_q = groups * QT * 32;
     float *yn_b = reinterpret_cast<float *>(shared + (SRC == MX4_SHARED ? QT * P.qtile_bytes : 0));   // |q|, 1 / |q| of the workgroup's queries
-    mx4_u4 *queue = reinterpret_cast<mx4_u4 *>(yn_b + 2 * block_q) + wave * MX4_QUEUE;   // FILTER: {query, row, dot, |x|}
-    uint32_t queued = 0;
+    Mx4Queue queue{reinterpret_cast<mx4_u4 *>(yn_b + 2 * block_q) + wave * MX4_QUEUE, 0};   // FILTER
     if constexpr (SRC == MX4_SHARED) {
         const mx4_u4 *src = reinterpret_cast<const mx4_u4 *>(tiles);
         const uint32_t n16 = QT * P.qtile_bytes / 16;
@@ -95,9 +183,9 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     __syncthreads();
     const float *yn_s = yn_b + group * QT * 32, *yr_s = yn_s + block_q;
     const uint32_t sc_at = kg * (BITS == 6 ? 4 * 1536 : 4 * 1024);
-    Mx4Operand<BITS> op[SRC == MX4_REGS ? QT * 4 * NB : 1];
-    int opsc[SRC == MX4_REGS ? QT * NB : 1];
-    if constexpr (SRC == MX4_REGS) {
+    Mx4Operand<BITS> op[HELD ? QT * 4 * NB : 1];
+    int opsc[HELD ? QT * NB : 1];
+    if constexpr (HELD) {
 #pragma unroll
         for (int q = 0; q < QT; q++) {
             const char *tile = tiles + q * P.qtile_bytes;
@@ -131,14 +219,6 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     uint32_t w = blockIdx.x * abreast + wave / groups;
     if (w >= n_take) return;
     const auto panel_of = [&](uint32_t i) -> uint64_t { return MODE == MX4_PROBE ? (i * P.every) >> 24 : i; };
-    // the wave's queue, 64 survivors at a time
-    const auto flush = [&]() {
-        for (uint32_t i = lane; i < queued; i += 64) {
-            const mx4_u4 e = queue[i];
-            mx4_admit(P, e[0], e[1], __uint_as_float(e[2]), __uint_as_float(e[3]), yn_s[e[0] - q0]);
-        }
-        queued = 0;
-    };
     Mx4Chunk buf[NB];
     mx4_f4 nrm[4];   // |x| of this lane's 16 rows (DENSE: nx, its one row), loaded with the panel's first chunks
     float nx = 0.f;
@@ -153,7 +233,7 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     fetch_norms(panel);
 #pragma unroll
     for (int g = 0; g < NB; g++)
-        if (g < (int)kg) mx4_fetch<SRC != MX4_REGS>(buf[g], panel, g, ks, lane);
+        if (g < (int)kg) mx4_fetch<!HELD>(buf[g], panel, g, ks, lane);
     for (; w < n_take; w += W) {
         const uint64_t p = panel_of(w);
         const uint32_t wn = w + W;
@@ -170,16 +250,17 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
                 if (g >= kg) break;
                 int sq[QT];
 #pragma unroll
-                for (int q = 0; q < QT; q++) sq[q] = SRC == MX4_REGS ? opsc[q * NB + j] : reinterpret_cast<const int *>(lds + q * P.qtile_bytes + sc_at + g * 256)[lane];
+                for (int q = 0; q < QT; q++) sq[q] = HELD ? opsc[q * NB + j] : reinterpret_cast<const int *>(lds + q * P.qtile_bytes + sc_at + g * 256)[lane];
+                const Mx4Chunk &c = buf[j];
                 const auto step = [&](auto index) {
                     constexpr int I = decltype(index)::value;
-                    const mx4_i8 t{buf[j].a[I][0], buf[j].a[I][1], buf[j].a[I][2], buf[j].a[I][3], 0, 0, 0, 0};
+                    const mx4_i8 t{c.a[I][0], c.a[I][1], c.a[I][2], c.a[I][3], 0, 0, 0, 0};
 #pragma unroll
                     for (int q = 0; q < QT; q++) {
                         Mx4Operand<BITS> o;
-                        if constexpr (SRC == MX4_REGS) o = op[q * 4 * NB + 4 * j + I];
+                        if constexpr (HELD) o = op[q * 4 * NB + 4 * j + I];
                         else o.load(lds + q * P.qtile_bytes, 4 * g + I, kg, lane);
-                        acc[q] = mx4_mma<BITS, SWAP, I>(t, o.get(), acc[q], buf[j].sc, sq[q]);
+                        acc[q] = mx4_mma<BITS, SWAP, I>(t, o.get(), acc[q], c.sc, sq[q]);
                     }
                 };
                 step(std::integral_constant<int, 0>{});
@@ -187,8 +268,8 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
                 step(std::integral_constant<int, 2>{});
                 step(std::integral_constant<int, 3>{});
                 // the buffer's next contents: NB chunks on in this panel, or the chunk of the next panel that it takes
-                if (SRC != MX4_REGS && g + NB < kg) mx4_fetch<true>(buf[j], panel, g + NB, ks, lane);
-                else mx4_fetch<SRC != MX4_REGS>(buf[j], next, j, ks, lane);
+                if (!HELD && g + NB < kg) mx4_fetch<true>(buf[j], panel, g + NB, ks, lane);
+                else mx4_fetch<!HELD>(buf[j], next, j, ks, lane);
             }
         }
         // this panel's norms, and the next one's on their way
@@ -199,7 +280,6 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
         fetch_norms(next);
         const uint64_t row0 = p * 32;
         const bool tail = row0 + 32 > P.rows.n;
-        const float inf = __uint_as_float(0x7F800000u), nan = __uint_as_float(0x7FC00000u);
         const auto row_of = [&](int v) { return row0 + 8 * (v >> 2) + 4 * half + (v & 3); };
         const auto dense = [&](auto metric, auto whole, auto divide) {
             constexpr int M = decltype(metric)::value;
@@ -225,98 +305,45 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
                     }
                 }
         };
-        // a survivor when its score may be at or below the query's threshold.  f is the dot less what its row asks for, and is held
-        // against one number a query:  L2 dot + slack |q| |x| - |x|^2 / 2,  IP dot + slack |q| |x|,  Cosine dot / |x|
         const auto filter = [&](auto metric) {
             constexpr int M = decltype(metric)::value;
-            mx4_f16 h;
-            bool odd = false;   // Cosine: vectors too short for this arithmetic go on to the exact one
+            bool odd = false;
+            if constexpr (M == MX4_COSINE) {
+                float least = xn[0];
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float x = xn[v];
-                if constexpr (M == MX4_L2) h[v] = 0.5f * (1.f - MX4_EPS) * x * x;
-                if constexpr (M == MX4_COSINE) {
-                    h[v] = __builtin_amdgcn_rcpf(x);   // (zero: 0 x infinity is NaN, never a survivor)
-                    odd |= x < MX4_SHORT && x > 0.f;
-                }
+                for (int v = 1; v < 16; v++) least = fminf(least, xn[v]);
+                odd = __any(least < MX4_SHORT);
             }
-            odd = M == MX4_COSINE && __any(odd);
 #pragma unroll
             for (int q = 0; q < QT; q++) {
-                const float bound = M == MX4_COSINE && beta[q] == 0.f ? alpha[q] : beta[q];
-                const auto f = [&](int v) {
-                    const float x = xn[v], d = acc[q][v];
-                    if constexpr (M == MX4_L2) return __fmaf_rn(-alpha[q], x, d) - h[v];
-                    else if constexpr (M == MX4_IP) return __fmaf_rn(-alpha[q], x, d);
-                    else return d * h[v];
-                };
-                float most = f(0);
+                float most = mx4_held<M>(acc[q][0], xn[0], alpha[q]);
 #pragma unroll
-                for (int v = 1; v < 16; v++) most = fmaxf(most, f(v));
-                if (!__any(most >= bound) && !odd) continue;
-                if (queued > MX4_QUEUE - 128) flush();
-                const uint32_t me = q0 + q * 32 + col, before = queued;
-                bool spilt = false;
-                const auto hit = [&](int v) {
-                    const float x = xn[v];
-                    return (f(v) >= bound || (M == MX4_COSINE && x < MX4_SHORT && x > 0.f && bound < inf)) && row_of(v) < P.rows.n;
-                };
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const bool mine = hit(v);
-                    const uint64_t b = __ballot(mine);
-                    if (b == 0) continue;
-                    const uint32_t at = queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
-                    queued += __builtin_popcountll(b);
-                    spilt |= queued > MX4_QUEUE;
-                    if (mine && at < MX4_QUEUE) queue[at] = mx4_u4{me, (uint32_t)row_of(v), __float_as_uint(acc[q][v]), __float_as_uint(xn[v])};
-                }
-                if (spilt) {   // a panel full of survivors: this tile's again, straight to the lists
-                    queued = before;
-#pragma unroll 1
-                    for (int v = 0; v < 16; v++)
-                        if (hit(v)) mx4_admit(P, me, (uint32_t)row_of(v), acc[q][v], xn[v], yn_s[q * 32 + col]);
-                }
+                for (int v = 1; v < 16; v++) most = fmaxf(most, mx4_held<M>(acc[q][v], xn[v], alpha[q]));
+                if (!__any(most >= beta[q]) && !odd) continue;
+                uint32_t mask = mx4_survivors<M>(acc[q], xn, alpha[q], beta[q]);
+                if (tail) mask &= mx4_rows_below(row0 + 4 * half, P.rows.n);
+                queue.push(P, yn_s - q0, lane, q0 + q * 32 + col, (uint32_t)row0, mask, acc[q]);
             }
         };
-        // the smallest upper bound (mx4_bounds, with a reciprocal's rounding in the slack) of this lane's 16 rows
         const auto probe = [&](auto metric) {
             constexpr int M = decltype(metric)::value;
-            float h[16];
+            mx4_f16 h;
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float x = xn[v];
-                const bool none = tail && row_of(v) >= P.rows.n;
-                if constexpr (M == MX4_L2) h[v] = none ? inf : (1.f + MX4_EPS) * x * x;
-                else if constexpr (M == MX4_IP) h[v] = none ? inf : 0.f;
-                else h[v] = none || x < MX4_SHORT ? nan : __builtin_amdgcn_rcpf(x);
-            }
+            for (int v = 0; v < 16; v++) h[v] = mx4_probe_row<M>(xn[v], tail && row_of(v) >= P.rows.n);
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 const uint32_t me = q0 + q * 32 + col;
-                const float y = alpha[q], c = P.slack * y;
-                const auto up = [&](float best) {
-                    float u;
-                    if constexpr (M == MX4_L2) u = best + __fmaf_rn((1.f + MX4_EPS) * y, y, MX4_TINY);
-                    else if constexpr (M == MX4_IP) u = 1.f + best, u = u + MX4_STEP * fmaxf(1.f, fabsf(u));
-                    else u = y < MX4_SHORT ? inf : __fmaf_rn(best, beta[q], 1.f + P.slack + MX4_STEP);
-                    return u == u ? u : inf;
-                };
-                const auto g = [&](int v) {   // smaller is nearer
-                    const float x = xn[v], d = acc[q][v];
-                    if constexpr (M == MX4_L2) return __fmaf_rn(2.f * c, x, __fmaf_rn(-2.f, d, h[v]));
-                    else if constexpr (M == MX4_IP) return __fmaf_rn(c, x, h[v] - d);
-                    else return -d * h[v];
-                };
+                const float c = P.slack * alpha[q];
                 if constexpr (MODE == MX4_PROBE_ROWS) {
 #pragma unroll
                     for (int v = 0; v < 16; v++)
-                        if (me < P.nq && row_of(v) < P.rows.n) P.minima[me * P.minima_stride + row_of(v)] = up(g(v));
+                        if (me < P.nq && row_of(v) < P.rows.n)
+                            P.minima[me * P.minima_stride + row_of(v)] = mx4_probe_bound<M>(mx4_probe_value<M>(acc[q][v], xn[v], h[v], c), alpha[q], beta[q], P.slack);
                 } else {
-                    float best = g(0);
+                    float best = mx4_probe_value<M>(acc[q][0], xn[0], h[0], c);
 #pragma unroll
-                    for (int v = 1; v < 16; v++) best = fminf(best, g(v));
-                    if (me < P.nq) P.minima[me * P.minima_stride + 2 * w + half] = up(best);
+                    for (int v = 1; v < 16; v++) best = fminf(best, mx4_probe_value<M>(acc[q][v], xn[v], h[v], c));
+                    if (me < P.nq) P.minima[me * P.minima_stride + 2 * w + half] = mx4_probe_bound<M>(best, alpha[q], beta[q], P.slack);
                 }
             }
         };
@@ -349,7 +376,197 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
         }
         panel = next;
     }
-    if constexpr (MODE == MX4_FILTER) flush();
+    if constexpr (MODE == MX4_FILTER) queue.flush(P, yn_s - q0, lane);
+}
+
+// The same passes for 65 to 256 queries against rows of at most 1024 elements.  Four waves, QT tiles each, take every panel together; it
+// comes through LDS, so that the memory's latency is covered by a ring of panels and not by registers, which hold the operands.  One
+// wave a SIMD: a panel's comparisons (prev) are made while the next one's matrix instructions run, a few between every two of them.
+template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_bounds__(256, 1) void k_mx4_ring(Mx4Scan P) {
+    extern __shared__ char shared[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    constexpr int PIECES = mx4_ring_pieces(NB), STAGES = mx4_ring_stages(NB), STAGE = PIECES * 1024;
+    constexpr int EACH = PIECES / MX4_RING_WAVES, OVER = PIECES % MX4_RING_WAVES;   // waves below OVER take one piece more
+    constexpr uint32_t BLOCK_Q = MX4_RING_WAVES * QT * 32;
+    const uint32_t block_q0 = blockIdx.y * BLOCK_Q, q0 = block_q0 + wave * QT * 32, ks = P.rows.ks;
+    const char *tiles = P.tiles + (size_t)(q0 / 32) * P.qtile_bytes;
+    float *yn_b = reinterpret_cast<float *>(shared + mx4_ring_bytes(NB));
+    Mx4Queue queue{reinterpret_cast<mx4_u4 *>(yn_b + 2 * BLOCK_Q) + wave * MX4_QUEUE, 0};
+    for (uint32_t i = threadIdx.x; i < BLOCK_Q; i += 256) {
+        const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
+        yn_b[i] = y;
+        yn_b[BLOCK_Q + i] = 1.f / y;
+    }
+    __syncthreads();
+    const float *norms = yn_b - block_q0;   // by query
+    Mx4Operand<BITS> op[QT][4 * NB];
+    int opsc[QT][NB];
+    float alpha[QT], beta[QT];   // FILTER: the threshold; PROBE: |q|, 1 / |q|
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+        const char *tile = tiles + q * P.qtile_bytes;
+#pragma unroll
+        for (int s = 0; s < 4 * NB; s++) op[q][s].load(tile, s, NB, lane);
+#pragma unroll
+        for (int g = 0; g < NB; g++) opsc[q][g] = reinterpret_cast<const int *>(tile + NB * (BITS == 6 ? 4 * 1536 : 4 * 1024) + g * 256)[lane];
+        const uint32_t me = q0 + q * 32 + col;
+        if constexpr (MODE == MX4_FILTER) {
+            const float2 l = me < P.nq ? P.limit[me] : make_float2(0.f, __uint_as_float(0x7F800000u));
+            alpha[q] = l.x;
+            beta[q] = l.y;
+        } else {
+            alpha[q] = norms[me];
+            beta[q] = norms[BLOCK_Q + me];
+        }
+    }
+    const uint32_t n_take = (uint32_t)P.n_take;
+    uint32_t w = blockIdx.x;
+    if (w >= n_take) return;
+    const auto panel_of = [&](uint32_t i) -> uint64_t { return MODE == MX4_PROBE ? (i * P.every) >> 24 : i; };
+    uint32_t ahead = w, fill = 0, use = 0;   // the panel to request next, the stage it goes to, the stage in use
+    const auto request = [&]() {   // (past the end the last panel again, so that the count of what is under way stays the same)
+        const uint64_t from = P.rows.uniform_at(panel_of(min(ahead, n_take - 1)));
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)shared + fill * STAGE;
+#pragma unroll
+        for (int i = 0; i <= EACH; i++) {
+            if (i == EACH && wave >= OVER) break;
+            const uint32_t offset = (i * MX4_RING_WAVES + wave) * 1024;
+            mx4_to_lds(to + offset, min(offset + lane * 16, P.rows.panel - 16), from);
+        }
+        ahead += gridDim.x;
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; i++) request();
+
+    struct Panel {
+        mx4_f16 acc[QT], x;   // dots, |x|
+        uint32_t w;
+    };
+    const auto row0_of = [&](const Panel &p) { return panel_of(p.w) * 32; };
+    // a panel's comparisons, v-th of its rows
+    float most[QT], least;
+    mx4_f16 h;
+    const auto compare = [&](const Panel &p, int v) {
+        if constexpr (MODE == MX4_FILTER) {
+            if (M == MX4_COSINE) least = v ? fminf(least, p.x[v]) : p.x[0];
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                const float f = mx4_held<M>(p.acc[q][v], p.x[v], alpha[q]);
+                most[q] = v ? fmaxf(most[q], f) : f;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                const float f = mx4_probe_value<M>(p.acc[q][v], p.x[v], h[v], P.slack * alpha[q]);
+                most[q] = v ? fminf(most[q], f) : f;
+            }
+        }
+    };
+    const auto conclude = [&](const Panel &p) {
+        if constexpr (MODE == MX4_FILTER) {
+            const bool odd = M == MX4_COSINE && __any(least < MX4_SHORT);
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                if (!__any(most[q] >= beta[q]) && !odd) continue;
+                const uint64_t row0 = row0_of(p);
+                uint32_t mask = mx4_survivors<M>(p.acc[q], p.x, alpha[q], beta[q]);
+                if (row0 + 32 > P.rows.n) mask &= mx4_rows_below(row0 + 4 * half, P.rows.n);
+                queue.push(P, norms, lane, q0 + q * 32 + col, (uint32_t)row0, mask, p.acc[q]);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                const uint32_t me = q0 + q * 32 + col;
+                if (me < P.nq) P.minima[me * P.minima_stride + 2 * p.w + half] = mx4_probe_bound<M>(most[q], alpha[q], beta[q], P.slack);
+            }
+        }
+    };
+    const auto prepare = [&](Panel &p) {   // PROBE: what is per row
+        if constexpr (MODE == MX4_PROBE) {
+            const uint64_t row0 = row0_of(p);
+#pragma unroll
+            for (int v = 0; v < 16; v++) h[v] = mx4_probe_row<M>(p.x[v], row0 + 8 * (v >> 2) + 4 * half + (v & 3) >= P.rows.n);
+        }
+    };
+    // one panel: its dots into p, and q's comparisons
+    const auto round = [&](Panel &p, Panel &q) {
+        // this wave's part of the stage is there; behind the barrier everybody's is, and nobody reads the stage before it any more
+        if (wave < OVER) mx4_wait_loads<(STAGES - 2) * (EACH + 1)>();
+        else mx4_wait_loads<(STAGES - 2) * EACH>();
+        asm volatile("s_barrier" ::: "memory");
+        request();
+        const char *stage = shared + use * STAGE;
+        use = use + 1 == STAGES ? 0 : use + 1;
+        prepare(q);
+        Mx4Chunk buf[2];
+        const auto take = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) buf[j & 1].a[i] = reinterpret_cast<const mx4_i4 *>(stage + min(4u * j + i, ks - 1) * 1024)[lane];
+            buf[j & 1].sc = reinterpret_cast<const int *>(stage + ks * 1024 + j * 256)[lane];
+        };
+        take(0);
+        mx4_f4 nrm[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) nrm[i] = reinterpret_cast<const mx4_f4 *>(stage + P.rows.panel - 128)[2 * i + half];
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) p.acc[t][v] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            if (j + 1 < NB) take(j + 1);
+            const Mx4Chunk &c = buf[j & 1];
+            const auto step = [&](auto index) {
+                constexpr int I = decltype(index)::value;
+                const mx4_i8 t{c.a[I][0], c.a[I][1], c.a[I][2], c.a[I][3], 0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < QT; i++) p.acc[i] = mx4_mma<BITS, false, I>(t, op[i][4 * j + I].get(), p.acc[i], c.sc, opsc[i][j]);
+                // 16 rows of the panel before, over 4 NB steps
+                const int s = 4 * j + I;
+#pragma unroll
+                for (int v = s * 16 / (4 * NB); v < (s + 1) * 16 / (4 * NB); v++) compare(q, v);
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        }
+#pragma unroll
+        for (int v = 0; v < 16; v++) p.x[v] = nrm[v >> 2][v & 3];
+        p.w = w;
+        conclude(q);
+    };
+    Panel a, b;   // b: a panel before the first one, without survivors
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        b.x[v] = 1.f;
+#pragma unroll
+        for (int q = 0; q < QT; q++) b.acc[q][v] = -3e38f;
+    }
+    b.w = w;   // (PROBE: overwritten with the panel's own result)
+    const auto last = [&](Panel &p) {
+        prepare(p);
+#pragma unroll
+        for (int v = 0; v < 16; v++) compare(p, v);
+        conclude(p);
+    };
+    for (;;) {
+        round(a, b);
+        w += gridDim.x;
+        if (w >= n_take) {
+            last(a);
+            break;
+        }
+        round(b, a);
+        w += gridDim.x;
+        if (w >= n_take) {
+            last(b);
+            break;
+        }
+    }
+    if constexpr (MODE == MX4_FILTER) queue.flush(P, norms, lane);
+    mx4_wait_loads<0>();   // (what is under way writes this workgroup's LDS)
 }
 
 }  // namespace vsg

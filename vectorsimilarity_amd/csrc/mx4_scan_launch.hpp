@@ -7,8 +7,8 @@
 namespace vsg {
 
 template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
-    const uint32_t waves = SRC == MX4_REGS ? (P.groups == 3 ? 3 : 4) : 4, abreast = waves / P.groups;
-    const size_t lds = (SRC == MX4_SHARED ? (size_t)QT * P.qtile_bytes : 0) + P.groups * QT * 256 + (MODE == MX4_FILTER ? 4 * MX4_QUEUE * 16 : 0);
+    const uint32_t waves = SRC == MX4_REGS && P.groups == 3 ? 3 : 4, groups = SRC == MX4_REGS ? P.groups : 1, abreast = waves / groups;
+    const size_t lds = (SRC == MX4_SHARED ? (size_t)QT * P.qtile_bytes : 0) + groups * QT * 256 + (MODE == MX4_FILTER ? waves * MX4_QUEUE * 16 : 0);
     if (lds > 64 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     // as many workgroups as stay resident; few panels: fewer, so that a wave's start is not most of its work
@@ -18,15 +18,40 @@ template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hi
     HIPCHK(hipGetLastError());
     return VSGPU_OK;
 }
+template <int BITS, int QT, int MODE, int SRC> static int launch_chunks(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
+    switch (P.rows.kg) {
+    case 1: return launch_scan<BITS, QT, MODE, 1, SRC>(s, P, shape);
+    case 2: return launch_scan<BITS, QT, MODE, 2, SRC>(s, P, shape);
+    case 3: return launch_scan<BITS, QT, MODE, 3, SRC>(s, P, shape);
+    default: return launch_scan<BITS, QT, MODE, 4, SRC>(s, P, shape);
+    }
+}
+template <int BITS, int QT, int MODE, int NB, int M> static int launch_ring4(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
+    const size_t lds = (size_t)mx4_ring_bytes(NB) + MX4_RING_WAVES * QT * 256 + (MODE == MX4_FILTER ? MX4_RING_WAVES * MX4_QUEUE * 16 : 0);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_ring<BITS, QT, MODE, NB, M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>(P.n_take, (uint64_t)shape.cus / shape.y));
+    hipLaunchKernelGGL((k_mx4_ring<BITS, QT, MODE, NB, M>), dim3((unsigned)gx, shape.y), dim3(64 * MX4_RING_WAVES), lds, s, P);
+    HIPCHK(hipGetLastError());
+    return VSGPU_OK;
+}
+template <int BITS, int QT, int MODE, int NB> static int launch_ring3(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
+    if (P.metric == MX4_L2) return launch_ring4<BITS, QT, MODE, NB, MX4_L2>(s, P, shape);
+    if (P.metric == MX4_IP) return launch_ring4<BITS, QT, MODE, NB, MX4_IP>(s, P, shape);
+    return launch_ring4<BITS, QT, MODE, NB, MX4_COSINE>(s, P, shape);
+}
+template <int BITS, int QT, int MODE> static int launch_ring(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
+    switch (P.rows.kg) {
+    case 1: return launch_ring3<BITS, QT, MODE, 1>(s, P, shape);
+    case 2: return launch_ring3<BITS, QT, MODE, 2>(s, P, shape);
+    case 3: return launch_ring3<BITS, QT, MODE, 3>(s, P, shape);
+    default: return launch_ring3<BITS, QT, MODE, 4>(s, P, shape);
+    }
+}
 template <int BITS, int MODE> static int launch_mode(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
     if (shape.src == MX4_GLOBAL) return launch_scan<BITS, 1, MODE, 4, MX4_GLOBAL>(s, P, shape);
-    if (shape.src == MX4_REGS) {
-        switch (P.rows.kg) {
-        case 1: return launch_scan<BITS, 2, MODE, 1, MX4_REGS>(s, P, shape);
-        case 2: return launch_scan<BITS, 2, MODE, 2, MX4_REGS>(s, P, shape);
-        case 3: return launch_scan<BITS, 2, MODE, 3, MX4_REGS>(s, P, shape);
-        default: return launch_scan<BITS, 2, MODE, 4, MX4_REGS>(s, P, shape);
-        }
+    if (shape.src == MX4_RING) {
+        if constexpr (MODE == MX4_DENSE || MODE == MX4_PROBE_ROWS) return launch_chunks<BITS, 2, MODE, MX4_REGS>(s, P, shape);
+        else return shape.qt == 1 ? launch_ring<BITS, 1, MODE>(s, P, shape) : launch_ring<BITS, 2, MODE>(s, P, shape);
     }
     if (P.rows.kg == 1) return shape.qt == 1 ? launch_scan<BITS, 1, MODE, 1, MX4_SHARED>(s, P, shape) : launch_scan<BITS, 2, MODE, 1, MX4_SHARED>(s, P, shape);
     return shape.qt == 1 ? launch_scan<BITS, 1, MODE, 4, MX4_SHARED>(s, P, shape) : launch_scan<BITS, 2, MODE, 4, MX4_SHARED>(s, P, shape);

@@ -75,9 +75,12 @@ static Plan plan_scan(size_t dim, size_t nq, int bits, int cus) {
     p.shape.cus = cus;
     p.groups = 1;
     if (nt > 2 && dim <= 1024) {
-        p.shape.src = MX4_REGS;
-        p.shape.qt = 2;
-        p.groups = std::min(4u, (nt + 1) / 2);
+        p.shape.src = MX4_RING;
+        p.shape.qt = nt <= 4 ? 1 : 2;
+        p.groups = std::min(4u, (nt + 1) / 2);   // (REGS: two tiles a wave)
+        p.tiles = 4 * p.shape.qt;
+        p.shape.y = 1;
+        return p;
     } else if (p.qtile_bytes + 256 > LDS_BUDGET) {
         p.shape.src = MX4_GLOBAL;
         p.shape.qt = 1;
@@ -85,9 +88,8 @@ static Plan plan_scan(size_t dim, size_t nq, int bits, int cus) {
         p.shape.src = MX4_SHARED;
         p.shape.qt = nt >= 2 && 2 * (p.qtile_bytes + 256) <= LDS_BUDGET ? 2 : 1;
     }
-    const uint32_t each = p.groups * p.shape.qt;
-    p.shape.y = (nt + each - 1) / each;
-    p.tiles = p.shape.y * each;
+    p.shape.y = (nt + p.shape.qt - 1) / p.shape.qt;
+    p.tiles = p.shape.y * p.shape.qt;
     return p;
 }
 static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int cus) {
