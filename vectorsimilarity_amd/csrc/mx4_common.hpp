@@ -72,12 +72,12 @@ constexpr float MX4_TINY = 1e-36f;                // L2 scores below it: fp32 ha
 constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: the product of the norms may leave fp32
 
 enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
-constexpr uint32_t MX4_SEGMENTS = 32;             // a query's candidate list: one counter for every panel modulo 32
+constexpr uint32_t MX4_SEGMENTS = 32;             // parts of a query's candidate list: one for every panel modulo 32,
+constexpr uint32_t MX4_SEGMENTS_MAX = 256;        // or one for each workgroup of k_mx4_ring
 constexpr uint32_t MX4_QUEUE = 128;               // survivors a wave collects in LDS before they go out
 struct Mx4Cand {
     uint32_t row;
-    float low, up;                // bounds of its score
-    uint32_t pad;
+    float dot, x;                 // of the matrix cores, |x|
 };
 struct Mx4Scan {
     Mx4Rows rows;
@@ -91,9 +91,9 @@ struct Mx4Scan {
     float *minima;                // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row
     uint64_t minima_stride;
     const float2 *limit;          // FILTER: {alpha, beta} of each query
-    uint32_t *counts;             // FILTER: [nq][MX4_SEGMENTS]
-    Mx4Cand *cand;                // [nq][MX4_SEGMENTS][segment]
-    uint32_t segment;
+    uint32_t *counts;             // FILTER: [nq][segments]
+    Mx4Cand *cand;                // [nq][segments][segment]
+    uint32_t segments, segment;
     float *out;                   // DENSE: [nq][out_stride]
     uint64_t out_stride;
     float slack;

@@ -3,6 +3,8 @@
 #pragma once
 #include "mx4_common.hpp"
 
+#include <type_traits>
+
 namespace vsg {
 
 __device__ __forceinline__ double mx4_pow2(int e) {   // 2^e, |e| <= 1000
@@ -332,7 +334,8 @@ __device__ __forceinline__ float mx4_unkey(uint32_t k) { return __uint_as_float(
 constexpr uint32_t MX4_KEY_INF = 0xFF800000u;   // key of infinity: not counted
 constexpr uint32_t MX4_BINS = 2048;
 struct Mx4Bins {   // shared
-    uint32_t hist[MX4_BINS];
+    uint32_t hist[MX4_BINS + MX4_BINS / 32];   // (a word free after every 32: the scan's lanes read 32 bins each)
+    __device__ __forceinline__ uint32_t &bin(uint32_t i) { return hist[i + (i >> 5)]; }
     uint32_t lo, hi, pick, left, in;
 };
 // A number at or above the k-th smallest of n keys, and close to it (MX4_KEY_INF: fewer than k of them are finite).  Bins of equal
@@ -370,18 +373,19 @@ template <typename F> __device__ __forceinline__ uint32_t mx4_kth(Mx4Bins &B, ui
         // bins of 2^shift keys from lo on
         const uint32_t range = hi - lo;
         const int shift = range < MX4_BINS ? 0 : 32 - __builtin_clz(range) - 11;
-        for (uint32_t i = threadIdx.x; i < MX4_BINS; i += blockDim.x) B.hist[i] = 0;
+        for (uint32_t i = threadIdx.x; i < MX4_BINS + MX4_BINS / 32; i += blockDim.x) B.hist[i] = 0;
         if (threadIdx.x == 0) B.pick = 0xFFFFFFFFu;
         __syncthreads();
         for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
             const uint32_t key = key_of(i);
-            if (key >= lo && key <= hi && key < MX4_KEY_INF) atomicAdd(&B.hist[(key - lo) >> shift], 1u);
+            if (key >= lo && key <= hi && key < MX4_KEY_INF) atomicAdd(&B.bin((key - lo) >> shift), 1u);
         }
         __syncthreads();
         if (threadIdx.x < 64) {   // one wave: 32 bins a lane, then the lane's own
             const uint32_t b0 = threadIdx.x * (MX4_BINS / 64);
-            uint32_t sum = 0;
-            for (uint32_t i = 0; i < MX4_BINS / 64; i++) sum += B.hist[b0 + i];
+            uint32_t sum = 0, own[MX4_BINS / 64];
+#pragma unroll
+            for (uint32_t i = 0; i < MX4_BINS / 64; i++) sum += own[i] = B.bin(b0 + i);
             uint32_t before = sum;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -390,11 +394,15 @@ template <typename F> __device__ __forceinline__ uint32_t mx4_kth(Mx4Bins &B, ui
             }
             before -= sum;
             if (before < need && need <= before + sum) {
-                uint32_t i = 0;
-                while (before + B.hist[b0 + i] < need) before += B.hist[b0 + i++];
-                B.pick = b0 + i;
-                B.left = need - before;
-                B.in = B.hist[b0 + i];
+                uint32_t pick = 0, left = 0, in = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < MX4_BINS / 64; i++) {
+                    if (before < need) pick = b0 + i, left = need - before, in = own[i];
+                    before += own[i];
+                }
+                B.pick = pick;
+                B.left = left;
+                B.in = in;
             }
         }
         __syncthreads();
@@ -407,6 +415,81 @@ template <typename F> __device__ __forceinline__ uint32_t mx4_kth(Mx4Bins &B, ui
         if (shift == 0 || in <= 8 + k / 16) break;
     }
     return hi;
+}
+// The ranks of n <= room keys (MX4_NONE: none, without a rank) by counting: bins of equal width between the least and the largest score,
+// keys in their bins' order, and a key's place in its bin by comparison with the others there.  False, and nothing done, when a bin
+// holds too many (scores that crowd): then they are sorted.  All threads; emit(rank, key).
+constexpr uint32_t MX4_CROWD = 128;
+template <typename F> __device__ __forceinline__ bool mx4_ranked(Mx4Bins &B, const uint64_t *keys, uint32_t n, uint64_t *binned, F emit) {
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < MX4_BINS + MX4_BINS / 32; i += blockDim.x) B.hist[i] = 0;
+    if (threadIdx.x == 0) {
+        B.lo = 0xFFFFFFFFu;
+        B.hi = 0;
+        B.in = 0;
+    }
+    __syncthreads();
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+        if (keys[i] != ~0ull) {
+            lo = min(lo, (uint32_t)(keys[i] >> 32));
+            hi = max(hi, (uint32_t)(keys[i] >> 32));
+        }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor(lo, o));
+        hi = max(hi, (uint32_t)__shfl_xor(hi, o));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        atomicMin(&B.lo, lo);
+        atomicMax(&B.hi, hi);
+    }
+    __syncthreads();
+    lo = B.lo;
+    hi = B.hi;
+    if (lo > hi) return true;   // no key
+    const uint32_t range = hi - lo;
+    const int shift = range < MX4_BINS ? 0 : 32 - __builtin_clz(range) - 11;
+    const auto bin_of = [&](uint64_t key) { return ((uint32_t)(key >> 32) - lo) >> shift; };
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+        if (keys[i] != ~0ull) atomicAdd(&B.bin(bin_of(keys[i])), 1u);
+    __syncthreads();
+    if (threadIdx.x < 64) {   // counts -> first places
+        const uint32_t b0 = threadIdx.x * (MX4_BINS / 64);
+        uint32_t sum = 0, most = 0, own[MX4_BINS / 64];
+#pragma unroll
+        for (uint32_t i = 0; i < MX4_BINS / 64; i++) {
+            sum += own[i] = B.bin(b0 + i);
+            most = max(most, own[i]);
+        }
+        uint32_t before = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(before, o);
+            if ((int)threadIdx.x >= o) before += t;
+        }
+        before -= sum;
+#pragma unroll
+        for (uint32_t i = 0; i < MX4_BINS / 64; i++) {
+            B.bin(b0 + i) = before;
+            before += own[i];
+        }
+        atomicMax(&B.in, most);
+    }
+    __syncthreads();
+    if (B.in > MX4_CROWD) return false;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+        if (keys[i] != ~0ull) binned[atomicAdd(&B.bin(bin_of(keys[i])), 1u)] = keys[i];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const uint64_t key = keys[i];
+        if (key == ~0ull) continue;
+        const uint32_t bin = bin_of(key), first = bin ? B.bin(bin - 1) : 0, last = B.bin(bin);   // (a bin's place is now its end)
+        uint32_t rank = first;
+        for (uint32_t j = first; j < last; j++) rank += binned[j] < key;
+        emit(rank, key);
+    }
+    return true;
 }
 struct Mx4Threshold {
     const float *minima;
@@ -467,19 +550,29 @@ template <typename F> __device__ __forceinline__ void mx4_unpack8(uint32_t codes
     const mx4_f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.f, 3);
     use(0, a[0]), use(1, a[1]), use(2, b[0]), use(3, b[1]), use(4, c[0]), use(5, c[1]), use(6, d[0]), use(7, d[1]);
 }
-// this lane's share of a row's sums: blocks first, first + by, ...   In a block the sums are whole numbers (of 1/16): exact.
-template <int BITS> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact &E, const char *tile, uint32_t col, const char *panel, uint32_t r,
-                                                                 uint32_t first, uint32_t by, double &dot, double &xx) {
+// this lane's share of R rows' sums: blocks first, first + by, ...   In a block the sums are whole numbers (of 1/16): exact.
+template <int BITS, int R> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact &E, const char *tile, uint32_t col, const uint32_t (&row)[R],
+                                                                        uint32_t first, uint32_t by, double (&dot)[R], double (&xx)[R]) {
     const uint32_t nb = E.rows.ks * 2;
-    dot = 0;
-    xx = 0;
+    const char *panel[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        panel[i] = E.rows.at(row[i] >> 5);
+        dot[i] = 0;
+        xx[i] = 0;
+    }
     for (uint32_t b = first; b < nb; b += by) {
-        const uint32_t s = b >> 1, half = b & 1, ra = r + 32 * half, qa = col + 32 * half;
-        const mx4_u4 x = *reinterpret_cast<const mx4_u4 *>(panel + (size_t)s * 1024 + ra * 16);
-        const uint32_t bx = (uint8_t)panel[(size_t)E.rows.ks * 1024 + (s >> 2) * 256 + ra * 4 + (s & 3)];
+        const uint32_t s = b >> 1, half = b & 1, qa = col + 32 * half;
+        mx4_u4 x[R];
+        uint32_t bx[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {   // (all rows' loads are under way before the first is used)
+            const uint32_t ra = (row[i] & 31) + 32 * half;
+            x[i] = *reinterpret_cast<const mx4_u4 *>(panel[i] + (size_t)s * 1024 + ra * 16);
+            bx[i] = (uint8_t)panel[i][(size_t)E.rows.ks * 1024 + (s >> 2) * 256 + ra * 4 + (s & 3)];
+        }
         const mx4_u4 lo = *reinterpret_cast<const mx4_u4 *>(tile + (size_t)s * 1024 + qa * 16);
         const uint32_t bq = (uint8_t)tile[(size_t)E.rows.kg * (BITS == 6 ? 4 * 1536 : 4 * 1024) + (s >> 2) * 256 + qa * 4 + (s & 3)];
-        float d = 0, sq = 0;
         mx4_f32 qv;
         if constexpr (BITS == 6) {
             const mx4_u2 hi = *reinterpret_cast<const mx4_u2 *>(tile + (size_t)E.rows.kg * 4096 + (size_t)s * 512 + qa * 8);
@@ -489,14 +582,18 @@ template <int BITS> __device__ __forceinline__ void mx4_row_sums(const Mx4Exact 
             for (int w = 0; w < 4; w++) mx4_unpack8(lo[w], [&](int j, float v) { qv[8 * w + j] = v; });
         }
 #pragma unroll
-        for (int w = 0; w < 4; w++)
-            mx4_unpack8(x[w], [&](int j, float v) {
-                d = __fmaf_rn(v, qv[8 * w + j], d);
-                sq = __fmaf_rn(v, v, sq);
-            });
-        const double nan = __builtin_nan("");
-        dot += bx == 255 || bq == 255 ? nan : (double)d * mx4_pow2((int)bx + (int)bq - 254);
-        xx += bx == 255 ? nan : (double)sq * mx4_pow2(2 * (int)bx - 254);
+        for (int i = 0; i < R; i++) {
+            float d = 0, sq = 0;
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                mx4_unpack8(x[i][w], [&](int j, float v) {
+                    d = __fmaf_rn(v, qv[8 * w + j], d);
+                    sq = __fmaf_rn(v, v, sq);
+                });
+            const double nan = __builtin_nan("");
+            dot[i] += bx[i] == 255 || bq == 255 ? nan : (double)d * mx4_pow2((int)bx[i] + (int)bq - 254);
+            xx[i] += bx[i] == 255 ? nan : (double)sq * mx4_pow2(2 * (int)bx[i] - 254);
+        }
     }
 }
 __device__ __forceinline__ float mx4_final(uint32_t metric, double dot, double xx, double qq) {
@@ -506,20 +603,30 @@ __device__ __forceinline__ float mx4_final(uint32_t metric, double dot, double x
 }
 // lanes on one row: one for each of its blocks, 4 to 32
 __host__ __device__ inline uint32_t mx4_row_lanes(uint32_t ks) { return ks <= 2 ? 4u : (ks <= 4 ? 8u : (ks <= 8 ? 16u : 32u)); }
-template <int BITS> __device__ __forceinline__ float mx4_exact_score(const Mx4Exact &E, uint32_t q, uint64_t row, uint32_t lanes) {
-    double dot, xx;
-    mx4_row_sums<BITS>(E, E.tiles + (size_t)(q >> 5) * E.qtile_bytes, q & 31, E.rows.at(row >> 5), (uint32_t)(row & 31), threadIdx.x & (lanes - 1), lanes, dot, xx);
-    for (int o = (int)lanes / 2; o; o >>= 1) {
-        dot += __shfl_xor(dot, o);
-        xx += __shfl_xor(xx, o);
+template <int BITS, int R> __device__ __forceinline__ void mx4_exact_scores(const Mx4Exact &E, uint32_t q, const uint32_t (&row)[R], uint32_t lanes, float (&score)[R]) {
+    double dot[R], xx[R];
+    mx4_row_sums<BITS, R>(E, E.tiles + (size_t)(q >> 5) * E.qtile_bytes, q & 31, row, threadIdx.x & (lanes - 1), lanes, dot, xx);
+    const double qq = E.qsq[q];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        for (int o = (int)lanes / 2; o; o >>= 1) {
+            dot[i] += __shfl_xor(dot[i], o);
+            xx[i] += __shfl_xor(xx[i], o);
+        }
+        score[i] = mx4_final(E.metric, dot[i], xx[i], qq);
     }
-    return mx4_final(E.metric, dot, xx, E.qsq[q]);
+}
+template <int BITS> __device__ __forceinline__ float mx4_exact_score(const Mx4Exact &E, uint32_t q, uint32_t row, uint32_t lanes) {
+    const uint32_t rows[1] = {row};
+    float s[1];
+    mx4_exact_scores<BITS, 1>(E, q, rows, lanes, s);
+    return s[0];
 }
 // rows first .. first + m - 1, or ids[0 .. m)
 template <int BITS> static __global__ __launch_bounds__(256) void k_mx4_exact_rows(Mx4Exact E, const uint32_t *ids, uint64_t first, uint64_t m, float *out) {
     const uint32_t lanes = mx4_row_lanes(E.rows.ks), at_once = 256 / lanes, me = threadIdx.x / lanes;
     for (uint64_t i = (uint64_t)blockIdx.x * at_once + me; i < m; i += (uint64_t)gridDim.x * at_once) {
-        const float s = mx4_exact_score<BITS>(E, 0, ids ? ids[i] : first + i, lanes);
+        const float s = mx4_exact_score<BITS>(E, 0, ids ? ids[i] : (uint32_t)(first + i), lanes);
         if ((threadIdx.x & (lanes - 1)) == 0) out[i] = s;
     }
 }
@@ -531,13 +638,15 @@ __device__ __forceinline__ uint64_t mx4_pack(float s, uint32_t row) {
     if (!(s == s)) return MX4_NONE;
     return (uint64_t)mx4_key(s == 0.f ? 0.f : s) << 32 | row;   // (-0 and 0 are equal)
 }
-// ascending bitonic sort of n (a power of two) keys in LDS by the whole workgroup
+// ascending bitonic sort of n (a power of two) keys in LDS by the whole workgroup.  Thread t takes pair t: with strides to 64 a wave's
+// pairs are 128 keys that nobody else touches, so that only longer strides need the workgroup's barrier.
 __device__ __forceinline__ void mx4_sort(uint64_t *k, uint32_t n) {
+    __syncthreads();
     for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t stride = size >> 1; stride; stride >>= 1) {
-            __syncthreads();
+        for (int s = 30 - __builtin_clz(size); s >= 0; s--) {
+            const uint32_t stride = 1u << s;
             for (uint32_t t = threadIdx.x; t < n / 2; t += blockDim.x) {
-                const uint32_t lo = (t / stride) * stride * 2 + t % stride, hi = lo + stride;
+                const uint32_t lo = (t >> s << (s + 1)) + (t & (stride - 1)), hi = lo + stride;
                 const bool up = (lo & size) == 0;
                 const uint64_t a = k[lo], b = k[hi];
                 if ((a > b) == up) {
@@ -545,6 +654,8 @@ __device__ __forceinline__ void mx4_sort(uint64_t *k, uint32_t n) {
                     k[hi] = a;
                 }
             }
+            if (stride > 64 || (stride == 1 && size >= 128)) __syncthreads();   // (the next stride is above 64, or this one was)
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     __syncthreads();
 }
@@ -580,8 +691,8 @@ __device__ __forceinline__ void mx4_keep_add(const Mx4Keep &K, uint64_t key, uin
 }
 struct Mx4Select {
     Mx4Exact E;
-    uint32_t nq, k, segment;
-    const uint32_t *counts;     // [nq][MX4_SEGMENTS]
+    uint32_t nq, k, segments, segment;
+    const uint32_t *counts;     // [nq][segments]
     const Mx4Cand *cand;
     const float *minima, *qnorm;   // DENSE: [nq][n] upper bounds
     float slack;
@@ -589,6 +700,11 @@ struct Mx4Select {
     uint64_t *again_limit;      // [nq] ... which then needs nothing above this
     int64_t *ids;               // [nq][k]
     float *scores;
+    // k_mx4_finish: workgroups a query, what each of them leaves for the last one, and how many of them have
+    uint32_t shares, room;
+    uint64_t *share;            // [nq][shares][room]
+    uint32_t *share_n;          // [nq][shares]
+    uint32_t *done;             // [nq]
     // k_mx4_again: slices of the table per query and their results
     uint32_t slices;
     uint64_t *part;             // [nq][slices][k]
@@ -601,35 +717,42 @@ __device__ __forceinline__ void mx4_emit(const Mx4Select &S, uint32_t q, const u
         S.scores[(size_t)q * S.k + i] = key == MX4_NONE ? -1.f : mx4_unkey((uint32_t)(key >> 32));
     }
 }
-// One workgroup a query: of its candidates only those whose lower bound is at or below the k-th smallest upper bound (little more
-// than k) are scored exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds
-// the probe's.
+// Of a query's candidates only those whose lower bound is at or below the k-th smallest upper bound (little more than k) are scored
+// exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds the probe's.  Few
+// queries with many rows to score: `shares` workgroups a query, each with every shares-th 64 candidates; the last one to end joins them.
 constexpr uint32_t MX4_FINISH = 1024;
+constexpr uint32_t MX4_SHARES = 16;     // most workgroups a query
 constexpr uint32_t MX4_LISTED = 6144;   // candidates kept in LDS; more are read from memory every time
 template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k_mx4_finish(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ Mx4Bins bins;
-    __shared__ uint32_t up_s[MX4_LISTED];   // keys of the upper bounds
+    __shared__ __attribute__((aligned(8))) uint32_t up_s[MX4_LISTED];   // keys of the upper bounds
     __shared__ uint32_t rows_s[2 * MX4_FINISH];
-    __shared__ uint32_t first_s[MX4_SEGMENTS + 1], n_s, rows_n;
+    __shared__ uint32_t first_s[MX4_SEGMENTS_MAX + 1], n_s, rows_n, last_s;
     __shared__ uint64_t limit_s;
     __shared__ int over_s;
-    const uint32_t q = blockIdx.x;
+    const uint32_t q = blockIdx.x, me = blockIdx.y;
     const Mx4Keep K{keys, &n_s, &limit_s, S.k};
     if (threadIdx.x < 64) {
+        constexpr int EACH = MX4_SEGMENTS_MAX / 64;
         bool over = false;
-        uint32_t sum = 0;
-        if (!DENSE && threadIdx.x < MX4_SEGMENTS) {
-            sum = S.counts[q * MX4_SEGMENTS + threadIdx.x];
-            over = sum > S.segment;
-            sum = min(sum, S.segment);
+        uint32_t sum = 0, own[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const uint32_t seg = threadIdx.x * EACH + i, have = !DENSE && seg < S.segments ? S.counts[(size_t)q * S.segments + seg] : 0;
+            over |= have > S.segment;
+            sum += min(have, S.segment);
+            own[i] = sum;
         }
+        uint32_t before = sum;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t t = __shfl_up(sum, o);
-            if ((int)threadIdx.x >= o) sum += t;
+            const uint32_t t = __shfl_up(before, o);
+            if ((int)threadIdx.x >= o) before += t;
         }
-        if (threadIdx.x < MX4_SEGMENTS) first_s[threadIdx.x + 1] = sum;
+        before -= sum;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) first_s[threadIdx.x * EACH + i + 1] = before + own[i];
         const bool any = __any(over);
         if (threadIdx.x == 0) {
             first_s[0] = 0;
@@ -640,16 +763,20 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         }
     }
     __syncthreads();
-    const uint32_t n = DENSE ? (uint32_t)S.E.rows.n : first_s[MX4_SEGMENTS];
+    const uint32_t n = DENSE ? (uint32_t)S.E.rows.n : first_s[MX4_SEGMENTS_MAX];
     const auto listed = [&](uint32_t i) -> const Mx4Cand & {   // candidate i of all segments
         uint32_t seg = 0;
 #pragma unroll
-        for (uint32_t step = MX4_SEGMENTS / 2; step; step >>= 1)
+        for (uint32_t step = MX4_SEGMENTS_MAX / 2; step; step >>= 1)
             if (first_s[seg + step] <= i) seg += step;
-        return S.cand[((size_t)q * MX4_SEGMENTS + seg) * S.segment + (i - first_s[seg])];
+        return S.cand[((size_t)q * S.segments + seg) * S.segment + (i - first_s[seg])];
     };
+    const float y = S.qnorm[q];
+    const auto bounds = [&](const Mx4Cand &c, float &low, float &up) { mx4_bounds(S.E.metric, c.dot, c.x, y, S.slack, low, up); };
     const auto up_key = [&](uint64_t i) {
-        const float up = DENSE ? S.minima[(size_t)q * S.E.rows.n + i] : listed((uint32_t)i).up;
+        float up, low;
+        if constexpr (DENSE) up = S.minima[(size_t)q * S.E.rows.n + i];
+        else bounds(listed((uint32_t)i), low, up);
         return up == up ? mx4_key(up) : MX4_KEY_INF;
     };
     uint32_t key = MX4_KEY_INF;
@@ -664,34 +791,47 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     const float most = mx4_unkey(key);
     // rows worth an exact score, collected and scored MX4_FINISH or more at a time
     const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
-    for (uint32_t i0 = 0; i0 < n; i0 += MX4_FINISH) {
-        const uint32_t i = i0 + threadIdx.x;
-        if (i < n) {
+    const uint32_t mine = (((n + 63) / 64 + S.shares - 1 - me) / S.shares) * 64;   // this workgroup's candidates, the last 64 perhaps fewer
+    for (uint32_t j0 = 0; j0 < mine; j0 += MX4_FINISH) {
+        const uint32_t j = j0 + threadIdx.x, i = ((j >> 6) * S.shares + me) * 64 + (j & 63);
+        if (j < mine && i < n) {
             uint32_t row = i;
             float low;
             if constexpr (DENSE) {
-                const float up = S.minima[(size_t)q * S.E.rows.n + i], y = S.qnorm[q];
+                const float up = S.minima[(size_t)q * S.E.rows.n + i];
                 const float x = reinterpret_cast<const float *>(S.E.rows.at(i / 32) + S.E.rows.panel - 128)[i & 31];
                 low = mx4_low(S.E.metric, up, x, y, S.slack);
             } else {
                 const Mx4Cand &c = listed(i);
+                float up;
                 row = c.row;
-                low = c.low;
+                bounds(c, low, up);
             }
             if (!(low > most)) rows_s[atomicAdd(&rows_n, 1u)] = row;
         }
         __syncthreads();
         const uint32_t m = rows_n;
-        if (m <= MX4_FINISH && i0 + MX4_FINISH < n) {   // (the same for all threads)
+        if (m <= MX4_FINISH && j0 + MX4_FINISH < mine) {   // (the same for all threads)
             __syncthreads();
             continue;
         }
         if (n_s + m > MX4_KEEP) mx4_keep_cut(K);
         const uint32_t base = n_s;
-        for (uint32_t r = threadIdx.x / lanes; r < m; r += at_once) {
-            const float s = mx4_exact_score<BITS>(S.E, q, rows_s[r], lanes);
-            if ((threadIdx.x & (lanes - 1)) == 0) keys[base + r] = mx4_pack(s, rows_s[r]);
-        }
+        const auto score = [&](auto each) {
+            constexpr int R = decltype(each)::value;
+            for (uint32_t r0 = threadIdx.x / lanes; r0 < m; r0 += R * at_once) {
+                uint32_t row[R];
+                float s[R];
+#pragma unroll
+                for (int i = 0; i < R; i++) row[i] = rows_s[min(r0 + i * at_once, m - 1)];
+                mx4_exact_scores<BITS, R>(S.E, q, row, lanes, s);
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    if ((threadIdx.x & (lanes - 1)) == 0 && r0 + i * at_once < m) keys[base + r0 + i * at_once] = mx4_pack(s[i], row[i]);
+            }
+        };
+        if (m <= at_once) score(std::integral_constant<int, 1>{});
+        else score(std::integral_constant<int, 2>{});
         __syncthreads();
         if (threadIdx.x == 0) {
             n_s = base + m;
@@ -699,15 +839,74 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         }
         __syncthreads();
     }
+    if (S.shares > 1) {
+        __syncthreads();
+        if (n_s > S.room) mx4_keep_cut(K);   // (room >= k)
+        uint64_t *to = S.share + ((size_t)q * S.shares + me) * S.room;
+        for (uint32_t i = threadIdx.x; i < n_s; i += MX4_FINISH) __hip_atomic_store(&to[i], keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) __hip_atomic_store(&S.share_n[q * S.shares + me], n_s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (threadIdx.x == 0) {   // (one thread's fences, on both sides, hold for the workgroup: the barriers are between)
+            __threadfence();
+            last_s = atomicAdd(&S.done[q], 1u) == S.shares - 1;
+            __threadfence();
+            n_s = 0;
+            limit_s = MX4_NONE;
+        }
+        __syncthreads();
+        if (!last_s) return;
+        if (threadIdx.x <= MX4_SHARES) first_s[threadIdx.x] = 0;
+        __syncthreads();
+        if (threadIdx.x < S.shares) {
+            const uint32_t m = __hip_atomic_load(&S.share_n[q * S.shares + threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (uint32_t w = threadIdx.x + 1; w <= S.shares; w++) atomicAdd(&first_s[w], m);
+        }
+        __syncthreads();
+        const uint32_t total = first_s[S.shares];
+        const uint64_t *from = S.share + (size_t)q * S.shares * S.room;
+        for (uint32_t i0 = 0; i0 < total; i0 += MX4_FINISH) {
+            const uint32_t i = i0 + threadIdx.x;
+            uint32_t w = 0;
+            while (w + 1 < S.shares && first_s[w + 1] <= i) w++;
+            const bool have = i < total;
+            mx4_keep_add(K, have ? __hip_atomic_load(&from[(size_t)w * S.room + (i - first_s[w])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE, MX4_FINISH);
+        }
+    }
+    __syncthreads();
+    const uint32_t have = n_s;
+    const auto conclude = [&](uint32_t got, uint64_t kth) {   // one thread
+        S.again[q] = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || (!DENSE && got < min((uint64_t)S.k, S.E.rows.n)));
+        S.ticket[q] = 0;
+        S.again_limit[q] = got >= S.k ? kth : MX4_NONE - 1;
+    };
+    if (have > 256 && 2 * have <= MX4_LISTED) {   // (up_s is free by now)
+        if (threadIdx.x == 0) {
+            rows_n = 0;
+            limit_s = MX4_NONE;
+        }
+        const bool done = mx4_ranked(bins, keys, have, reinterpret_cast<uint64_t *>(up_s), [&](uint32_t rank, uint64_t key) {
+            if (rank < S.k) {
+                S.ids[(size_t)q * S.k + rank] = (int64_t)(uint32_t)key;
+                S.scores[(size_t)q * S.k + rank] = mx4_unkey((uint32_t)(key >> 32));
+                if (rank == S.k - 1) limit_s = key;
+            }
+            atomicAdd(&rows_n, 1u);
+        });
+        __syncthreads();
+        if (done) {
+            const uint32_t got = rows_n;
+            for (uint32_t i = got + threadIdx.x; i < S.k; i += MX4_FINISH) {
+                S.ids[(size_t)q * S.k + i] = -1;
+                S.scores[(size_t)q * S.k + i] = -1.f;
+            }
+            if (threadIdx.x == 0) conclude(got, limit_s);
+            return;
+        }
+    }
     mx4_keep_cut(K);
     uint32_t got = n_s;
     while (got && keys[got - 1] == MX4_NONE) got--;   // NaN scores
-    const bool again = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || (!DENSE && got < min((uint64_t)S.k, S.E.rows.n)));
-    if (threadIdx.x == 0) {
-        S.again[q] = again;
-        S.ticket[q] = 0;
-        S.again_limit[q] = got >= S.k ? keys[S.k - 1] : MX4_NONE - 1;
-    }
+    if (threadIdx.x == 0) conclude(got, keys[S.k - 1]);
     mx4_emit(S, q, keys, got);
 }
 // Queries whose candidates overflowed (many rows as near as the k-th), or were fewer than k: every row scored exactly, `slices`
@@ -729,7 +928,7 @@ template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx
         const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = 512 / lanes;
         for (uint64_t r0 = a; r0 < b; r0 += at_once) {
             const uint64_t row = r0 + threadIdx.x / lanes;
-            const float s = mx4_exact_score<BITS>(S.E, q, min(row, n - 1), lanes);
+            const float s = mx4_exact_score<BITS>(S.E, q, (uint32_t)min(row, n - 1), lanes);
             mx4_keep_add(K, (threadIdx.x & (lanes - 1)) == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
         }
         mx4_keep_cut(K);

@@ -57,11 +57,7 @@ struct Mx4Queue {
             const uint32_t q = e[0], row = e[1], list = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
             const float x = reinterpret_cast<const float *>(P.rows.at(row >> 5) + P.rows.panel - 128)[row & 31];
             const uint32_t at = atomicAdd(&P.counts[list], 1u);
-            if (at < P.segment) {
-                Mx4Cand c{row, 0.f, 0.f, 0u};
-                mx4_bounds(P.metric, __uint_as_float(e[2]), x, norm[q], P.slack, c.low, c.up);
-                P.cand[(size_t)list * P.segment + at] = c;
-            }
+            if (at < P.segment) P.cand[(size_t)list * P.segment + at] = Mx4Cand{row, __uint_as_float(e[2]), x};
         }
         n = 0;
     }
@@ -130,7 +126,7 @@ template <int M> __device__ __forceinline__ float mx4_probe_bound(float best, fl
     return u == u ? u : inf;
 }
 
-// The ring of k_mx4_ring: the workgroup's four waves bring every panel into LDS together, a KiB at a time in turn, and `stages` panels
+// The ring of k_mx4_ring: the workgroup's waves bring every panel into LDS together, a KiB at a time in turn, and `stages` panels
 // are under way or in use.  Constants by the chunks of a panel (codes, scales, norms in whole KiB); the stages fill the LDS beside the queues.
 constexpr int mx4_ring_pieces(int nb) { return (4 * nb * 1024 + nb * 256 + 128 + 1023) / 1024; }
 constexpr int mx4_ring_stages(int nb) { return nb == 1 ? 16 : (nb == 2 ? 15 : (nb == 3 ? 10 : 7)); }
@@ -142,6 +138,16 @@ __device__ __forceinline__ void mx4_to_lds(uint32_t lds, uint32_t offset, uint64
 }
 template <int N> __device__ __forceinline__ void mx4_wait_loads() {   // until at most N of the wave's memory operations are under way
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// The same two for some of the waves (wave < first), the branches inside: to the compiler they are one straight line, and what
+// stands before and behind them may be mixed.
+template <int N> __device__ __forceinline__ void mx4_to_lds_first(int wave, uint32_t lds, uint32_t offset, uint64_t base) {
+    asm volatile("s_cmp_lt_i32 %0, %1\n\ts_cbranch_scc0 .Lmx4_none_%=\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %4\n.Lmx4_none_%=:"
+                 ::"s"(wave), "n"(N), "s"(lds), "v"(offset), "s"(base) : "memory", "scc");
+}
+template <int FIRST, int MANY, int FEW> __device__ __forceinline__ void mx4_wait_loads_first(int wave) {   // at most MANY or FEW
+    asm volatile("s_cmp_lt_i32 %0, %1\n\ts_cbranch_scc0 .Lmx4_few_%=\n\ts_waitcnt vmcnt(%2)\n\ts_branch .Lmx4_there_%=\n.Lmx4_few_%=:\n\ts_waitcnt vmcnt(%3)\n.Lmx4_there_%=:"
+                 ::"s"(wave), "n"(FIRST), "n"(MANY), "n"(FEW) : "memory", "scc");
 }
 // registers of a wave, about: what its operands, sums and panel in flight need
 constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
@@ -381,7 +387,12 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
 
 // The same passes for 65 to 256 queries against rows of at most 1024 elements.  Four waves, QT tiles each, take every panel together; it
 // comes through LDS, so that the memory's latency is covered by a ring of panels and not by registers, which hold the operands.  One
-// wave a SIMD: a panel's comparisons (prev) are made while the next one's matrix instructions run, a few between every two of them.
+// wave a SIMD: the comparisons of the panel before are made between the matrix instructions of this one, whose last chunk covers the
+// barrier and the first reads of the next.  Survivors go straight to the workgroup's own part of their query's list (a counter in LDS, a
+// store that nobody waits for): a queue's flush would wait for the ring's loads as well.
+// 1M x 1024, few survivors: 128 queries 105 us (5.2 TB/s: the memory), 256 queries 160 us (537 GFLOP at 3.4 PFLOP/s; the chip's clock
+// falls to 1.7 GHz under it, and with less work beside the matrix instructions hardly rises).  Each panel with survivors costs its
+// wave some 800 cycles: 256 queries, top-100: 245 us.  Eight waves of one tile each read the LDS twice as often: 207 us.
 template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_bounds__(256, 1) void k_mx4_ring(Mx4Scan P) {
     extern __shared__ char shared[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
@@ -390,15 +401,17 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
     constexpr uint32_t BLOCK_Q = MX4_RING_WAVES * QT * 32;
     const uint32_t block_q0 = blockIdx.y * BLOCK_Q, q0 = block_q0 + wave * QT * 32, ks = P.rows.ks;
     const char *tiles = P.tiles + (size_t)(q0 / 32) * P.qtile_bytes;
-    float *yn_b = reinterpret_cast<float *>(shared + mx4_ring_bytes(NB));
-    Mx4Queue queue{reinterpret_cast<mx4_u4 *>(yn_b + 2 * BLOCK_Q) + wave * MX4_QUEUE, 0};
+    float *yn_b = reinterpret_cast<float *>(shared + mx4_ring_bytes(NB));      // PROBE: |q|, 1 / |q|
+    uint32_t *taken = reinterpret_cast<uint32_t *>(yn_b);                      // FILTER: candidates of each query so far
     for (uint32_t i = threadIdx.x; i < BLOCK_Q; i += 256) {
-        const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
-        yn_b[i] = y;
-        yn_b[BLOCK_Q + i] = 1.f / y;
+        if constexpr (MODE == MX4_FILTER) taken[i] = 0;
+        else {
+            const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
+            yn_b[i] = y;
+            yn_b[BLOCK_Q + i] = 1.f / y;
+        }
     }
     __syncthreads();
-    const float *norms = yn_b - block_q0;   // by query
     Mx4Operand<BITS> op[QT][4 * NB];
     int opsc[QT][NB];
     float alpha[QT], beta[QT];   // FILTER: the threshold; PROBE: |q|, 1 / |q|
@@ -415,8 +428,8 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
             alpha[q] = l.x;
             beta[q] = l.y;
         } else {
-            alpha[q] = norms[me];
-            beta[q] = norms[BLOCK_Q + me];
+            alpha[q] = yn_b[me - block_q0];
+            beta[q] = yn_b[BLOCK_Q + me - block_q0];
         }
     }
     const uint32_t n_take = (uint32_t)P.n_take;
@@ -424,20 +437,24 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
     if (w >= n_take) return;
     const auto panel_of = [&](uint32_t i) -> uint64_t { return MODE == MX4_PROBE ? (i * P.every) >> 24 : i; };
     uint32_t ahead = w, fill = 0, use = 0;   // the panel to request next, the stage it goes to, the stage in use
-    const auto request = [&]() {   // (past the end the last panel again, so that the count of what is under way stays the same)
-        const uint64_t from = P.rows.uniform_at(panel_of(min(ahead, n_take - 1)));
+    // (past the end the last panel again, so that the count of what is under way stays the same)
+    const auto requested = [&]() -> uint64_t { return P.rows.uniform_at(panel_of(min(ahead, n_take - 1))); };
+    const auto request = [&](uint64_t from) {
         const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)shared + fill * STAGE;
 #pragma unroll
-        for (int i = 0; i <= EACH; i++) {
-            if (i == EACH && wave >= OVER) break;
+        for (int i = 0; i < EACH; i++) {
             const uint32_t offset = (i * MX4_RING_WAVES + wave) * 1024;
             mx4_to_lds(to + offset, min(offset + lane * 16, P.rows.panel - 16), from);
+        }
+        if constexpr (OVER != 0) {
+            const uint32_t offset = (EACH * MX4_RING_WAVES + wave) * 1024;
+            mx4_to_lds_first<OVER>(wave, to + offset, min(offset + lane * 16, P.rows.panel - 16), from);
         }
         ahead += gridDim.x;
         fill = fill + 1 == STAGES ? 0 : fill + 1;
     };
 #pragma unroll 1
-    for (int i = 0; i < STAGES - 1; i++) request();
+    for (int i = 0; i < STAGES - 1; i++) request(requested());
 
     struct Panel {
         mx4_f16 acc[QT], x;   // dots, |x|
@@ -465,14 +482,44 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
     };
     const auto conclude = [&](const Panel &p) {
         if constexpr (MODE == MX4_FILTER) {
-            const bool odd = M == MX4_COSINE && __any(least < MX4_SHORT);
+            const uint64_t row0 = row0_of(p);
+            uint64_t any[QT], all = 0;
+#pragma unroll
+            for (int q = 0; q < QT; q++) all |= any[q] = __ballot(most[q] >= beta[q]);
+            // vectors too short for fp32 arithmetic go on to the exact one, zero vectors (score NaN) do not; the last panel's padding
+            bool odd = row0 + 32 > P.rows.n;
+            if (M == MX4_COSINE && __any(least < MX4_SHORT)) {
+                asm volatile("");   // (or the compiler computes it every time)
+                bool some = false;
+#pragma unroll
+                for (int v = 0; v < 16; v++) some |= p.x[v] < MX4_SHORT && p.x[v] > 0.f;
+                odd |= __any(some);
+            }
+            if (all == 0 && !odd) return;
 #pragma unroll
             for (int q = 0; q < QT; q++) {
-                if (!__any(most[q] >= beta[q]) && !odd) continue;
-                const uint64_t row0 = row0_of(p);
-                uint32_t mask = mx4_survivors<M>(p.acc[q], p.x, alpha[q], beta[q]);
-                if (row0 + 32 > P.rows.n) mask &= mx4_rows_below(row0 + 4 * half, P.rows.n);
-                queue.push(P, norms, lane, q0 + q * 32 + col, (uint32_t)row0, mask, p.acc[q]);
+                if (any[q] == 0 && !odd) continue;
+                const uint32_t me = wave * QT * 32 + q * 32 + col;
+                Mx4Cand *list = P.cand + ((size_t)(block_q0 + me) * P.segments + blockIdx.x) * P.segment;
+                uint32_t rows = 0, mask = 0;   // rows with a survivor in some lane, this lane's: without branches, which would cost more
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const bool hit = mx4_held<M>(p.acc[q][v], p.x[v], alpha[q]) >= beta[q];
+                    mask |= hit ? 1u << v : 0u;
+                    rows |= __ballot(hit) ? 1u << v : 0u;
+                }
+                if (odd) {
+                    asm volatile("");
+                    rows = 0xFFFFu;
+                    mask = mx4_survivors<M>(p.acc[q], p.x, alpha[q], beta[q]) & mx4_rows_below(row0 + 4 * half, P.rows.n);
+                }
+                uint32_t at = mask ? atomicAdd(&taken[me], (uint32_t)__builtin_popcount(mask)) : 0;
+                while (rows) {
+                    const int v = __builtin_ctz(rows);
+                    rows &= rows - 1;
+                    if (mask >> v & 1 && at < P.segment) list[at] = Mx4Cand{(uint32_t)row0 + 8 * (v >> 2) + 4 * half + (v & 3), p.acc[q][v], p.x[v]};
+                    at += mask >> v & 1;
+                }
             }
         } else {
 #pragma unroll
@@ -489,23 +536,28 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
             for (int v = 0; v < 16; v++) h[v] = mx4_probe_row<M>(p.x[v], row0 + 8 * (v >> 2) + 4 * half + (v & 3) >= P.rows.n);
         }
     };
-    // one panel: its dots into p, and q's comparisons
-    const auto round = [&](Panel &p, Panel &q) {
-        // this wave's part of the stage is there; behind the barrier everybody's is, and nobody reads the stage before it any more
-        if (wave < OVER) mx4_wait_loads<(STAGES - 2) * (EACH + 1)>();
-        else mx4_wait_loads<(STAGES - 2) * EACH>();
-        asm volatile("s_barrier" ::: "memory");
-        request();
-        const char *stage = shared + use * STAGE;
-        use = use + 1 == STAGES ? 0 : use + 1;
-        prepare(q);
-        Mx4Chunk buf[2];
-        const auto take = [&](int j) {
+    Mx4Chunk buf[2];
+    const char *stage = shared;
+    const auto take = [&](Mx4Chunk &c, int j) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) buf[j & 1].a[i] = reinterpret_cast<const mx4_i4 *>(stage + min(4u * j + i, ks - 1) * 1024)[lane];
-            buf[j & 1].sc = reinterpret_cast<const int *>(stage + ks * 1024 + j * 256)[lane];
-        };
-        take(0);
+        for (int i = 0; i < 4; i++) c.a[i] = reinterpret_cast<const mx4_i4 *>(stage + min(4u * j + i, ks - 1) * 1024)[lane];
+        c.sc = reinterpret_cast<const int *>(stage + ks * 1024 + j * 256)[lane];
+    };
+    // this wave's part of the next panel is there, with AFTER panels behind it under way; beyond the barrier everybody's is, and
+    // nobody reads the panel before this one any more: what comes next goes into its stage
+    const auto arrive = [&](auto after) {
+        constexpr int AFTER = decltype(after)::value;
+        mx4_wait_loads_first<OVER, AFTER *(EACH + 1), AFTER * EACH>(wave);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    arrive(std::integral_constant<int, STAGES - 2>{});
+    take(buf[0], 0);
+    // one panel: its dots into p, and q's comparisons.  Its first chunk is in buf[FIRST], its last one's matrix instructions cover the
+    // wait for the next panel's first
+    const auto round = [&](Panel &p, Panel &q, auto parity) {
+        constexpr int FIRST = decltype(parity)::value;
+        const uint64_t from = requested();
+        prepare(q);
         mx4_f4 nrm[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) nrm[i] = reinterpret_cast<const mx4_f4 *>(stage + P.rows.panel - 128)[2 * i + half];
@@ -515,8 +567,16 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
             for (int v = 0; v < 16; v++) p.acc[t][v] = 0.f;
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-            if (j + 1 < NB) take(j + 1);
-            const Mx4Chunk &c = buf[j & 1];
+            Mx4Chunk &c = buf[(FIRST + j) & 1], &next = buf[(FIRST + j + 1) & 1];
+            if (j + 1 < NB) {
+                take(next, j + 1);
+            } else {
+                arrive(std::integral_constant<int, STAGES - 3>{});
+                request(from);
+                use = use + 1 == STAGES ? 0 : use + 1;
+                stage = shared + use * STAGE;
+                take(next, 0);
+            }
             const auto step = [&](auto index) {
                 constexpr int I = decltype(index)::value;
                 const mx4_i8 t{c.a[I][0], c.a[I][1], c.a[I][2], c.a[I][3], 0, 0, 0, 0};
@@ -526,6 +586,7 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
                 const int s = 4 * j + I;
 #pragma unroll
                 for (int v = s * 16 / (4 * NB); v < (s + 1) * 16 / (4 * NB); v++) compare(q, v);
+                __builtin_amdgcn_sched_barrier(0);   // (left to itself the compiler puts them all behind the matrix instructions)
             };
             step(std::integral_constant<int, 0>{});
             step(std::integral_constant<int, 1>{});
@@ -535,6 +596,8 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
 #pragma unroll
         for (int v = 0; v < 16; v++) p.x[v] = nrm[v >> 2][v & 3];
         p.w = w;
+#pragma unroll
+        for (int i = 0; i < QT; i++) asm volatile("" : "+a"(p.acc[i]), "+v"(most[i]));   // (... or behind the branches of the rare case)
         conclude(q);
     };
     Panel a, b;   // b: a panel before the first one, without survivors
@@ -552,21 +615,24 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
         conclude(p);
     };
     for (;;) {
-        round(a, b);
+        round(a, b, std::integral_constant<int, 0>{});
         w += gridDim.x;
         if (w >= n_take) {
             last(a);
             break;
         }
-        round(b, a);
+        round(b, a, std::integral_constant<int, NB & 1>{});
         w += gridDim.x;
         if (w >= n_take) {
             last(b);
             break;
         }
     }
-    if constexpr (MODE == MX4_FILTER) queue.flush(P, norms, lane);
     mx4_wait_loads<0>();   // (what is under way writes this workgroup's LDS)
+    if constexpr (MODE == MX4_FILTER) {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < BLOCK_Q && block_q0 + i < P.nq; i += 256) P.counts[(size_t)(block_q0 + i) * P.segments + blockIdx.x] = taken[i];
+    }
 }
 
 }  // namespace vsg

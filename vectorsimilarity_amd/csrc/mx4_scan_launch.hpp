@@ -27,10 +27,10 @@ template <int BITS, int QT, int MODE, int SRC> static int launch_chunks(hipStrea
     }
 }
 template <int BITS, int QT, int MODE, int NB, int M> static int launch_ring4(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
-    const size_t lds = (size_t)mx4_ring_bytes(NB) + MX4_RING_WAVES * QT * 256 + (MODE == MX4_FILTER ? MX4_RING_WAVES * MX4_QUEUE * 16 : 0);
+    const size_t lds = (size_t)mx4_ring_bytes(NB) + MX4_RING_WAVES * QT * 256;
     (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_ring<BITS, QT, MODE, NB, M>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>(P.n_take, (uint64_t)shape.cus / shape.y));
-    hipLaunchKernelGGL((k_mx4_ring<BITS, QT, MODE, NB, M>), dim3((unsigned)gx, shape.y), dim3(64 * MX4_RING_WAVES), lds, s, P);
+    const uint64_t gx = MODE == MX4_FILTER ? P.segments : std::min<uint64_t>(P.n_take, (uint64_t)shape.cus);
+    hipLaunchKernelGGL((k_mx4_ring<BITS, QT, MODE, NB, M>), dim3((unsigned)gx), dim3(64 * MX4_RING_WAVES), lds, s, P);
     HIPCHK(hipGetLastError());
     return VSGPU_OK;
 }

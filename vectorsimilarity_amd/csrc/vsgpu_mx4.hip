@@ -66,7 +66,9 @@ struct Plan {
     bool by_row;                 // the probe keeps every row's bound, not one of 16 rows
     bool dense;                  // ... and those bounds are the candidate list: no threshold, no second pass
     uint64_t minima;             // floats per query
-    uint32_t segment, slices;    // candidates a list segment holds; workgroups per query that k_mx4_again may need
+    uint32_t segments, segment;  // parts of a candidate list and what each holds
+    uint32_t shares, room;       // workgroups per query that k_mx4_finish takes, candidates each may leave
+    uint32_t slices;             // ... that k_mx4_again may need
 };
 static Plan plan_scan(size_t dim, size_t nq, int bits, int cus) {
     Plan p{};
@@ -110,8 +112,18 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
         p.minima = 2 * p.take;
         expected = k * ((p.panels + p.take - 1) / p.take);
     }
-    // four times a segment's share: panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one
-    p.segment = (uint32_t)std::min<uint64_t>((n + MX4_SEGMENTS * 32 - 1) / (MX4_SEGMENTS * 32) * 32, expected * 4 / MX4_SEGMENTS + 64);
+    // Panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one: a few times its share
+    if (p.shape.src == MX4_RING && !p.dense) {
+        p.segments = (uint32_t)std::min<uint64_t>({(uint64_t)cus, (uint64_t)MX4_SEGMENTS_MAX, p.panels});
+        p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 40);
+    } else {
+        p.segments = MX4_SEGMENTS;
+        p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 4 / MX4_SEGMENTS + 64);
+    }
+    // k rows or more are scored exactly, a workgroup 1024 / lanes of them at once: several of these rounds are worth a second workgroup
+    const size_t rounds = k * mx4_row_lanes(mx4_steps((uint32_t)dim)) / 1024;
+    p.shares = (uint32_t)std::max<size_t>(1, std::min<size_t>({MX4_SHARES, rounds / 2, (size_t)cus / nq}));
+    p.room = (uint32_t)std::max<size_t>(k, 1024);
     p.slices = k <= 128 ? 32 : 8;
     return p;
 }
@@ -140,8 +152,8 @@ static QueryBlock take_queries(Layout &L, const Plan &p) {
 struct TopkBlock {
     QueryBlock q;
     float2 *limit;
-    uint32_t *counts, *again, *ticket;
-    uint64_t *again_limit;
+    uint32_t *done, *counts, *share_n, *again, *ticket;
+    uint64_t *again_limit, *share;
     float *minima;
     Mx4Cand *cand;
     uint64_t *part;
@@ -150,12 +162,15 @@ static TopkBlock take_topk(Layout &L, const Plan &p, size_t nq, size_t k) {
     TopkBlock b;
     b.q = take_queries(L, p);
     b.limit = L.take<float2>(nq);
-    b.counts = L.take<uint32_t>(nq * MX4_SEGMENTS);
+    b.done = L.take<uint32_t>(nq * (1 + (size_t)p.segments));
+    b.counts = b.done + nq;
+    b.share_n = L.take<uint32_t>(p.shares > 1 ? nq * p.shares : 0);
+    b.share = L.take<uint64_t>(p.shares > 1 ? nq * p.shares * (size_t)p.room : 0);
     b.again = L.take<uint32_t>(nq);
     b.ticket = L.take<uint32_t>(nq);
     b.again_limit = L.take<uint64_t>(nq);
     b.minima = L.take<float>(nq * p.minima);
-    b.cand = L.take<Mx4Cand>(nq * (size_t)p.segment * MX4_SEGMENTS);
+    b.cand = L.take<Mx4Cand>(nq * (size_t)p.segment * p.segments);
     b.part = L.take<uint64_t>(nq * p.slices * k);
     return b;
 }
@@ -247,7 +262,8 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     L.base = static_cast<char *>(ws);
     const TopkBlock b = take_topk(L, p, nq, k);
     if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
-    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.counts, nq * MX4_SEGMENTS);
+    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.done,
+                                nq * (p.shape.src == MX4_RING ? 1 : 1 + p.segments));   // (k_mx4_ring's counters are its own)
     if (rc) return rc;
     Mx4Scan P{};
     P.rows = R;
@@ -264,6 +280,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.limit = b.limit;
     P.counts = b.counts;
     P.cand = b.cand;
+    P.segments = p.segments;
     P.segment = p.segment;
     P.slack = mx4_slack(R.ks);
     if (p.dense && scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
@@ -283,7 +300,13 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
     S.nq = (uint32_t)nq;
     S.k = (uint32_t)k;
+    S.segments = p.segments;
     S.segment = p.segment;
+    S.shares = p.shares;
+    S.room = p.room;
+    S.share = b.share;
+    S.share_n = b.share_n;
+    S.done = b.done;
     S.counts = b.counts;
     S.cand = b.cand;
     S.again = b.again;
@@ -296,7 +319,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.minima = b.minima;
     S.qnorm = b.q.norm;
     S.slack = P.slack;
-    const dim3 fg((unsigned)nq), ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
+    const dim3 fg((unsigned)nq, p.shares), ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
     if (p.dense) {
         if (bits == 6) hipLaunchKernelGGL((k_mx4_finish<6, true>), fg, dim3(MX4_FINISH), 0, s, S);
         else hipLaunchKernelGGL((k_mx4_finish<4, true>), fg, dim3(MX4_FINISH), 0, s, S);
