@@ -161,7 +161,8 @@ int vsgpu_mx4_write(int device, void *stream, void *table, size_t capacity, size
 int vsgpu_mx4_read(int device, void *stream, const void *table, size_t capacity, size_t dim, const void *slots, int slot_bytes, size_t first, size_t m,
                    void *out, int type, size_t stride);
 /* fp32 scores of every query against rows [0, n): scores[q * scores_stride + row].  Dots are accumulated in fp32 and norms are kept
- * in fp32, so a Cosine score of vectors shorter than 2^-100 has few digits.  Workspace: 256-byte aligned device memory. */
+ * in fp32, so a Cosine score of vectors shorter than 2^-100 has few digits, and one of vectors longer than 2^62 may be infinite or
+ * NaN where a sum leaves fp32 (vsgpu_mx4_topk has neither limit).  Workspace: 256-byte aligned device memory. */
 size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits);   /* 0: bad arguments */
 int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride,
                      int metric, int bits, float *scores, size_t scores_stride, void *workspace, size_t workspace_bytes);

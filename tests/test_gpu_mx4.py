@@ -343,3 +343,155 @@ def test_refusals():
     assert mx4.scores(table, 0, x, ref.L2).shape == (4, 0) and mx4.scores(table, 40, x[:0], ref.L2).shape == (0, 40)
     ids, best = mx4.topk(table, 0, x, 3, ref.L2)
     assert (ids == -1).all() and (best == -1).all() and mx4.topk(table, 40, x[:0], 3, ref.L2)[0].shape == (0, 3)
+
+
+# ---- 65 to 256 queries: panels in an LDS ring -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("nq,n,dim,k,bits", [(65, 7001, 64, 1, 6), (128, 20000, 300, 10, 4), (129, 12345, 257, 100, 6), (256, 9000, 700, 10, 6),
+                                             (257, 6400, 1024, 20, 4), (200, 8200, 1, 5, 6), (66, 70000, 96, 1000, 6), (256, 33000, 128, 500, 4)])
+def test_topk_of_many_queries(nq, n, dim, k, bits, metric):
+    dtype = DTYPES[(nq + n + dim) % 3]
+    check_topk(vectors(n, dim, 1, dtype), vectors(nq, dim, 2, dtype), k, metric, bits)
+
+
+@pytest.mark.parametrize("nq", [5, 100, 200])
+@pytest.mark.parametrize("metric", METRICS)
+def test_topk_rows_without_a_score_and_short_ones(metric, nq):
+    """zero rows, rows of NaN, rows whose norm is far below the others', a table with fewer scores than k, queries without any"""
+    n, dim = 30000, 96
+    x, q = vectors(n, dim, 3), vectors(nq, dim, 4)
+    x[::5] = 0
+    x[1::7, 90] = float("nan")
+    x[2::11] *= 1e-25
+    q[1] = 0
+    q[3, 7] = float("inf")
+    q[4] *= 1e-22
+    check_topk(x, q, 10, metric, 6)
+    few = x[:7000].clone()
+    few[:] = float("nan")
+    few[[3, 40, 41, 6999]] = x[[3, 42, 41, 6999]]
+    check_topk(few, q, 10, metric, 6)
+
+
+@pytest.mark.parametrize("nq", [3, 70, 150])
+@pytest.mark.parametrize("metric", METRICS)
+def test_topk_dots_that_leave_fp32(metric, nq):
+    """partial sums beyond fp32 whose total is not: the rows' true scores decide"""
+    dim = 64
+    for n in (500, 9000):
+        x, q = vectors(n, dim, 5), vectors(nq, dim, 6)
+        x[7::50] *= 2.0 ** 90
+        x[11] = 0
+        x[11, 0], x[11, 40] = 2.0 ** 126, 2.0 ** 60
+        q[0, 40] = 0.5
+        q[1] *= 2.0 ** 100
+        q[2] = 0
+        q[2, 0], q[2, 32], q[2, 5] = 2.0 ** 70, 2.0 ** 70, 2.0 ** 69
+        x[13], x[14] = 0, 0
+        x[13, 0], x[13, 32], x[13, 40] = 2.0 ** 70, -(2.0 ** 70), 1.0
+        x[14, 0], x[14, 32], x[14, 5] = -(2.0 ** 70), 2.0 ** 70, 2.0 ** 63
+        check_topk(x, q, 10, metric, 6)
+        check_topk(x, q, 300, metric, 4)
+
+
+@pytest.mark.parametrize("nq", [2, 90])
+def test_topk_many_best_rows_that_crowd(nq):
+    """k best of which one is far from the others, and scores equal in groups"""
+    n, dim = 50000, 64
+    x, q = vectors(n, dim, 7), vectors(nq, dim, 8)
+    x[100] *= 1e4
+    x[200:700] = x[200]
+    for metric in METRICS:
+        check_topk(x, q, 1000, metric, 6)
+    check_topk(x[:20000], q[:2], 4096, ref.IP, 4)
+
+
+def test_a_store_beyond_4_gib():
+    n, dim = 8_400_000, 1024
+    table = mx4.empty(n, dim, DEV)
+    assert table.numel() > 1 << 32
+    x, q = vectors(1000, dim, 9), vectors(100, dim, 10)
+    slots = torch.cat([torch.arange(500), torch.arange(n - 500, n)])
+    mx4.write(table, x.to(DEV), slots.to(DEV))
+    values = ref.micro(x.double().numpy(), 4)
+    same(mx4.read(table, dim, slots.to(DEV)), values)
+    for nq in (1, 40, 100):
+        ids, best = mx4.topk(table, n, q[:nq].to(DEV), 5, ref.COSINE)
+        want_ids, want = ref.topk(q[:nq].double().numpy(), values, 5, ref.COSINE, 6)
+        np.testing.assert_array_equal(ids.cpu().numpy(), slots.numpy()[want_ids])
+        np.testing.assert_array_equal(best.cpu().numpy(), want)
+    got = mx4.scores(table, n, q[:70].to(DEV), ref.IP)
+    want = ref.scores(q[:70].double().numpy(), values, ref.IP, 6)
+    assert (np.abs(got[:, slots.to(DEV)].double().cpu().numpy() - want) <= ref.bound(q[:70].double().numpy(), values, ref.IP, 6)).all()
+    assert (got[:, 500:n - 500] == 1).all()
+
+
+# ---- the C entries -----------------------------------------------------------------------------------------------------------------
+def entry_topk(table, n, q, k, metric, bits, ws, size):
+    ids = torch.empty(len(q), k, dtype=torch.int64, device=DEV)
+    best = torch.empty(len(q), k, device=DEV)
+    rc = mx4._load().vsgpu_mx4_topk(0, torch.cuda.current_stream().cuda_stream, table.data_ptr(), n, q.shape[1], q.data_ptr(), mx4._TYPES[q.dtype],
+                                    len(q), q.stride(0) * q.element_size(), k, metric, bits, ids.data_ptr(), best.data_ptr(), ws.data_ptr(), size)
+    return rc, ids, best
+
+
+@pytest.mark.parametrize("nq,n,dim,k", [(1, 5000, 64, 10), (7, 20000, 300, 1000), (60, 20000, 64, 10), (100, 9000, 1024, 50), (256, 9000, 64, 1),
+                                        (300, 30000, 64, 10), (2, 7000, 9001, 5)])
+def test_workspaces_are_as_large_as_said(nq, n, dim, k):
+    """nothing is written behind one, and a smaller one is refused"""
+    table, q = store_of(vectors(n, dim, 1)), vectors(nq, dim, 2).to(DEV)
+    lib = mx4._load()
+    size = lib.vsgpu_mx4_topk_workspace(n, dim, nq, k, 6)
+    ws = torch.full((size + 4096,), 0x5A, dtype=torch.uint8, device=DEV)
+    rc, ids, best = entry_topk(table, n, q, k, ref.L2, 6, ws, size)
+    assert rc == 0 and (ws[size:] == 0x5A).all()
+    want = mx4.topk(table, n, q, k, ref.L2)
+    assert torch.equal(ids, want[0]) and torch.equal(best, want[1])
+    assert entry_topk(table, n, q, k, ref.L2, 6, ws, size - 256)[0] != 0
+    size = lib.vsgpu_mx4_scores_workspace(dim, nq, 6)
+    ws.fill_(0x5A)
+    out = torch.full((nq, n + 5), -7.0, device=DEV)
+    rc = lib.vsgpu_mx4_scores(0, torch.cuda.current_stream().cuda_stream, table.data_ptr(), n, dim, q.data_ptr(), mx4._TYPES[q.dtype], nq, dim * 4,
+                              ref.L2, 6, out.data_ptr(), n + 5, ws.data_ptr(), size)
+    assert rc == 0 and (ws[size:] == 0x5A).all() and (out[:, n:] == -7).all()
+    assert torch.equal(out[:, :n], mx4.scores(table, n, q, ref.L2))
+
+
+def test_two_threads_at_once():
+    import threading
+    table, q = store_of(vectors(40000, 96, 1)), [vectors(5, 96, 2).to(DEV), vectors(120, 96, 3).to(DEV)]
+    want = [mx4.topk(table, 40000, v, 20, ref.L2) for v in q]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = mx4.topk(table, 40000, q[i], 20, ref.L2)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_many_queries_captured_and_replayed():
+    n, dim = 20000, 128
+    table, q = store_of(vectors(n, dim, 1)), torch.empty(130, dim, device=DEV)
+    q.copy_(vectors(130, dim, 2))
+    mx4.topk(table, n, q, 1000, ref.IP)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (*mx4.topk(table, n, q, 10, ref.L2), *mx4.topk(table, n, q[:20], 1000, ref.IP))
+    for seed in (5, 6, 7):
+        q.copy_(vectors(130, dim, seed))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        for a, b in zip(got, (*mx4.topk(table, n, q, 10, ref.L2), *mx4.topk(table, n, q[:20], 1000, ref.IP))):
+            assert torch.equal(a, b)

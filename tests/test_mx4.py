@@ -53,7 +53,11 @@ def test_workspace_sizes():
     assert g.vsgpu_mx4_scores_workspace(0, 1, 6) == 0 and g.vsgpu_mx4_scores_workspace(64, 1, 5) == 0
     assert g.vsgpu_mx4_topk_workspace(100, 64, 1, 0, 6) == 0 and g.vsgpu_mx4_topk_workspace(100, 64, 1, 4097, 6) == 0
     assert 0 < g.vsgpu_mx4_scores_workspace(768, 64, 6) < 1 << 20
-    # batches of 256: more queries need no more room
+    # batches of 256: as much as the largest of them, the last one may plan a wider probe
+    for n, dim, k in ((10 ** 6, 768, 10), (50000, 64, 100), (4000, 300, 7), (300000, 128, 4096)):
+        for rest in (1, 40, 65, 130, 255):
+            both = max(g.vsgpu_mx4_topk_workspace(n, dim, 256, k, 6), g.vsgpu_mx4_topk_workspace(n, dim, rest, k, 6))
+            assert g.vsgpu_mx4_topk_workspace(n, dim, 512 + rest, k, 6) == both
     assert g.vsgpu_mx4_topk_workspace(10 ** 6, 768, 256, 10, 6) == g.vsgpu_mx4_topk_workspace(10 ** 6, 768, 5000, 10, 6)
 
 

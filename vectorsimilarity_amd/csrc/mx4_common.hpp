@@ -70,6 +70,7 @@ constexpr float MX4_EPS = 1.9073486328125e-6f;    // 2^-19, of |q|^2 + |x|^2 (L2
 constexpr float MX4_STEP = 9.5367431640625e-7f;   // 2^-20: what rounding a score to fp32 may move it, and more
 constexpr float MX4_TINY = 1e-36f;                // L2 scores below it: fp32 has no digits left to rank them by
 constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: the product of the norms may leave fp32
+constexpr float MX4_LONG = 4.611686018427388e18f; // 2^62: a dot of longer vectors may, as a whole or in one of its partial sums
 
 enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
 constexpr uint32_t MX4_SEGMENTS = 32;             // parts of a query's candidate list: one for every panel modulo 32,
@@ -114,12 +115,14 @@ __device__ __forceinline__ void mx4_bounds(uint32_t metric, float d, float x, fl
         e = slack + MX4_STEP;
         if (x < MX4_SHORT || y < MX4_SHORT) s = 1.f, e = 1.001f;
     }
+    if (x > MX4_LONG || y > MX4_LONG) s = 0.f, e = __uint_as_float(0x7F800000u);
     low = s - e;
     up = s + e;
 }
 
 // a lower bound from the upper one
 __device__ __forceinline__ float mx4_low(uint32_t metric, float up, float x, float y, float slack) {
+    if (x > MX4_LONG || y > MX4_LONG) return -__uint_as_float(0x7F800000u);
     if (metric == MX4_L2) return up - 2.f * __fmaf_rn(2.f * slack * x, y, __fmaf_rn(2.f * MX4_EPS, __fmaf_rn(x, x, y * y), MX4_TINY));
     if (metric == MX4_IP) return up - 2.f * __fmaf_rn(2.f * slack * x, y, 2.f * MX4_STEP * fmaxf(1.f, fabsf(up)));
     return x < MX4_SHORT || y < MX4_SHORT ? -1.f : up - 4.f * (slack + MX4_STEP);

@@ -533,7 +533,7 @@ static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
         l.x = ((1.f - tau) - T.slack - MX4_STEP) * yn;
         l.y = yn < MX4_SHORT ? -inf : 1e-42f;   // (0: a zero vector's dot is 0, and its score NaN)
     }
-    if (tau == inf) l = make_float2(0.f, -inf);
+    if (tau == inf || yn > MX4_LONG) l = make_float2(0.f, -inf);
     if (mx4_dead(T.metric, T.qsq[q])) l = make_float2(0.f, inf);
     T.limit[q] = l;
 }
@@ -759,7 +759,7 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
             n_s = 0;
             rows_n = 0;
             limit_s = MX4_NONE;
-            over_s = any;
+            over_s = any || S.qnorm[q] > MX4_LONG;   // (its dots may be NaN where the scores are not)
         }
     }
     __syncthreads();
@@ -775,7 +775,7 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     const auto bounds = [&](const Mx4Cand &c, float &low, float &up) { mx4_bounds(S.E.metric, c.dot, c.x, y, S.slack, low, up); };
     const auto up_key = [&](uint64_t i) {
         float up, low;
-        if constexpr (DENSE) up = S.minima[(size_t)q * S.E.rows.n + i];
+        if constexpr (DENSE) up = y > MX4_LONG ? __uint_as_float(0x7F800000u) : S.minima[(size_t)q * S.E.rows.n + i];
         else bounds(listed((uint32_t)i), low, up);
         return up == up ? mx4_key(up) : MX4_KEY_INF;
     };

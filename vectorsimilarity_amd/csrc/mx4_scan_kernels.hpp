@@ -87,13 +87,15 @@ template <int M> __device__ __forceinline__ float mx4_held(float d, float x, flo
     if constexpr (M == MX4_L2) return __fmaf_rn(x * (-0.5f * (1.f - MX4_EPS)), x, f);
     else return f;
 }
-// this lane's survivors.  Cosine: vectors too short for fp32 arithmetic go on to the exact one, zero vectors (score NaN) do not
+// rows that fp32 arithmetic says nothing about: they go on to the exact one (zero vectors, whose Cosine is NaN, need not)
+template <int M> __device__ __forceinline__ bool mx4_beyond(float x) { return x > MX4_LONG || (M == MX4_COSINE && x < MX4_SHORT && x > 0.f); }
+// this lane's survivors
 template <int M> __device__ __forceinline__ uint32_t mx4_survivors(const mx4_f16 &d, const mx4_f16 &x, float alpha, float beta) {
     uint32_t mask = 0;
 #pragma unroll
     for (int v = 0; v < 16; v++) {
         bool hit = mx4_held<M>(d[v], x[v], alpha) >= beta;
-        if constexpr (M == MX4_COSINE) hit |= x[v] < MX4_SHORT && x[v] > 0.f && beta < __uint_as_float(0x7F800000u);
+        hit |= mx4_beyond<M>(x[v]) && beta < __uint_as_float(0x7F800000u);
         mask |= hit ? 1u << v : 0u;
     }
     return mask;
@@ -108,6 +110,7 @@ __device__ __forceinline__ uint32_t mx4_rows_below(uint64_t first, uint64_t n) {
 // PROBE: smaller is nearer, then the upper bound (mx4_bounds, a reciprocal's rounding in the slack) of the smallest.  h is per row
 template <int M> __device__ __forceinline__ float mx4_probe_row(float x, bool none) {
     const float inf = __uint_as_float(0x7F800000u), nan = __uint_as_float(0x7FC00000u);
+    none |= x > MX4_LONG;
     if constexpr (M == MX4_L2) return none ? inf : (1.f + MX4_EPS) * x * x;
     else if constexpr (M == MX4_IP) return none ? inf : 0.f;
     else return none || x < MX4_SHORT ? nan : __builtin_amdgcn_rcpf(x);
@@ -313,13 +316,13 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
         };
         const auto filter = [&](auto metric) {
             constexpr int M = decltype(metric)::value;
-            bool odd = false;
-            if constexpr (M == MX4_COSINE) {
-                float least = xn[0];
+            float least = xn[0], longest = xn[0];
 #pragma unroll
-                for (int v = 1; v < 16; v++) least = fminf(least, xn[v]);
-                odd = __any(least < MX4_SHORT);
+            for (int v = 1; v < 16; v++) {
+                least = fminf(least, xn[v]);
+                longest = fmaxf(longest, xn[v]);
             }
+            const bool odd = __any(longest > MX4_LONG || (M == MX4_COSINE && least < MX4_SHORT));
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 float most = mx4_held<M>(acc[q][0], xn[0], alpha[q]);
@@ -462,11 +465,12 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
     };
     const auto row0_of = [&](const Panel &p) { return panel_of(p.w) * 32; };
     // a panel's comparisons, v-th of its rows
-    float most[QT], least;
+    float most[QT], least, longest;
     mx4_f16 h;
     const auto compare = [&](const Panel &p, int v) {
         if constexpr (MODE == MX4_FILTER) {
             if (M == MX4_COSINE) least = v ? fminf(least, p.x[v]) : p.x[0];
+            longest = v ? fmaxf(longest, p.x[v]) : p.x[0];
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 const float f = mx4_held<M>(p.acc[q][v], p.x[v], alpha[q]);
@@ -486,13 +490,12 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
             uint64_t any[QT], all = 0;
 #pragma unroll
             for (int q = 0; q < QT; q++) all |= any[q] = __ballot(most[q] >= beta[q]);
-            // vectors too short for fp32 arithmetic go on to the exact one, zero vectors (score NaN) do not; the last panel's padding
-            bool odd = row0 + 32 > P.rows.n;
-            if (M == MX4_COSINE && __any(least < MX4_SHORT)) {
+            bool odd = row0 + 32 > P.rows.n;   // the last panel's padding
+            if (__any(longest > MX4_LONG || (M == MX4_COSINE && least < MX4_SHORT))) {
                 asm volatile("");   // (or the compiler computes it every time)
                 bool some = false;
 #pragma unroll
-                for (int v = 0; v < 16; v++) some |= p.x[v] < MX4_SHORT && p.x[v] > 0.f;
+                for (int v = 0; v < 16; v++) some |= mx4_beyond<M>(p.x[v]);
                 odd |= __any(some);
             }
             if (all == 0 && !odd) return;
@@ -600,12 +603,12 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
         for (int i = 0; i < QT; i++) asm volatile("" : "+a"(p.acc[i]), "+v"(most[i]));   // (... or behind the branches of the rare case)
         conclude(q);
     };
-    Panel a, b;   // b: a panel before the first one, without survivors
+    Panel a, b;   // b: a panel before the first one, without survivors at any threshold
 #pragma unroll
     for (int v = 0; v < 16; v++) {
         b.x[v] = 1.f;
 #pragma unroll
-        for (int q = 0; q < QT; q++) b.acc[q][v] = -3e38f;
+        for (int q = 0; q < QT; q++) b.acc[q][v] = __uint_as_float(0x7FC00000u);
     }
     b.w = w;   // (PROBE: overwritten with the panel's own result)
     const auto last = [&](Panel &p) {

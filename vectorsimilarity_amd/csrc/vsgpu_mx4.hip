@@ -24,6 +24,7 @@ struct DeviceScope {
 };
 
 constexpr size_t MAX_DIM = 65536, MAX_ROWS = 0xFFFFFFE0ull, QUERY_BATCH = 256;
+constexpr int PLAN_CUS = 256;   // what sizes a workspace: it does not depend on the device that will be given it
 constexpr size_t LDS_BUDGET = 160 * 1024 - 4 * MX4_QUEUE * 16;   // for the queries' operands; the rest is the filter's queues
 
 int elem_size(int type) { return type == VSGPU_F32 ? 4 : (type == VSGPU_F16 || type == VSGPU_BF16 ? 2 : 0); }
@@ -114,7 +115,7 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
     }
     // Panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one: a few times its share
     if (p.shape.src == MX4_RING && !p.dense) {
-        p.segments = (uint32_t)std::min<uint64_t>({(uint64_t)cus, (uint64_t)MX4_SEGMENTS_MAX, p.panels});
+        p.segments = (uint32_t)std::min<uint64_t>({(uint64_t)PLAN_CUS, (uint64_t)MX4_SEGMENTS_MAX, p.panels});
         p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 40);
     } else {
         p.segments = MX4_SEGMENTS;
@@ -122,7 +123,7 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
     }
     // k rows or more are scored exactly, a workgroup 1024 / lanes of them at once: several of these rounds are worth a second workgroup
     const size_t rounds = k * mx4_row_lanes(mx4_steps((uint32_t)dim)) / 1024;
-    p.shares = (uint32_t)std::max<size_t>(1, std::min<size_t>({MX4_SHARES, rounds / 2, (size_t)cus / nq}));
+    p.shares = (uint32_t)std::max<size_t>(1, std::min<size_t>({MX4_SHARES, rounds / 2, (size_t)PLAN_CUS / nq}));
     p.room = (uint32_t)std::max<size_t>(k, 1024);
     p.slices = k <= 128 ? 32 : 8;
     return p;
@@ -239,18 +240,13 @@ int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
 }
 
 size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
-    Layout L;
-    nq = std::min(nq, QUERY_BATCH);
-    take_topk(L, plan_topk(n, dim, nq, k, bits, 256), nq, k);
+    const auto bytes = [&](size_t m) {
+        Layout L;
+        take_topk(L, plan_topk(n, dim, m, k, bits, PLAN_CUS), m, k);
+        return L.at;
+    };
     // (a last batch of fewer queries may plan a wider probe)
-    size_t most = L.at;
-    for (size_t m : {(size_t)1, (size_t)32, (size_t)64, (size_t)128}) {
-        if (m >= nq) break;
-        Layout M;
-        take_topk(M, plan_topk(n, dim, m, k, bits, 256), m, k);
-        most = std::max(most, M.at);
-    }
-    return most;
+    return nq > QUERY_BATCH && nq % QUERY_BATCH ? std::max(bytes(QUERY_BATCH), bytes(nq % QUERY_BATCH)) : bytes(std::min(nq, QUERY_BATCH));
 }
 
 // queries of one batch -> ids / scores [nq][k] on the device
@@ -474,7 +470,7 @@ int mx4_table_topk(vsgpu_table *t, const void *queries, size_t nq, size_t qstrid
         return VSGPU_OK;
     }
     const Mx4Rows R = rows_of(t);
-    const size_t row = in_bytes(t), batch = std::min(nq, QUERY_BATCH), ws = mx4_topk_bytes(n, t->dim, batch, take, t->mx4_bits);
+    const size_t row = in_bytes(t), batch = std::min(nq, QUERY_BATCH), ws = mx4_topk_bytes(n, t->dim, nq, take, t->mx4_bits);
     const size_t ids_bytes = (batch * take * 8 + 255) & ~(size_t)255, out_bytes = ids_bytes + batch * take * 4;
     int rc = ensure(c, c->dense, ws);
     if (!rc) rc = ensure(c, c->sel, out_bytes);
@@ -604,7 +600,7 @@ extern "C" int vsgpu_mx4_read(int device, void *stream, const void *table, size_
 extern "C" size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits) {
     if (bad_shape(0, dim) || (bits != 4 && bits != 6) || nq == 0) return 0;
     Layout L;
-    take_queries(L, plan_scan(dim, std::min(nq, QUERY_BATCH), bits, 256));
+    take_queries(L, plan_scan(dim, std::min(nq, QUERY_BATCH), bits, PLAN_CUS));
     return L.at;
 }
 extern "C" int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq,
