@@ -348,7 +348,7 @@ def test_refusals():
 # ---- 65 to 256 queries: panels in an LDS ring -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("metric", METRICS)
 @pytest.mark.parametrize("nq,n,dim,k,bits", [(65, 7001, 64, 1, 6), (128, 20000, 300, 10, 4), (129, 12345, 257, 100, 6), (256, 9000, 700, 10, 6),
-                                             (257, 6400, 1024, 20, 4), (200, 8200, 1, 5, 6), (66, 70000, 96, 1000, 6), (256, 33000, 128, 500, 4)])
+                                             (257, 6400, 1024, 20, 4), (65, 7100, 600, 3, 6), (100, 6999, 1000, 40, 4), (128, 9001, 1024, 10, 6), (200, 8200, 1, 5, 6), (66, 70000, 96, 1000, 6), (256, 33000, 128, 500, 4)])
 def test_topk_of_many_queries(nq, n, dim, k, bits, metric):
     dtype = DTYPES[(nq + n + dim) % 3]
     check_topk(vectors(n, dim, 1, dtype), vectors(nq, dim, 2, dtype), k, metric, bits)
@@ -358,7 +358,7 @@ def test_topk_of_many_queries(nq, n, dim, k, bits, metric):
 @pytest.mark.parametrize("metric", METRICS)
 def test_topk_rows_without_a_score_and_short_ones(metric, nq):
     """zero rows, rows of NaN, rows whose norm is far below the others', a table with fewer scores than k, queries without any"""
-    n, dim = 30000, 96
+    n, dim = 30000, 96 if nq == 5 else 640
     x, q = vectors(n, dim, 3), vectors(nq, dim, 4)
     x[::5] = 0
     x[1::7, 90] = float("nan")
@@ -377,7 +377,7 @@ def test_topk_rows_without_a_score_and_short_ones(metric, nq):
 @pytest.mark.parametrize("metric", METRICS)
 def test_topk_dots_that_leave_fp32(metric, nq):
     """partial sums beyond fp32 whose total is not: the rows' true scores decide"""
-    dim = 64
+    dim = 64 if nq == 3 else 576
     for n in (500, 9000):
         x, q = vectors(n, dim, 5), vectors(nq, dim, 6)
         x[7::50] *= 2.0 ** 90
@@ -397,7 +397,7 @@ def test_topk_dots_that_leave_fp32(metric, nq):
 @pytest.mark.parametrize("nq", [2, 90])
 def test_topk_many_best_rows_that_crowd(nq):
     """k best of which one is far from the others, and scores equal in groups"""
-    n, dim = 50000, 64
+    n, dim = 50000, 64 if nq == 2 else 520
     x, q = vectors(n, dim, 7), vectors(nq, dim, 8)
     x[100] *= 1e4
     x[200:700] = x[200]
@@ -480,7 +480,7 @@ def test_two_threads_at_once():
 
 
 def test_many_queries_captured_and_replayed():
-    n, dim = 20000, 128
+    n, dim = 20000, 640
     table, q = store_of(vectors(n, dim, 1)), torch.empty(130, dim, device=DEV)
     q.copy_(vectors(130, dim, 2))
     mx4.topk(table, n, q, 1000, ref.IP)

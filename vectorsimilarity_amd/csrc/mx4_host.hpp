@@ -5,9 +5,10 @@
 namespace vsg {
 struct Mx4Write;
 struct Mx4Read;
-enum { MX4_SHARED = 0, MX4_GLOBAL = 1, MX4_REGS = 2, MX4_RING = 3 };   // where the queries' operands are; RING: k_mx4_ring, or REGS for what it does not do
+enum { MX4_SHARED = 0, MX4_GLOBAL = 1, MX4_REGS = 2 };   // where k_mx4_scan has the queries' operands (REGS: in passes that keep every row's result; the others SHARED)
 struct Mx4ScanShape {
     int src, cus;
+    bool ring;        // the probe and the filter are k_mx4_ring
     uint32_t qt, y;   // query tiles a wave, workgroups side by side (each with groups x qt tiles)
 };
 int mx4_scan4(hipStream_t s, int mode, const Mx4Scan &P, const Mx4ScanShape &shape);

@@ -16,31 +16,32 @@ template <int T> __device__ __forceinline__ float mx4_widen(const void *p, size_
     else if constexpr (T == MX4_F16) return (float)static_cast<const _Float16 *>(p)[i];
     else return __uint_as_float((uint32_t)static_cast<const uint16_t *>(p)[i] << 16);
 }
-// 32 elements from x on, `have` of them in the row.  WIDE: x is 16-byte aligned
-template <int T, bool WIDE> __device__ __forceinline__ void mx4_load32(const void *x, int have, float v[32]) {
-    if (WIDE && have >= 32) {
-        if constexpr (T == MX4_F32) {
+// 16 bytes of a caller's vectors, aligned to their elements only (the memory takes a wide access at any of their addresses)
+typedef float mx4_f4_at __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t mx4_u4_at __attribute__((ext_vector_type(4), aligned(2)));
+// 32 elements from x on, `have` of them in the row
+template <int T> __device__ __forceinline__ void mx4_load32(const void *x, int have, float v[32]) {
+    constexpr int EACH = T == MX4_F32 ? 4 : 8;   // a load's
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const mx4_f4 w = static_cast<const mx4_f4 *>(x)[i];
+    for (int i = 0; i < 32 / EACH; i++) {
+        if (EACH * (i + 1) <= have) {
+            if constexpr (T == MX4_F32) {
+                const mx4_f4_at w = static_cast<const mx4_f4_at *>(x)[i];
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const mx4_u4 w = static_cast<const mx4_u4 *>(x)[i];
+            } else {
+                const mx4_u4_at w = static_cast<const mx4_u4_at *>(x)[i];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
                     v[8 * i + j] = T == MX4_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
                 }
             }
-        }
-        return;
-    }
+        } else {
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = j < have ? mx4_widen<T>(x, (size_t)j) : 0.f;
+            for (int j = EACH * i; j < EACH * (i + 1); j++) v[j] = j < have ? mx4_widen<T>(x, (size_t)j) : 0.f;
+        }
+    }
 }
 
 // the block's scale byte, and 2^-E for its elements (0 where the block is NaN or zero)
@@ -121,7 +122,7 @@ static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) 
 }
 // One workgroup takes 32 vectors, its waves (up to 16) the k-steps in turn; a lane rounds one block (half, row) by itself, so neither
 // the maximum nor the codes cross lanes.
-template <int T, bool WIDE> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
+template <int T> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
     __shared__ double part[16][64];
     __shared__ int64_t slot_s[32];
     __shared__ int lost_s[32];
@@ -159,7 +160,7 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(1024) void k_mx4
         for (uint32_t s = wave; s < W.rows.ks; s += waves) {
             const int have = (int)W.rows.dim - (int)(2 * s + half) * 32;
             float v[32], inv;
-            if (have > 0) mx4_load32<T, WIDE>(x + (size_t)(2 * s + half) * 32 * esz, have, v);
+            if (have > 0) mx4_load32<T>(x + (size_t)(2 * s + half) * 32 * esz, have, v);
             else {
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = 0.f;
@@ -207,7 +208,7 @@ __device__ __forceinline__ float mx4_code_value(uint32_t c) {   // c: 4 bits
 }
 // A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  A
 // workgroup takes `rows` whole rows (rows * per_row < 2^16: the division is one multiplication, by ceil(2^32 / per_row)).
-template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t recip) {
+template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t recip) {
     const uint64_t i0 = (uint64_t)blockIdx.x * rows;
     const uint32_t work = (uint32_t)min((uint64_t)rows, R.m - i0) * per_row;
     for (uint32_t t = threadIdx.x; t < work; t += 256) {
@@ -231,9 +232,9 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
         char *o = R.out + i * R.stride;
         if constexpr (T == MX4_F32) {
             float *of = reinterpret_cast<float *>(o) + e;
-            if (WIDE && e + 8 <= R.rows.dim) {
-                *reinterpret_cast<mx4_f4 *>(of) = mx4_f4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<mx4_f4 *>(of + 4) = mx4_f4{v[4], v[5], v[6], v[7]};
+            if (e + 8 <= R.rows.dim) {
+                *reinterpret_cast<mx4_f4_at *>(of) = mx4_f4_at{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<mx4_f4_at *>(of + 4) = mx4_f4_at{v[4], v[5], v[6], v[7]};
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -245,11 +246,11 @@ template <int T, bool WIDE> static __global__ __launch_bounds__(256) void k_mx4_
 #pragma unroll
             for (int j = 0; j < 8; j++) h[j] = T == MX4_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : (uint16_t)(__float_as_uint(v[j]) >> 16);
             uint16_t *oh = reinterpret_cast<uint16_t *>(o) + e;
-            if (WIDE && e + 8 <= R.rows.dim) {
-                mx4_u4 w;
+            if (e + 8 <= R.rows.dim) {
+                mx4_u4_at w;
 #pragma unroll
                 for (int j = 0; j < 4; j++) w[j] = (uint32_t)h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-                *reinterpret_cast<mx4_u4 *>(oh) = w;
+                *reinterpret_cast<mx4_u4_at *>(oh) = w;
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -282,7 +283,7 @@ struct Mx4Queries {
     uint32_t *zero;      // words to clear for the kernels behind this one
     uint32_t zero_words;
 };
-template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) void k_mx4_queries(Mx4Queries Q) {
+template <int T, int BITS> static __global__ __launch_bounds__(1024) void k_mx4_queries(Mx4Queries Q) {
     __shared__ double part[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, row = lane & 31, half = lane >> 5;
     const uint32_t q = blockIdx.x * 32 + row;
@@ -295,7 +296,7 @@ template <int T, bool WIDE, int BITS> static __global__ __launch_bounds__(1024) 
         char *sc = scales + (s >> 2) * 256 + lane * 4 + (s & 3);
         const int have = q < Q.nq ? (int)Q.dim - (int)(2 * s + half) * 32 : 0;
         float v[32], inv;
-        if (have > 0) mx4_load32<T, WIDE>(Q.x + q * Q.stride + (size_t)(2 * s + half) * 32 * esz, have, v);
+        if (have > 0) mx4_load32<T>(Q.x + q * Q.stride + (size_t)(2 * s + half) * 32 * esz, have, v);
         else {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = 0.f;
@@ -779,8 +780,9 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         else bounds(listed((uint32_t)i), low, up);
         return up == up ? mx4_key(up) : MX4_KEY_INF;
     };
+    const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
     uint32_t key = MX4_KEY_INF;
-    if (n > S.k) {
+    if (n > S.k && n > 2 * at_once) {   // (two rounds' scores cost less than what would save them)
         if (n <= MX4_LISTED) {
             for (uint32_t i = threadIdx.x; i < n; i += MX4_FINISH) up_s[i] = up_key(i);
             key = mx4_kth(bins, n, S.k, [&](uint64_t i) { return up_s[i]; });
@@ -790,7 +792,6 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     }
     const float most = mx4_unkey(key);
     // rows worth an exact score, collected and scored MX4_FINISH or more at a time
-    const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
     const uint32_t mine = (((n + 63) / 64 + S.shares - 1 - me) / S.shares) * 64;   // this workgroup's candidates, the last 64 perhaps fewer
     for (uint32_t j0 = 0; j0 < mine; j0 += MX4_FINISH) {
         const uint32_t j = j0 + threadIdx.x, i = ((j >> 6) * S.shares + me) * 64 + (j & 63);
@@ -879,19 +880,29 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         S.ticket[q] = 0;
         S.again_limit[q] = got >= S.k ? kth : MX4_NONE - 1;
     };
-    if (have > 256 && 2 * have <= MX4_LISTED) {   // (up_s is free by now)
+    if (2 * have <= MX4_LISTED) {   // (up_s is free by now)
         if (threadIdx.x == 0) {
             rows_n = 0;
             limit_s = MX4_NONE;
         }
-        const bool done = mx4_ranked(bins, keys, have, reinterpret_cast<uint64_t *>(up_s), [&](uint32_t rank, uint64_t key) {
+        __syncthreads();
+        const auto emit = [&](uint32_t rank, uint64_t key) {
             if (rank < S.k) {
                 S.ids[(size_t)q * S.k + rank] = (int64_t)(uint32_t)key;
                 S.scores[(size_t)q * S.k + rank] = mx4_unkey((uint32_t)(key >> 32));
                 if (rank == S.k - 1) limit_s = key;
             }
             atomicAdd(&rows_n, 1u);
-        });
+        };
+        bool done = true;
+        if (have > 256) {
+            done = mx4_ranked(bins, keys, have, reinterpret_cast<uint64_t *>(up_s), emit);
+        } else if (threadIdx.x < have && keys[threadIdx.x] != MX4_NONE) {   // few: against each of the others
+            const uint64_t key = keys[threadIdx.x];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < have; j++) rank += keys[j] < key;
+            emit(rank, key);
+        }
         __syncthreads();
         if (done) {
             const uint32_t got = rows_n;

@@ -132,7 +132,7 @@ template <int M> __device__ __forceinline__ float mx4_probe_bound(float best, fl
 // The ring of k_mx4_ring: the workgroup's waves bring every panel into LDS together, a KiB at a time in turn, and `stages` panels
 // are under way or in use.  Constants by the chunks of a panel (codes, scales, norms in whole KiB); the stages fill the LDS beside the queues.
 constexpr int mx4_ring_pieces(int nb) { return (4 * nb * 1024 + nb * 256 + 128 + 1023) / 1024; }
-constexpr int mx4_ring_stages(int nb) { return nb == 1 ? 16 : (nb == 2 ? 15 : (nb == 3 ? 10 : 7)); }
+constexpr int mx4_ring_stages(int nb) { return nb == 2 ? 15 : (nb == 3 ? 10 : 7); }
 constexpr int mx4_ring_bytes(int nb) { return mx4_ring_stages(nb) * mx4_ring_pieces(nb) * 1024; }
 constexpr int MX4_RING_WAVES = 4;
 // 16 bytes a lane from base + offset to LDS (lds: the wave's first byte), without passing through registers
@@ -161,9 +161,9 @@ constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
 // flight: chunk g of the next panel is requested as soon as chunk g of this one has gone into the matrix cores.  Panels of more than
 // 4 chunks go through the same four buffers several times.  The queries' operands (SRC) are
 //   up to 64 queries          in LDS, read per k-step: the registers hold more of the table in flight instead
-//   more, rows to 1024        in registers: LDS could not feed the matrix cores (1.5 KiB a tile and step against 32 cycles of matrix
-//                             work on each of four SIMDs), so a wave keeps one or two tiles and the waves take the same panels, through
-//                             LDS (RING) or, where stores are most of the traffic (DENSE), each by itself through the CU's cache (REGS)
+//   more, rows to 1024        in registers for scores and bounds of every row: a wave keeps two tiles, and the waves take the same
+//                             panels through the CU's cache; LDS would be read 1.5 KiB a tile and step against 32 cycles of matrix
+//                             work on each of four SIMDs.  Probe and filter: LDS too, or k_mx4_ring
 //   rows beyond the LDS       in global memory, through the caches
 template <int BITS, int QT, int MODE, int NB, int SRC>
 static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)) void k_mx4_scan(Mx4Scan P) {

@@ -13,8 +13,9 @@ template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hi
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     // as many workgroups as stay resident; few panels: fewer, so that a wave's start is not most of its work
     const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(mx4_scan_waves(BITS, QT, MODE, NB, SRC), (160 * 1024) / (lds + 512)));
-    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + abreast - 1) / abreast, (uint64_t)shape.cus * fit / shape.y));
-    hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, SRC>), dim3((unsigned)gx, shape.y), dim3(64 * waves), lds, s, P);
+    const uint32_t y = SRC == MX4_REGS ? 1 : shape.y;   // (REGS: all of a batch's tiles in one workgroup)
+    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + abreast - 1) / abreast, (uint64_t)shape.cus * fit / y));
+    hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, SRC>), dim3((unsigned)gx, y), dim3(64 * waves), lds, s, P);
     HIPCHK(hipGetLastError());
     return VSGPU_OK;
 }
@@ -40,18 +41,16 @@ template <int BITS, int QT, int MODE, int NB> static int launch_ring3(hipStream_
     return launch_ring4<BITS, QT, MODE, NB, MX4_COSINE>(s, P, shape);
 }
 template <int BITS, int QT, int MODE> static int launch_ring(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
-    switch (P.rows.kg) {
-    case 1: return launch_ring3<BITS, QT, MODE, 1>(s, P, shape);
-    case 2: return launch_ring3<BITS, QT, MODE, 2>(s, P, shape);
-    case 3: return launch_ring3<BITS, QT, MODE, 3>(s, P, shape);
-    default: return launch_ring3<BITS, QT, MODE, 4>(s, P, shape);
-    }
+    if constexpr (QT == 2)
+        if (P.rows.kg == 2) return launch_ring3<BITS, QT, MODE, 2>(s, P, shape);
+    return P.rows.kg == 3 ? launch_ring3<BITS, QT, MODE, 3>(s, P, shape) : launch_ring3<BITS, QT, MODE, 4>(s, P, shape);
 }
 template <int BITS, int MODE> static int launch_mode(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
     if (shape.src == MX4_GLOBAL) return launch_scan<BITS, 1, MODE, 4, MX4_GLOBAL>(s, P, shape);
-    if (shape.src == MX4_RING) {
-        if constexpr (MODE == MX4_DENSE || MODE == MX4_PROBE_ROWS) return launch_chunks<BITS, 2, MODE, MX4_REGS>(s, P, shape);
-        else return shape.qt == 1 ? launch_ring<BITS, 1, MODE>(s, P, shape) : launch_ring<BITS, 2, MODE>(s, P, shape);
+    if constexpr (MODE == MX4_DENSE || MODE == MX4_PROBE_ROWS) {
+        if (shape.src == MX4_REGS) return launch_chunks<BITS, 2, MODE, MX4_REGS>(s, P, shape);
+    } else if (shape.ring) {
+        return shape.qt == 1 ? launch_ring<BITS, 1, MODE>(s, P, shape) : launch_ring<BITS, 2, MODE>(s, P, shape);
     }
     if (P.rows.kg == 1) return shape.qt == 1 ? launch_scan<BITS, 1, MODE, 1, MX4_SHARED>(s, P, shape) : launch_scan<BITS, 2, MODE, 1, MX4_SHARED>(s, P, shape);
     return shape.qt == 1 ? launch_scan<BITS, 1, MODE, 4, MX4_SHARED>(s, P, shape) : launch_scan<BITS, 2, MODE, 4, MX4_SHARED>(s, P, shape);

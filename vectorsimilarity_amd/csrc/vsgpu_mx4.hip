@@ -78,11 +78,16 @@ static Plan plan_scan(size_t dim, size_t nq, int bits, int cus) {
     p.shape.cus = cus;
     p.groups = 1;
     if (nt > 2 && dim <= 1024) {
-        p.shape.src = MX4_RING;
-        p.shape.qt = nt <= 4 ? 1 : 2;
-        p.groups = std::min(4u, (nt + 1) / 2);   // (REGS: two tiles a wave)
-        p.tiles = 4 * p.shape.qt;
-        p.shape.y = 1;
+        // Scores and bounds of every row: operands in registers.  The probe and the filter: the ring where a panel's matrix work
+        // outweighs its barrier and comparisons, queries in LDS and panels by wave below that (2M rows, top-10, 128 queries: 256
+        // elements 150 us against the ring's 202, 512 221 : 228, 1024 406 : 285; 256 queries: 256 elements 260 : 267, 512 402 : 310)
+        const uint32_t kg = mx4_groups((uint32_t)dim);
+        p.shape.src = MX4_REGS;
+        p.shape.ring = kg > (nt <= 4 ? 2u : 1u);
+        p.shape.qt = p.shape.ring && nt <= 4 ? 1 : 2;
+        p.groups = (nt + 1) / 2;   // (REGS: two tiles a wave)
+        p.shape.y = (nt + 1) / 2;
+        p.tiles = p.shape.ring ? 4 * p.shape.qt : 2 * p.shape.y;
         return p;
     } else if (p.qtile_bytes + 256 > LDS_BUDGET) {
         p.shape.src = MX4_GLOBAL;
@@ -114,7 +119,7 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
         expected = k * ((p.panels + p.take - 1) / p.take);
     }
     // Panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one: a few times its share
-    if (p.shape.src == MX4_RING && !p.dense) {
+    if (p.shape.ring && !p.dense) {
         p.segments = (uint32_t)std::min<uint64_t>({(uint64_t)PLAN_CUS, (uint64_t)MX4_SEGMENTS_MAX, p.panels});
         p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 40);
     } else {
@@ -177,11 +182,9 @@ static TopkBlock take_topk(Layout &L, const Plan &p, size_t nq, size_t k) {
 }
 
 template <int BITS> static int launch_queries(hipStream_t s, const Mx4Queries &Q, uint32_t tiles, int type) {
-    const bool wide = (((uintptr_t)Q.x | Q.stride) & 15) == 0;
     const dim3 g(tiles), b(64 * std::min(16u, Q.kg * 4));
 #define MX4_CASE(T)                                                                                       \
-    if (wide) hipLaunchKernelGGL((k_mx4_queries<T, true, BITS>), g, b, 0, s, Q);                          \
-    else hipLaunchKernelGGL((k_mx4_queries<T, false, BITS>), g, b, 0, s, Q);
+    hipLaunchKernelGGL((k_mx4_queries<T, BITS>), g, b, 0, s, Q);
     if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
     else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
     else { MX4_CASE(MX4_BF16) }
@@ -208,11 +211,11 @@ int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
         hipLaunchKernelGGL(k_mx4_claim, g, dim3(256), 0, s, W, 1);
         W.claimed = 1;
     }
-    const bool wide = (((uintptr_t)W.x | W.stride) & 15) == 0;
-    const dim3 g((unsigned)((W.m + 31) / 32)), b(64 * std::min(16u, W.rows.ks));
+    // (waves beyond the rows' steps only help in that search)
+    const unsigned search = W.slots && !W.claimed ? (unsigned)std::min<uint64_t>(16, (W.m + 127) / 128) : 1;
+    const dim3 g((unsigned)((W.m + 31) / 32)), b(64 * std::max(search, std::min(16u, W.rows.ks)));
 #define MX4_CASE(T)                                                                \
-    if (wide) hipLaunchKernelGGL((k_mx4_write<T, true>), g, b, 0, s, W);           \
-    else hipLaunchKernelGGL((k_mx4_write<T, false>), g, b, 0, s, W);
+    hipLaunchKernelGGL((k_mx4_write<T>), g, b, 0, s, W);
     if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
     else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
     else { MX4_CASE(MX4_BF16) }
@@ -226,11 +229,9 @@ int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
     // about 1024 threads' work a workgroup, fewer rows when there are not enough of them to fill the chip
     uint64_t rows = std::max<uint64_t>(1, 1024 / per_row);
     rows = std::max<uint64_t>(std::min<uint64_t>(rows, R.m / ((uint64_t)cus * 8)), std::max<uint64_t>(1, std::min<uint64_t>(256 / per_row, R.m)));
-    const bool wide = (((uintptr_t)R.out | R.stride) & 15) == 0;
     const dim3 g((unsigned)((R.m + rows - 1) / rows)), b(256);
 #define MX4_CASE(T)                                                                                                           \
-    if (wide) hipLaunchKernelGGL((k_mx4_read<T, true>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);                       \
-    else hipLaunchKernelGGL((k_mx4_read<T, false>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);
+    hipLaunchKernelGGL((k_mx4_read<T>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);
     if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
     else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
     else { MX4_CASE(MX4_BF16) }
@@ -259,7 +260,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     const TopkBlock b = take_topk(L, p, nq, k);
     if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
     int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.done,
-                                nq * (p.shape.src == MX4_RING ? 1 : 1 + p.segments));   // (k_mx4_ring's counters are its own)
+                                nq * (p.shape.ring ? 1 : 1 + p.segments));   // (k_mx4_ring's counters are its own)
     if (rc) return rc;
     Mx4Scan P{};
     P.rows = R;
