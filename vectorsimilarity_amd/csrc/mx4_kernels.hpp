@@ -602,8 +602,8 @@ __device__ __forceinline__ float mx4_final(uint32_t metric, double dot, double x
     if (metric == MX4_L2) return (float)(qq + xx - 2.0 * dot);
     return (float)(1.0 - dot / (sqrt(qq) * sqrt(xx)));
 }
-// lanes on one row: one for each of its blocks, 4 to 32
-__host__ __device__ inline uint32_t mx4_row_lanes(uint32_t ks) { return ks <= 2 ? 4u : (ks <= 4 ? 8u : (ks <= 8 ? 16u : 32u)); }
+// lanes on one row: one for each of its blocks, 2 to 32
+__host__ __device__ inline uint32_t mx4_row_lanes(uint32_t ks) { return ks <= 1 ? 2u : ks <= 2 ? 4u : (ks <= 4 ? 8u : (ks <= 8 ? 16u : 32u)); }
 template <int BITS, int R> __device__ __forceinline__ void mx4_exact_scores(const Mx4Exact &E, uint32_t q, const uint32_t (&row)[R], uint32_t lanes, float (&score)[R]) {
     double dot[R], xx[R];
     mx4_row_sums<BITS, R>(E, E.tiles + (size_t)(q >> 5) * E.qtile_bytes, q & 31, row, threadIdx.x & (lanes - 1), lanes, dot, xx);
@@ -682,13 +682,15 @@ __device__ __forceinline__ void mx4_keep_cut(const Mx4Keep &K) {   // all thread
     }
     __syncthreads();
 }
-// called by all threads, at most `room` of them with a key (MX4_NONE: none)
-__device__ __forceinline__ void mx4_keep_add(const Mx4Keep &K, uint64_t key, uint32_t room) {
+// called by all threads, with at most `room` keys in all (MX4_NONE: none)
+template <int R> __device__ __forceinline__ void mx4_keep_add(const Mx4Keep &K, const uint64_t (&key)[R], uint32_t room) {
     __syncthreads();
     const bool full = *K.n + room > MX4_KEEP;   // (the same for all threads: nobody adds before the next barrier)
     __syncthreads();
     if (full) mx4_keep_cut(K);
-    if (key < *K.limit) K.keys[atomicAdd(K.n, 1u)] = key;
+#pragma unroll
+    for (int i = 0; i < R; i++)
+        if (key[i] < *K.limit) K.keys[atomicAdd(K.n, 1u)] = key[i];
 }
 struct Mx4Select {
     Mx4Exact E;
@@ -870,7 +872,8 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
             uint32_t w = 0;
             while (w + 1 < S.shares && first_s[w + 1] <= i) w++;
             const bool have = i < total;
-            mx4_keep_add(K, have ? __hip_atomic_load(&from[(size_t)w * S.room + (i - first_s[w])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE, MX4_FINISH);
+            const uint64_t key[1] = {have ? __hip_atomic_load(&from[(size_t)w * S.room + (i - first_s[w])], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE};
+            mx4_keep_add(K, key, MX4_FINISH);
         }
     }
     __syncthreads();
@@ -927,6 +930,7 @@ template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ uint32_t n_s, last_s;
     __shared__ uint64_t limit_s;
+    constexpr int EACH = 4;   // rows under way to a lane
     for (uint32_t q = blockIdx.y; q < S.nq; q += gridDim.y) {
         if (!S.again[q]) continue;
         const Mx4Keep K{keys, &n_s, &limit_s, S.k};
@@ -937,29 +941,41 @@ template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx
         }
         const uint64_t n = S.E.rows.n, per = (n + S.slices - 1) / S.slices, a = min(n, per * blockIdx.x), b = min(n, a + per);
         const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = 512 / lanes;
-        for (uint64_t r0 = a; r0 < b; r0 += at_once) {
-            const uint64_t row = r0 + threadIdx.x / lanes;
-            const float s = mx4_exact_score<BITS>(S.E, q, (uint32_t)min(row, n - 1), lanes);
-            mx4_keep_add(K, (threadIdx.x & (lanes - 1)) == 0 && row < b ? mx4_pack(s, (uint32_t)row) : MX4_NONE, at_once);
+        for (uint64_t r0 = a; r0 < b; r0 += EACH * at_once) {
+            uint32_t row[EACH];
+            float score[EACH];
+            uint64_t key[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; i++) row[i] = (uint32_t)min(r0 + i * at_once + threadIdx.x / lanes, n - 1);
+            mx4_exact_scores<BITS, EACH>(S.E, q, row, lanes, score);
+#pragma unroll
+            for (int i = 0; i < EACH; i++)
+                key[i] = (threadIdx.x & (lanes - 1)) == 0 && r0 + i * at_once + threadIdx.x / lanes < b ? mx4_pack(score[i], row[i]) : MX4_NONE;
+            mx4_keep_add(K, key, EACH * at_once);
         }
         mx4_keep_cut(K);
         uint64_t *mine = S.part + ((size_t)q * S.slices + blockIdx.x) * S.k;
         for (uint32_t i = threadIdx.x; i < S.k; i += 512) __hip_atomic_store(&mine[i], i < n_s ? keys[i] : MX4_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) last_s = atomicAdd(&S.ticket[q], 1u) == S.slices - 1;
-        __syncthreads();
-        if (!last_s) continue;
-        __threadfence();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0) {   // (as in k_mx4_finish)
+            __threadfence();
+            last_s = atomicAdd(&S.ticket[q], 1u) == S.slices - 1;
+            __threadfence();
             n_s = 0;
             limit_s = MX4_NONE;
         }
+        __syncthreads();
+        if (!last_s) continue;
         const uint64_t total = (uint64_t)S.slices * S.k;
         const uint64_t *all = S.part + (size_t)q * total;
-        for (uint64_t i0 = 0; i0 < total; i0 += 512) {
-            const uint64_t i = i0 + threadIdx.x;
-            mx4_keep_add(K, i < total ? __hip_atomic_load(&all[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE, 512);
+        for (uint64_t i0 = 0; i0 < total; i0 += EACH * 512) {
+            uint64_t key[EACH];
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                const uint64_t i = i0 + j * 512 + threadIdx.x;
+                key[j] = i < total ? __hip_atomic_load(&all[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : MX4_NONE;
+            }
+            mx4_keep_add(K, key, EACH * 512);
         }
         mx4_keep_cut(K);
         mx4_emit(S, q, keys, n_s);
