@@ -73,9 +73,7 @@ constexpr float MX4_SHORT = 1e-18f;               // Cosine of shorter vectors: 
 constexpr float MX4_LONG = 4.611686018427388e18f; // 2^62: a dot of longer vectors may, as a whole or in one of its partial sums
 
 enum { MX4_PROBE = 0, MX4_PROBE_ROWS = 1, MX4_FILTER = 2, MX4_DENSE = 3 };
-constexpr uint32_t MX4_SEGMENTS = 32;             // parts of a query's candidate list: one for every panel modulo 32,
-constexpr uint32_t MX4_SEGMENTS_MAX = 256;        // or one for each workgroup of k_mx4_ring
-constexpr uint32_t MX4_QUEUE = 128;               // survivors a wave collects in LDS before they go out
+constexpr uint32_t MX4_SEGMENTS = 1024;           // parts of a query's candidate list at most: one for each workgroup of the filter
 struct Mx4Cand {
     uint32_t row;
     float dot, x;                 // of the matrix cores, |x|

@@ -11,6 +11,19 @@ struct Mx4ScanShape {
     bool ring;        // the probe and the filter are k_mx4_ring
     uint32_t qt, y;   // query tiles a wave, workgroups side by side (each with groups x qt tiles)
 };
+// registers of a wave of k_mx4_scan, about: what its operands, sums and panel in flight need
+constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
+    const int regs = (src == MX4_REGS ? qt * nb * (bits == 6 ? 25 : 17) : qt * 12) + qt * 16 + nb * 17 + (mode == MX4_DENSE ? 60 : 105);
+    return regs <= 128 ? 4 : (regs <= 168 ? 3 : (regs <= 256 ? 2 : 1));
+}
+// ... its workgroups along the table: as many as stay resident; few panels: fewer, so that a wave's start is not most of its work
+inline uint64_t mx4_scan_grid(int bits, int qt, int mode, int nb, int src, size_t lds, uint64_t n_take, uint32_t abreast, int cus, uint32_t y) {
+    const uint64_t fit = lds + 512 > 160 * 1024 ? 1 : (160 * 1024) / (lds + 512), waves = (uint64_t)mx4_scan_waves(bits, qt, mode, nb, src);
+    const uint64_t all = (uint64_t)cus * (fit < waves ? fit : waves) / y, need = (n_take + abreast - 1) / abreast;
+    return all < need ? (all ? all : 1) : need;
+}
+inline int mx4_scan_chunks(uint32_t kg) { return kg == 1 ? 1 : 4; }   // SHARED: a panel's chunks in flight
+inline size_t mx4_scan_lds(int src, uint32_t qt, uint32_t groups, uint32_t qtile_bytes) { return (src == MX4_SHARED ? (size_t)qt * qtile_bytes : 0) + groups * qt * 256; }
 int mx4_scan4(hipStream_t s, int mode, const Mx4Scan &P, const Mx4ScanShape &shape);
 int mx4_scan6(hipStream_t s, int mode, const Mx4Scan &P, const Mx4ScanShape &shape);
 Mx4Rows mx4_rows_of(const void *base, size_t n, size_t dim);

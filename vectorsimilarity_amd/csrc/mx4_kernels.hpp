@@ -449,9 +449,10 @@ template <typename F> __device__ __forceinline__ bool mx4_ranked(Mx4Bins &B, con
     lo = B.lo;
     hi = B.hi;
     if (lo > hi) return true;   // no key
-    const uint32_t range = hi - lo;
-    const int shift = range < MX4_BINS ? 0 : 32 - __builtin_clz(range) - 11;
-    const auto bin_of = [&](uint64_t key) { return ((uint32_t)(key >> 32) - lo) >> shift; };
+    // (by the scores and not by their bits, which spread an exact match and the rest over all the powers of two between them)
+    const float least = mx4_unkey(lo), range = mx4_unkey(hi) - least, per = range > 0 ? (float)MX4_BINS / range : 0.f;
+    if (!(range < 3e38f) || !(per < 3e38f)) return false;
+    const auto bin_of = [&](uint64_t key) { return min((uint32_t)((mx4_unkey((uint32_t)(key >> 32)) - least) * per), MX4_BINS - 1); };
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
         if (keys[i] != ~0ull) atomicAdd(&B.bin(bin_of(keys[i])), 1u);
     __syncthreads();
@@ -499,6 +500,7 @@ struct Mx4Threshold {
     const float *qnorm;
     const double *qsq;
     float2 *limit;
+    float *tau;
     float slack;
 };
 // a Cosine query of norm zero, or one that holds an infinity or a NaN: every score is NaN
@@ -522,7 +524,8 @@ static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
     }
     if (threadIdx.x) return;
     const float inf = __uint_as_float(0x7F800000u);
-    const float tau = mx4_unkey(key), yn = T.qnorm[q];
+    const float yn = T.qnorm[q], tau = yn > MX4_LONG ? inf : mx4_unkey(key);
+    T.tau[q] = tau;
     float2 l;
     if (T.metric == MX4_L2) {
         l.x = -T.slack * yn;
@@ -534,7 +537,7 @@ static __global__ __launch_bounds__(1024) void k_mx4_threshold(Mx4Threshold T) {
         l.x = ((1.f - tau) - T.slack - MX4_STEP) * yn;
         l.y = yn < MX4_SHORT ? -inf : 1e-42f;   // (0: a zero vector's dot is 0, and its score NaN)
     }
-    if (tau == inf || yn > MX4_LONG) l = make_float2(0.f, -inf);
+    if (tau == inf) l = make_float2(0.f, -inf);
     if (mx4_dead(T.metric, T.qsq[q])) l = make_float2(0.f, inf);
     T.limit[q] = l;
 }
@@ -685,7 +688,7 @@ __device__ __forceinline__ void mx4_keep_cut(const Mx4Keep &K) {   // all thread
 // called by all threads, with at most `room` keys in all (MX4_NONE: none)
 template <int R> __device__ __forceinline__ void mx4_keep_add(const Mx4Keep &K, const uint64_t (&key)[R], uint32_t room) {
     __syncthreads();
-    const bool full = *K.n + room > MX4_KEEP;   // (the same for all threads: nobody adds before the next barrier)
+    const bool full = *K.n + room > MX4_KEEP || *K.n >= 2 * K.k + 512;   // (the same for all threads: nobody adds before the next barrier)
     __syncthreads();
     if (full) mx4_keep_cut(K);
 #pragma unroll
@@ -698,6 +701,7 @@ struct Mx4Select {
     const uint32_t *counts;     // [nq][segments]
     const Mx4Cand *cand;
     const float *minima, *qnorm;   // DENSE: [nq][n] upper bounds
+    const float *tau;           // others: what the filter took rows by: k scores at least are at or below it
     float slack;
     uint32_t *again;            // [nq]: 1 = the list did not hold the answer: k_mx4_again
     uint64_t *again_limit;      // [nq] ... which then needs nothing above this
@@ -730,48 +734,63 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ Mx4Bins bins;
     __shared__ __attribute__((aligned(8))) uint32_t up_s[MX4_LISTED];   // keys of the upper bounds
+    __shared__ uint16_t segment_s[DENSE ? 1 : MX4_LISTED];   // where a candidate is listed
     __shared__ uint32_t rows_s[2 * MX4_FINISH];
-    __shared__ uint32_t first_s[MX4_SEGMENTS_MAX + 1], n_s, rows_n, last_s;
+    __shared__ uint32_t first_s[MX4_SEGMENTS + 1], n_s, rows_n, last_s;
     __shared__ uint64_t limit_s;
     __shared__ int over_s;
     const uint32_t q = blockIdx.x, me = blockIdx.y;
     const Mx4Keep K{keys, &n_s, &limit_s, S.k};
-    if (threadIdx.x < 64) {
-        constexpr int EACH = MX4_SEGMENTS_MAX / 64;
-        bool over = false;
-        uint32_t sum = 0, own[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const uint32_t seg = threadIdx.x * EACH + i, have = !DENSE && seg < S.segments ? S.counts[(size_t)q * S.segments + seg] : 0;
-            over |= have > S.segment;
-            sum += min(have, S.segment);
-            own[i] = sum;
-        }
-        uint32_t before = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t t = __shfl_up(before, o);
-            if ((int)threadIdx.x >= o) before += t;
-        }
-        before -= sum;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) first_s[threadIdx.x * EACH + i + 1] = before + own[i];
-        const bool any = __any(over);
-        if (threadIdx.x == 0) {
-            first_s[0] = 0;
-            n_s = 0;
-            rows_n = 0;
-            limit_s = MX4_NONE;
-            over_s = any || S.qnorm[q] > MX4_LONG;   // (its dots may be NaN where the scores are not)
-        }
+    if (threadIdx.x == 0) {
+        first_s[0] = 0;
+        n_s = 0;
+        rows_n = 0;
+        limit_s = MX4_NONE;
+        over_s = !DENSE && S.qnorm[q] > MX4_LONG;   // (its dots may be NaN where the scores are not)
     }
     __syncthreads();
-    const uint32_t n = DENSE ? (uint32_t)S.E.rows.n : first_s[MX4_SEGMENTS_MAX];
+    if constexpr (!DENSE) {   // a segment a thread
+        static_assert(MX4_SEGMENTS == MX4_FINISH, "");
+        const uint32_t have = threadIdx.x < S.segments ? S.counts[(size_t)q * S.segments + threadIdx.x] : 0;
+        if (have > S.segment) over_s = 1;
+        uint32_t sum = have;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(sum, o);
+            if ((int)(threadIdx.x & 63) >= o) sum += t;
+        }
+        if ((threadIdx.x & 63) == 63) up_s[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        uint32_t waves = up_s[threadIdx.x & 15];
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const uint32_t t = __shfl_up(waves, o);
+            if ((int)(threadIdx.x & 15) >= o) waves += t;
+        }
+        if (threadIdx.x >= 64) sum += __shfl(waves, (int)(threadIdx.x >> 6) - 1);
+        first_s[threadIdx.x + 1] = sum;
+        for (uint32_t i = sum - have; i < min(sum, MX4_LISTED); i++) segment_s[i] = (uint16_t)threadIdx.x;
+        __syncthreads();
+        if (over_s) {   // part of the list is lost: every row is looked at (k_mx4_again)
+            if (threadIdx.x == 0 && me == 0) {
+                const bool dead = mx4_dead(S.E.metric, S.E.qsq[q]);
+                S.again[q] = !dead;
+                S.ticket[q] = 0;
+                S.again_limit[q] = (uint64_t)mx4_key(S.tau[q]) << 32 | 0xFFFFFFFFu;
+            }
+            return;
+        }
+    }
+    const uint32_t n = DENSE ? (uint32_t)S.E.rows.n : first_s[MX4_SEGMENTS];
     const auto listed = [&](uint32_t i) -> const Mx4Cand & {   // candidate i of all segments
         uint32_t seg = 0;
+        if (i < MX4_LISTED) {
+            seg = segment_s[i];
+        } else {
 #pragma unroll
-        for (uint32_t step = MX4_SEGMENTS_MAX / 2; step; step >>= 1)
-            if (first_s[seg + step] <= i) seg += step;
+            for (uint32_t step = MX4_SEGMENTS / 2; step; step >>= 1)
+                if (first_s[seg + step] <= i) seg += step;
+        }
         return S.cand[((size_t)q * S.segments + seg) * S.segment + (i - first_s[seg])];
     };
     const float y = S.qnorm[q];
@@ -784,7 +803,7 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     };
     const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
     uint32_t key = MX4_KEY_INF;
-    if (n > S.k && n > 2 * at_once) {   // (two rounds' scores cost less than what would save them)
+    if (n > S.k) {
         if (n <= MX4_LISTED) {
             for (uint32_t i = threadIdx.x; i < n; i += MX4_FINISH) up_s[i] = up_key(i);
             key = mx4_kth(bins, n, S.k, [&](uint64_t i) { return up_s[i]; });
@@ -879,7 +898,7 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     __syncthreads();
     const uint32_t have = n_s;
     const auto conclude = [&](uint32_t got, uint64_t kth) {   // one thread
-        S.again[q] = !mx4_dead(S.E.metric, S.E.qsq[q]) && (over_s || (!DENSE && got < min((uint64_t)S.k, S.E.rows.n)));
+        S.again[q] = !DENSE && !mx4_dead(S.E.metric, S.E.qsq[q]) && got < min((uint64_t)S.k, S.E.rows.n);
         S.ticket[q] = 0;
         S.again_limit[q] = got >= S.k ? kth : MX4_NONE - 1;
     };
@@ -926,7 +945,7 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
 // Queries whose candidates overflowed (many rows as near as the k-th), or were fewer than k: every row scored exactly, `slices`
 // workgroups a query, the last one joins their lists.  It only ever reads memory of its own query and waits for nobody.  The grid
 // is slices x groups: a group takes every groups-th query, so that the usual case -- nobody's list overflowed -- is a short launch.
-template <int BITS> static __global__ __launch_bounds__(512) void k_mx4_again(Mx4Select S) {
+template <int BITS> static __global__ __launch_bounds__(512, 4) void k_mx4_again(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];
     __shared__ uint32_t n_s, last_s;
     __shared__ uint64_t limit_s;

@@ -1,7 +1,7 @@
 // mx4_scan_kernels.hpp -- the passes over a table of MXFP4 rows: every row's dot with every query on the matrix cores, then the
 // scores themselves (DENSE), upper bounds of a sample (PROBE, PROBE_ROWS) or the rows that may be among the k best (FILTER).
 #pragma once
-#include "mx4_common.hpp"
+#include "mx4_host.hpp"
 
 #include <type_traits>
 
@@ -44,42 +44,6 @@ template <int BITS> struct Mx4Operand {
         else return mx4_i8{lo[0], lo[1], lo[2], lo[3], 0, 0, 0, 0};
     }
 };
-// A wave's survivors, collected in LDS and sent to their queries' lists 64 at a time: the returning atomic of a list's counter takes
-// microseconds, and a wave that waited for each by itself would do little else.  A list has 32 counters (every panel modulo 32), one
-// would make all waves wait in line.
-struct Mx4Queue {
-    mx4_u4 *slots;       // [MX4_QUEUE], LDS: {query, row, dot}
-    uint32_t n;
-    // norm[q]: |q|
-    __device__ __forceinline__ void flush(const Mx4Scan &P, const float *norm, int lane) {
-        for (uint32_t i = lane; i < n; i += 64) {
-            const mx4_u4 e = slots[i];
-            const uint32_t q = e[0], row = e[1], list = q * MX4_SEGMENTS + ((row >> 5) & (MX4_SEGMENTS - 1));
-            const float x = reinterpret_cast<const float *>(P.rows.at(row >> 5) + P.rows.panel - 128)[row & 31];
-            const uint32_t at = atomicAdd(&P.counts[list], 1u);
-            if (at < P.segment) P.cand[(size_t)list * P.segment + at] = Mx4Cand{row, __uint_as_float(e[2]), x};
-        }
-        n = 0;
-    }
-    // mask: this lane's survivors among its 16 rows (bit v: dot d[v], row row0 + 8 (v / 4) + 4 half + v % 4)
-    __device__ __forceinline__ void push(const Mx4Scan &P, const float *norm, int lane, uint32_t q, uint32_t row0, uint32_t mask, const mx4_f16 &d) {
-        for (;;) {
-            const uint64_t b = __ballot(mask != 0);
-            if (b == 0) break;
-            if (n > MX4_QUEUE - 64) flush(P, norm, lane);
-            if (mask != 0) {
-                const int v = __builtin_ctz(mask);
-                float dot = d[0];
-#pragma unroll
-                for (int i = 1; i < 16; i++) dot = v == i ? d[i] : dot;
-                const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
-                slots[at] = mx4_u4{q, row0 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3), __float_as_uint(dot), 0u};
-                mask &= mask - 1;
-            }
-            n += __builtin_popcountll(b);
-        }
-    }
-};
 // What a row's dot is held against: f(dot, row) >= beta when the row's score may be at or below the query's threshold
 // (k_mx4_threshold).  L2 dot + slack |q| |x| - |x|^2 / 2,  IP dot + slack |q| |x|,  Cosine dot - least cosine x |q| |x|
 template <int M> __device__ __forceinline__ float mx4_held(float d, float x, float alpha) {
@@ -107,6 +71,31 @@ __device__ __forceinline__ uint32_t mx4_rows_below(uint64_t first, uint64_t n) {
     for (int v = 0; v < 16; v++) mask |= first + 8 * (v >> 2) + (v & 3) < n ? 1u << v : 0u;
     return mask;
 }
+// A panel's survivors for one query tile go straight to the workgroup's own part of their query's list: a counter in LDS, stores that
+// nobody waits for.  (Lists that workgroups share want a returning atomic each, which takes microseconds, and where many rows crowd
+// around a threshold all wait for the same few: 1.4 M survivors, 580 us.)  taken, list: this lane's query's.  odd: see its callers
+template <int M> __device__ __forceinline__ void mx4_survive(const Mx4Scan &P, uint32_t *taken, Mx4Cand *list, const mx4_f16 &d, const mx4_f16 &x, float alpha,
+                                                             float beta, uint64_t row0, int half, bool odd) {
+    uint32_t rows = 0, mask = 0;   // rows with a survivor in some lane, this lane's: without branches, which would cost more
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+        const bool hit = mx4_held<M>(d[v], x[v], alpha) >= beta;
+        mask |= hit ? 1u << v : 0u;
+        rows |= __ballot(hit) ? 1u << v : 0u;
+    }
+    if (odd) {
+        asm volatile("");   // (or the compiler computes it every time)
+        rows = 0xFFFFu;
+        mask = mx4_survivors<M>(d, x, alpha, beta) & mx4_rows_below(row0 + 4 * half, P.rows.n);
+    }
+    uint32_t at = mask ? atomicAdd(taken, (uint32_t)__builtin_popcount(mask)) : 0;
+    while (rows) {
+        const int v = __builtin_ctz(rows);
+        rows &= rows - 1;
+        if (mask >> v & 1 && at < P.segment) list[at] = Mx4Cand{(uint32_t)row0 + 8 * (v >> 2) + 4 * half + (v & 3), d[v], x[v]};
+        at += mask >> v & 1;
+    }
+}
 // PROBE: smaller is nearer, then the upper bound (mx4_bounds, a reciprocal's rounding in the slack) of the smallest.  h is per row
 template <int M> __device__ __forceinline__ float mx4_probe_row(float x, bool none) {
     const float inf = __uint_as_float(0x7F800000u), nan = __uint_as_float(0x7FC00000u);
@@ -130,7 +119,7 @@ template <int M> __device__ __forceinline__ float mx4_probe_bound(float best, fl
 }
 
 // The ring of k_mx4_ring: the workgroup's waves bring every panel into LDS together, a KiB at a time in turn, and `stages` panels
-// are under way or in use.  Constants by the chunks of a panel (codes, scales, norms in whole KiB); the stages fill the LDS beside the queues.
+// are under way or in use.  Constants by the chunks of a panel (codes, scales, norms in whole KiB); the stages fill the LDS.
 constexpr int mx4_ring_pieces(int nb) { return (4 * nb * 1024 + nb * 256 + 128 + 1023) / 1024; }
 constexpr int mx4_ring_stages(int nb) { return nb == 2 ? 15 : (nb == 3 ? 10 : 7); }
 constexpr int mx4_ring_bytes(int nb) { return mx4_ring_stages(nb) * mx4_ring_pieces(nb) * 1024; }
@@ -151,11 +140,6 @@ template <int N> __device__ __forceinline__ void mx4_to_lds_first(int wave, uint
 template <int FIRST, int MANY, int FEW> __device__ __forceinline__ void mx4_wait_loads_first(int wave) {   // at most MANY or FEW
     asm volatile("s_cmp_lt_i32 %0, %1\n\ts_cbranch_scc0 .Lmx4_few_%=\n\ts_waitcnt vmcnt(%2)\n\ts_branch .Lmx4_there_%=\n.Lmx4_few_%=:\n\ts_waitcnt vmcnt(%3)\n.Lmx4_there_%=:"
                  ::"s"(wave), "n"(FIRST), "n"(MANY), "n"(FEW) : "memory", "scc");
-}
-// registers of a wave, about: what its operands, sums and panel in flight need
-constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
-    const int regs = (src == MX4_REGS ? qt * nb * (bits == 6 ? 25 : 17) : qt * 12) + qt * 16 + nb * 17 + (mode == MX4_DENSE ? 60 : 105);
-    return regs <= 128 ? 4 : (regs <= 168 ? 3 : (regs <= 256 ? 2 : 1));
 }
 // A wave takes whole panels, one after the other, every wave of the grid in turn.  NB chunks of the panel (256 elements each) are in
 // flight: chunk g of the next panel is requested as soon as chunk g of this one has gone into the matrix cores.  Panels of more than
@@ -178,16 +162,20 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     const char *lds = SRC == MX4_SHARED ? shared : tiles;
     const uint32_t block_q = groups * QT * 32;
     float *yn_b = reinterpret_cast<float *>(shared + (SRC == MX4_SHARED ? QT * P.qtile_bytes : 0));   // |q|, 1 / |q| of the workgroup's queries
-    Mx4Queue queue{reinterpret_cast<mx4_u4 *>(yn_b + 2 * block_q) + wave * MX4_QUEUE, 0};   // FILTER
+    uint32_t *taken = reinterpret_cast<uint32_t *>(yn_b);   // FILTER: candidates of each of them so far
     if constexpr (SRC == MX4_SHARED) {
         const mx4_u4 *src = reinterpret_cast<const mx4_u4 *>(tiles);
         const uint32_t n16 = QT * P.qtile_bytes / 16;
         for (uint32_t i = threadIdx.x; i < n16; i += blockDim.x) reinterpret_cast<mx4_u4 *>(shared)[i] = src[i];
     }
     for (uint32_t i = threadIdx.x; i < block_q; i += blockDim.x) {
-        const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
-        yn_b[i] = y;
-        yn_b[block_q + i] = 1.f / y;
+        if constexpr (MODE == MX4_FILTER) {
+            taken[i] = 0;
+        } else {
+            const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
+            yn_b[i] = y;
+            yn_b[block_q + i] = 1.f / y;
+        }
     }
     __syncthreads();
     const float *yn_s = yn_b + group * QT * 32, *yr_s = yn_s + block_q;
@@ -225,8 +213,9 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     }
     const uint32_t abreast = (blockDim.x / 64) / groups;   // panels that a workgroup's waves take at a time
     const uint32_t W = gridDim.x * abreast, n_take = (uint32_t)P.n_take;
-    uint32_t w = blockIdx.x * abreast + wave / groups;
-    if (w >= n_take) return;
+    // FILTER: neighbouring panels go to different workgroups, so that rows that crowd together fill no part of a list
+    uint32_t w = MODE == MX4_FILTER ? wave * gridDim.x + blockIdx.x : blockIdx.x * abreast + wave / groups;
+    if (MODE != MX4_FILTER && w >= n_take) return;
     const auto panel_of = [&](uint32_t i) -> uint64_t { return MODE == MX4_PROBE ? (i * P.every) >> 24 : i; };
     Mx4Chunk buf[NB];
     mx4_f4 nrm[4];   // |x| of this lane's 16 rows (DENSE: nx, its one row), loaded with the panel's first chunks
@@ -238,7 +227,7 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
             for (int i = 0; i < 4; i++) nrm[i] = mx4_in_memory<mx4_f4>(of + P.rows.panel - 128)[2 * i + half];
         }
     };
-    uint64_t panel = P.rows.uniform_at(panel_of(w));
+    uint64_t panel = P.rows.uniform_at(panel_of(min(w, n_take - 1)));
     fetch_norms(panel);
 #pragma unroll
     for (int g = 0; g < NB; g++)
@@ -322,16 +311,15 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
                 least = fminf(least, xn[v]);
                 longest = fmaxf(longest, xn[v]);
             }
-            const bool odd = __any(longest > MX4_LONG || (M == MX4_COSINE && least < MX4_SHORT));
+            const bool odd = tail || __any(longest > MX4_LONG || (M == MX4_COSINE && least < MX4_SHORT));
 #pragma unroll
             for (int q = 0; q < QT; q++) {
                 float most = mx4_held<M>(acc[q][0], xn[0], alpha[q]);
 #pragma unroll
                 for (int v = 1; v < 16; v++) most = fmaxf(most, mx4_held<M>(acc[q][v], xn[v], alpha[q]));
                 if (!__any(most >= beta[q]) && !odd) continue;
-                uint32_t mask = mx4_survivors<M>(acc[q], xn, alpha[q], beta[q]);
-                if (tail) mask &= mx4_rows_below(row0 + 4 * half, P.rows.n);
-                queue.push(P, yn_s - q0, lane, q0 + q * 32 + col, (uint32_t)row0, mask, acc[q]);
+                const uint32_t me = q * 32 + col;
+                mx4_survive<M>(P, taken + me, P.cand + ((size_t)(q0 + me) * P.segments + blockIdx.x) * P.segment, acc[q], xn, alpha[q], beta[q], row0, half, odd);
             }
         };
         const auto probe = [&](auto metric) {
@@ -385,14 +373,16 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
         }
         panel = next;
     }
-    if constexpr (MODE == MX4_FILTER) queue.flush(P, yn_s - q0, lane);
+    if constexpr (MODE == MX4_FILTER) {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < block_q && block_q0 + i < P.nq; i += blockDim.x) P.counts[(size_t)(block_q0 + i) * P.segments + blockIdx.x] = taken[i];
+    }
 }
 
 // The same passes for 65 to 256 queries against rows of at most 1024 elements.  Four waves, QT tiles each, take every panel together; it
 // comes through LDS, so that the memory's latency is covered by a ring of panels and not by registers, which hold the operands.  One
 // wave a SIMD: the comparisons of the panel before are made between the matrix instructions of this one, whose last chunk covers the
-// barrier and the first reads of the next.  Survivors go straight to the workgroup's own part of their query's list (a counter in LDS, a
-// store that nobody waits for): a queue's flush would wait for the ring's loads as well.
+// barrier and the first reads of the next. 
 // 1M x 1024, few survivors: 128 queries 105 us (5.2 TB/s: the memory), 256 queries 160 us (537 GFLOP at 3.4 PFLOP/s; the chip's clock
 // falls to 1.7 GHz under it, and with less work beside the matrix instructions hardly rises).  Each panel with survivors costs its
 // wave some 800 cycles: 256 queries, top-100: 245 us.  Eight waves of one tile each read the LDS twice as often: 207 us.
@@ -503,26 +493,7 @@ template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_
             for (int q = 0; q < QT; q++) {
                 if (any[q] == 0 && !odd) continue;
                 const uint32_t me = wave * QT * 32 + q * 32 + col;
-                Mx4Cand *list = P.cand + ((size_t)(block_q0 + me) * P.segments + blockIdx.x) * P.segment;
-                uint32_t rows = 0, mask = 0;   // rows with a survivor in some lane, this lane's: without branches, which would cost more
-#pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const bool hit = mx4_held<M>(p.acc[q][v], p.x[v], alpha[q]) >= beta[q];
-                    mask |= hit ? 1u << v : 0u;
-                    rows |= __ballot(hit) ? 1u << v : 0u;
-                }
-                if (odd) {
-                    asm volatile("");
-                    rows = 0xFFFFu;
-                    mask = mx4_survivors<M>(p.acc[q], p.x, alpha[q], beta[q]) & mx4_rows_below(row0 + 4 * half, P.rows.n);
-                }
-                uint32_t at = mask ? atomicAdd(&taken[me], (uint32_t)__builtin_popcount(mask)) : 0;
-                while (rows) {
-                    const int v = __builtin_ctz(rows);
-                    rows &= rows - 1;
-                    if (mask >> v & 1 && at < P.segment) list[at] = Mx4Cand{(uint32_t)row0 + 8 * (v >> 2) + 4 * half + (v & 3), p.acc[q][v], p.x[v]};
-                    at += mask >> v & 1;
-                }
+                mx4_survive<M>(P, taken + me, P.cand + ((size_t)(block_q0 + me) * P.segments + blockIdx.x) * P.segment, p.acc[q], p.x, alpha[q], beta[q], row0, half, odd);
             }
         } else {
 #pragma unroll

@@ -8,13 +8,11 @@ namespace vsg {
 
 template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hipStream_t s, const Mx4Scan &P, const Mx4ScanShape &shape) {
     const uint32_t waves = SRC == MX4_REGS && P.groups == 3 ? 3 : 4, groups = SRC == MX4_REGS ? P.groups : 1, abreast = waves / groups;
-    const size_t lds = (SRC == MX4_SHARED ? (size_t)QT * P.qtile_bytes : 0) + groups * QT * 256 + (MODE == MX4_FILTER ? waves * MX4_QUEUE * 16 : 0);
+    const uint32_t y = SRC == MX4_REGS ? 1 : shape.y;   // (REGS: all of a batch's tiles in one workgroup)
+    const size_t lds = mx4_scan_lds(SRC, QT, groups, P.qtile_bytes);
     if (lds > 64 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    // as many workgroups as stay resident; few panels: fewer, so that a wave's start is not most of its work
-    const uint64_t fit = std::max<uint64_t>(1, std::min<uint64_t>(mx4_scan_waves(BITS, QT, MODE, NB, SRC), (160 * 1024) / (lds + 512)));
-    const uint32_t y = SRC == MX4_REGS ? 1 : shape.y;   // (REGS: all of a batch's tiles in one workgroup)
-    const uint64_t gx = std::max<uint64_t>(1, std::min<uint64_t>((P.n_take + abreast - 1) / abreast, (uint64_t)shape.cus * fit / y));
+    const uint64_t gx = MODE == MX4_FILTER ? P.segments : mx4_scan_grid(BITS, QT, MODE, NB, SRC, lds, P.n_take, abreast, shape.cus, y);
     hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, SRC>), dim3((unsigned)gx, y), dim3(64 * waves), lds, s, P);
     HIPCHK(hipGetLastError());
     return VSGPU_OK;

@@ -25,7 +25,7 @@ struct DeviceScope {
 
 constexpr size_t MAX_DIM = 65536, MAX_ROWS = 0xFFFFFFE0ull, QUERY_BATCH = 256;
 constexpr int PLAN_CUS = 256;   // what sizes a workspace: it does not depend on the device that will be given it
-constexpr size_t LDS_BUDGET = 160 * 1024 - 4 * MX4_QUEUE * 16;   // for the queries' operands; the rest is the filter's queues
+constexpr size_t LDS_BUDGET = 160 * 1024 - 1024;   // for the queries' operands
 
 int elem_size(int type) { return type == VSGPU_F32 ? 4 : (type == VSGPU_F16 || type == VSGPU_BF16 ? 2 : 0); }
 
@@ -118,14 +118,13 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
         p.minima = 2 * p.take;
         expected = k * ((p.panels + p.take - 1) / p.take);
     }
-    // Panels are dealt over the segments in turn, so that only rows crowded around the threshold fill one: a few times its share
-    if (p.shape.ring && !p.dense) {
-        p.segments = (uint32_t)std::min<uint64_t>({(uint64_t)PLAN_CUS, (uint64_t)MX4_SEGMENTS_MAX, p.panels});
-        p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 40);
-    } else {
-        p.segments = MX4_SEGMENTS;
-        p.segment = (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 4 / MX4_SEGMENTS + 64);
-    }
+    // A segment for each workgroup of the filter.  Panels are dealt over them in turn, so that only rows crowded around the threshold
+    // fill one: twice its share and two panels
+    if (p.shape.ring) p.segments = (uint32_t)std::min<uint64_t>(PLAN_CUS, p.panels);
+    else p.segments = (uint32_t)mx4_scan_grid(bits, p.shape.qt, MX4_FILTER, p.shape.src == MX4_GLOBAL ? 4 : mx4_scan_chunks(mx4_groups((uint32_t)dim)),
+                                              p.shape.src == MX4_GLOBAL ? MX4_GLOBAL : MX4_SHARED,
+                                              mx4_scan_lds(p.shape.src == MX4_GLOBAL ? MX4_GLOBAL : MX4_SHARED, p.shape.qt, 1, p.qtile_bytes), p.panels, 4, PLAN_CUS, p.shape.y);
+    p.segment = p.dense ? 0 : (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 72);
     // k rows or more are scored exactly, a workgroup 1024 / lanes of them at once: several of these rounds are worth a second workgroup
     const size_t rounds = k * mx4_row_lanes(mx4_steps((uint32_t)dim)) / 1024;
     p.shares = (uint32_t)std::max<size_t>(1, std::min<size_t>({MX4_SHARES, rounds / 2, (size_t)PLAN_CUS / nq}));
@@ -158,6 +157,7 @@ static QueryBlock take_queries(Layout &L, const Plan &p) {
 struct TopkBlock {
     QueryBlock q;
     float2 *limit;
+    float *tau;
     uint32_t *done, *counts, *share_n, *again, *ticket;
     uint64_t *again_limit, *share;
     float *minima;
@@ -168,8 +168,9 @@ static TopkBlock take_topk(Layout &L, const Plan &p, size_t nq, size_t k) {
     TopkBlock b;
     b.q = take_queries(L, p);
     b.limit = L.take<float2>(nq);
-    b.done = L.take<uint32_t>(nq * (1 + (size_t)p.segments));
-    b.counts = b.done + nq;
+    b.tau = L.take<float>(nq);
+    b.done = L.take<uint32_t>(nq);
+    b.counts = L.take<uint32_t>(p.dense ? 0 : nq * (size_t)p.segments);
     b.share_n = L.take<uint32_t>(p.shares > 1 ? nq * p.shares : 0);
     b.share = L.take<uint64_t>(p.shares > 1 ? nq * p.shares * (size_t)p.room : 0);
     b.again = L.take<uint32_t>(nq);
@@ -259,8 +260,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     L.base = static_cast<char *>(ws);
     const TopkBlock b = take_topk(L, p, nq, k);
     if (L.at > ws_bytes) return fail(VSGPU_ERR_ARG, "workspace of %zu bytes, %zu needed", ws_bytes, L.at);
-    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.done,
-                                nq * (p.shape.ring ? 1 : 1 + p.segments));   // (k_mx4_ring's counters are its own)
+    int rc = mx4_launch_queries(s, queries, type, qstride, nq, R, bits, p.tiles, b.q.tiles, b.q.norm, b.q.sq, b.done, nq);
     if (rc) return rc;
     Mx4Scan P{};
     P.rows = R;
@@ -284,7 +284,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     rc = launch_scan(s, p.by_row ? MX4_PROBE_ROWS : MX4_PROBE, P, p, bits);
     if (rc) return rc;
     if (!p.dense) {
-        const Mx4Threshold T{b.minima, p.minima, p.minima, (uint32_t)k, (uint32_t)metric, b.q.norm, b.q.sq, b.limit, P.slack};
+        const Mx4Threshold T{b.minima, p.minima, p.minima, (uint32_t)k, (uint32_t)metric, b.q.norm, b.q.sq, b.limit, b.tau, P.slack};
         hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
         HIPCHK(hipGetLastError());
         P.n_take = p.panels;
@@ -315,6 +315,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     S.ticket = b.ticket;
     S.minima = b.minima;
     S.qnorm = b.q.norm;
+    S.tau = b.tau;
     S.slack = P.slack;
     const dim3 fg((unsigned)nq, p.shares), ag(p.slices, (unsigned)std::max<size_t>(1, std::min<size_t>(nq, (size_t)cus / p.slices)));
     if (p.dense) {
