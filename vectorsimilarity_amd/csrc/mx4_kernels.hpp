@@ -19,24 +19,33 @@ template <int T> __device__ __forceinline__ float mx4_widen(const void *p, size_
 // 16 bytes of a caller's vectors, aligned to their elements only (the memory takes a wide access at any of their addresses)
 typedef float mx4_f4_at __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t mx4_u4_at __attribute__((ext_vector_type(4), aligned(2)));
+template <int T> constexpr int MX4_EACH = T == MX4_F32 ? 4 : 8;   // elements of such an access
+template <int T> __device__ __forceinline__ void mx4_widen16(const void *x, int i, float v[32]) {   // the i-th
+    if constexpr (T == MX4_F32) {
+        const mx4_f4_at w = static_cast<const mx4_f4_at *>(x)[i];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
+    } else {
+        const mx4_u4_at w = static_cast<const mx4_u4_at *>(x)[i];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+            v[8 * i + j] = T == MX4_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+        }
+    }
+}
 // 32 elements from x on, `have` of them in the row
 template <int T> __device__ __forceinline__ void mx4_load32(const void *x, int have, float v[32]) {
-    constexpr int EACH = T == MX4_F32 ? 4 : 8;   // a load's
+    constexpr int EACH = MX4_EACH<T>;
+    if (have >= 32) {   // (by itself: all of its loads are under way together)
+#pragma unroll
+        for (int i = 0; i < 32 / EACH; i++) mx4_widen16<T>(x, i, v);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 32 / EACH; i++) {
         if (EACH * (i + 1) <= have) {
-            if constexpr (T == MX4_F32) {
-                const mx4_f4_at w = static_cast<const mx4_f4_at *>(x)[i];
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[4 * i + j] = w[j];
-            } else {
-                const mx4_u4_at w = static_cast<const mx4_u4_at *>(x)[i];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-                    v[8 * i + j] = T == MX4_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
-                }
-            }
+            mx4_widen16<T>(x, i, v);
         } else {
 #pragma unroll
             for (int j = EACH * i; j < EACH * (i + 1); j++) v[j] = j < have ? mx4_widen<T>(x, (size_t)j) : 0.f;
@@ -121,7 +130,8 @@ static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) 
     else atomicMax(norm, 0x80000000u | (uint32_t)i);
 }
 // One workgroup takes 32 vectors, its waves (up to 16) the k-steps in turn; a lane rounds one block (half, row) by itself, so neither
-// the maximum nor the codes cross lanes.
+// the maximum nor the codes cross lanes.  Bound by memory: 1M x 768 bf16 into rows in any order 405 us, 1.95 GB at 4.8 TB/s (a copy of
+// the card's: 4.76), although a row's codes are 16-byte pieces 512 bytes apart; 4097 x 1000 fp16 10 us.
 template <int T> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
     __shared__ double part[16][64];
     __shared__ int64_t slot_s[32];
@@ -206,7 +216,9 @@ __device__ __forceinline__ float mx4_code_value(uint32_t c) {   // c: 4 bits
     const float v = m < 2 ? 0.5f * (float)m : (float)((2u | (m & 1u)) << ((m >> 1) - 1)) * 0.5f;
     return c & 8u ? -v : v;
 }
-// A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  A
+// A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  Rows in
+// any order cost the sectors around their 16-byte pieces, four times their bytes: 700K of 1M x 1024 to bf16 708 us (1.43 GB written,
+// 1.7 GB read: 4.4 TB/s), 1M x 768 524 us; 100 rows of 128 2.7 us.  A
 // workgroup takes `rows` whole rows (rows * per_row < 2^16: the division is one multiplication, by ceil(2^32 / per_row)).
 template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t recip) {
     const uint64_t i0 = (uint64_t)blockIdx.x * rows;
@@ -505,6 +517,7 @@ struct Mx4Threshold {
 };
 // a Cosine query of norm zero, or one that holds an infinity or a NaN: every score is NaN
 __device__ __forceinline__ bool mx4_dead(uint32_t metric, double sq) { return !(sq == sq) || (metric == MX4_COSINE && sq == 0); }
+// One workgroup a query, latency of a few passes over LDS: 256 queries of 7800 bounds 10.8 us, 1 of 400 4.2 us.
 // tau = a little above the k-th smallest upper bound (each of different rows, so at least k rows are at or below it), then what the
 // filter compares against
 constexpr uint32_t MX4_STAGED = 16384;
@@ -727,6 +740,9 @@ __device__ __forceinline__ void mx4_emit(const Mx4Select &S, uint32_t q, const u
 // Of a query's candidates only those whose lower bound is at or below the k-th smallest upper bound (little more than k) are scored
 // exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds the probe's.  Few
 // queries with many rows to score: `shares` workgroups a query, each with every shares-th 64 candidates; the last one to end joins them.
+// Steps of latency, then the gather: 1 query, k 10 9.1 us (lists 2, bounds and their k-th 3.5, scores 1.1, ranks 0.9); 256 queries
+// against 1M x 1024, k 100 34 us, of which 20 the 26 K rows' pieces (64 bytes of memory each); 7 queries, k 1000 27 us (one workgroup
+// a query 52, with a bitonic sort of the k).
 constexpr uint32_t MX4_FINISH = 1024;
 constexpr uint32_t MX4_SHARES = 16;     // most workgroups a query
 constexpr uint32_t MX4_LISTED = 6144;   // candidates kept in LDS; more are read from memory every time
@@ -942,8 +958,9 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     if (threadIdx.x == 0) conclude(got, keys[S.k - 1]);
     mx4_emit(S, q, keys, got);
 }
-// Queries whose candidates overflowed (many rows as near as the k-th), or were fewer than k: every row scored exactly, `slices`
-// workgroups a query, the last one joins their lists.  It only ever reads memory of its own query and waits for nobody.  The grid
+// Queries whose candidates overflowed (many rows as near as the k-th, or beyond fp32), or were fewer than k: every row scored exactly, `slices`
+// workgroups a query, the last one joins their lists.  It only ever reads memory of its own query and waits for nobody.  All
+// rows of one score, the worst case: 41 queries against 67 K x 1 270 us, 32 against 2.8M x 3 (k 26) 200.  The grid
 // is slices x groups: a group takes every groups-th query, so that the usual case -- nobody's list overflowed -- is a short launch.
 template <int BITS> static __global__ __launch_bounds__(512, 4) void k_mx4_again(Mx4Select S) {
     __shared__ uint64_t keys[MX4_KEEP];

@@ -112,8 +112,10 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
         p.minima = n;
         expected = k;
     } else {
-        // a probe of n / div rows leaves about k div candidates per query: div balances its bytes against what they cost
-        const double div = std::min(64.0, std::max(8.0, std::sqrt(0.15 * (double)n / ((double)nq * (double)k))));
+        // a probe of n / div rows leaves about k div candidates per query: div balances its bytes against what they cost.  Whole
+        // calls at div 8 | 16 | 32 | 64: 64 queries x 4M x 768, k 10: 356 | 324 | 315 | 312 us, k 100: 381 | 357 | 350 | 357;
+        // 256 x 1M x 1024, k 10: 255 | 250 | 264 | 279, k 100: 313 | 338 | 362 | 406
+        const double div = std::min(64.0, std::max(8.0, std::sqrt((double)n / ((double)nq * (double)k))));
         p.take = std::min<uint64_t>(p.panels, std::max<uint64_t>((uint64_t)((double)p.panels / div), 4 * k));
         p.minima = 2 * p.take;
         expected = k * ((p.panels + p.take - 1) / p.take);
