@@ -757,18 +757,19 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     __shared__ int over_s;
     const uint32_t q = blockIdx.x, me = blockIdx.y;
     const Mx4Keep K{keys, &n_s, &limit_s, S.k};
+    static_assert(MX4_SEGMENTS == MX4_FINISH, "");
+    const uint32_t have = !DENSE && threadIdx.x < S.segments ? S.counts[(size_t)q * S.segments + threadIdx.x] : 0;   // a segment a thread
+    const float y = S.qnorm[q];
     if (threadIdx.x == 0) {
         first_s[0] = 0;
         n_s = 0;
         rows_n = 0;
         limit_s = MX4_NONE;
-        over_s = !DENSE && S.qnorm[q] > MX4_LONG;   // (its dots may be NaN where the scores are not)
+        over_s = 0;
     }
     __syncthreads();
-    if constexpr (!DENSE) {   // a segment a thread
-        static_assert(MX4_SEGMENTS == MX4_FINISH, "");
-        const uint32_t have = threadIdx.x < S.segments ? S.counts[(size_t)q * S.segments + threadIdx.x] : 0;
-        if (have > S.segment) over_s = 1;
+    if constexpr (!DENSE) {
+        if (have > S.segment || y > MX4_LONG) over_s = 1;   // (a long query's dots may be NaN where the scores are not)
         uint32_t sum = have;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -809,7 +810,6 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         }
         return S.cand[((size_t)q * S.segments + seg) * S.segment + (i - first_s[seg])];
     };
-    const float y = S.qnorm[q];
     const auto bounds = [&](const Mx4Cand &c, float &low, float &up) { mx4_bounds(S.E.metric, c.dot, c.x, y, S.slack, low, up); };
     const auto up_key = [&](uint64_t i) {
         float up, low;
@@ -912,13 +912,13 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         }
     }
     __syncthreads();
-    const uint32_t have = n_s;
+    const uint32_t scored = n_s;
     const auto conclude = [&](uint32_t got, uint64_t kth) {   // one thread
         S.again[q] = !DENSE && !mx4_dead(S.E.metric, S.E.qsq[q]) && got < min((uint64_t)S.k, S.E.rows.n);
         S.ticket[q] = 0;
         S.again_limit[q] = got >= S.k ? kth : MX4_NONE - 1;
     };
-    if (2 * have <= MX4_LISTED) {   // (up_s is free by now)
+    if (2 * scored <= MX4_LISTED) {   // (up_s is free by now)
         if (threadIdx.x == 0) {
             rows_n = 0;
             limit_s = MX4_NONE;
@@ -933,12 +933,12 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
             atomicAdd(&rows_n, 1u);
         };
         bool done = true;
-        if (have > 256) {
-            done = mx4_ranked(bins, keys, have, reinterpret_cast<uint64_t *>(up_s), emit);
-        } else if (threadIdx.x < have && keys[threadIdx.x] != MX4_NONE) {   // few: against each of the others
+        if (scored > 256) {
+            done = mx4_ranked(bins, keys, scored, reinterpret_cast<uint64_t *>(up_s), emit);
+        } else if (threadIdx.x < scored && keys[threadIdx.x] != MX4_NONE) {   // few: against each of the others
             const uint64_t key = keys[threadIdx.x];
             uint32_t rank = 0;
-            for (uint32_t j = 0; j < have; j++) rank += keys[j] < key;
+            for (uint32_t j = 0; j < scored; j++) rank += keys[j] < key;
             emit(rank, key);
         }
         __syncthreads();
@@ -967,6 +967,8 @@ template <int BITS> static __global__ __launch_bounds__(512, 4) void k_mx4_again
     __shared__ uint32_t n_s, last_s;
     __shared__ uint64_t limit_s;
     constexpr int EACH = 4;   // rows under way to a lane
+    const uint32_t ask = blockIdx.y + threadIdx.x * gridDim.y;   // (all of a group's queries at once: a batch has fewer than threads)
+    if (!__syncthreads_or(ask < S.nq && S.again[ask])) return;
     for (uint32_t q = blockIdx.y; q < S.nq; q += gridDim.y) {
         if (!S.again[q]) continue;
         const Mx4Keep K{keys, &n_s, &limit_s, S.k};

@@ -27,6 +27,8 @@ _TYPES = {torch.float32: _capi.VecSimType_FLOAT32, torch.float16: _capi.VecSimTy
 _METRICS = (VecSimMetric_L2, VecSimMetric_IP, VecSimMetric_Cosine)
 _ERR_ARG, _ERR_UNSUPPORTED = 3, 4
 _lib = None
+# torch.cuda.current_stream(device).cuda_stream, a microsecond sooner
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _load():
@@ -136,7 +138,7 @@ def write(table, vectors, slots=None, first=0):
     if m == 0:
         return
     device = table.device.index
-    rc = lib.vsgpu_mx4_write(device, torch.cuda.current_stream(device).cuda_stream, table.data_ptr(), capacity, dim, x.data_ptr(), kind, m, stride,
+    rc = lib.vsgpu_mx4_write(device, _stream(device), table.data_ptr(), capacity, dim, x.data_ptr(), kind, m, stride,
                              where, size, first)
     if rc:
         _raise(rc)
@@ -163,7 +165,7 @@ def read(table, dim, slots=None, dtype=torch.float32, n=None):
     out = torch.empty((m, dim), dtype=dtype, device=table.device)
     if m:
         device = table.device.index
-        rc = lib.vsgpu_mx4_read(device, torch.cuda.current_stream(device).cuda_stream, table.data_ptr(), capacity, dim, where, size, 0, m,
+        rc = lib.vsgpu_mx4_read(device, _stream(device), table.data_ptr(), capacity, dim, where, size, 0, m,
                                 out.data_ptr(), kind, dim * out.element_size())
         if rc:
             _raise(rc)
@@ -192,7 +194,7 @@ def scores(table, n, queries, metric, query_bits=6):
         size = _scores_bytes(dim, nq, query_bits)
         ws = torch.empty(size, dtype=torch.uint8, device=table.device)
         device = table.device.index
-        rc = lib.vsgpu_mx4_scores(device, torch.cuda.current_stream(device).cuda_stream, table.data_ptr(), n, dim, q.data_ptr(), kind, nq, stride,
+        rc = lib.vsgpu_mx4_scores(device, _stream(device), table.data_ptr(), n, dim, q.data_ptr(), kind, nq, stride,
                                   metric, query_bits, out.data_ptr(), n, ws.data_ptr(), size)
         if rc:
             _raise(rc)
@@ -215,7 +217,7 @@ def topk(table, n, queries, k, metric, query_bits=6):
         size = _topk_bytes(n, dim, nq, k, query_bits)
         ws = torch.empty(size, dtype=torch.uint8, device=table.device)
         device = table.device.index
-        rc = lib.vsgpu_mx4_topk(device, torch.cuda.current_stream(device).cuda_stream, table.data_ptr(), n, dim, q.data_ptr(), kind, nq, stride, k,
+        rc = lib.vsgpu_mx4_topk(device, _stream(device), table.data_ptr(), n, dim, q.data_ptr(), kind, nq, stride, k,
                                 metric, query_bits, ids.data_ptr(), best.data_ptr(), ws.data_ptr(), size)
         if rc:
             _raise(rc)
