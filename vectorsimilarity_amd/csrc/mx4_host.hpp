@@ -16,10 +16,17 @@ constexpr int mx4_scan_waves(int bits, int qt, int mode, int nb, int src) {
     const int regs = (src == MX4_REGS ? qt * nb * (bits == 6 ? 25 : 17) : qt * 12) + qt * 16 + nb * 17 + (mode == MX4_DENSE ? 60 : 105);
     return regs <= 128 ? 4 : (regs <= 168 ? 3 : (regs <= 256 ? 2 : 1));
 }
-// ... its workgroups along the table: as many as stay resident; few panels: fewer, so that a wave's start is not most of its work
-inline uint64_t mx4_scan_grid(int bits, int qt, int mode, int nb, int src, size_t lds, uint64_t n_take, uint32_t abreast, int cus, uint32_t y) {
-    const uint64_t fit = lds + 512 > 160 * 1024 ? 1 : (160 * 1024) / (lds + 512), waves = (uint64_t)mx4_scan_waves(bits, qt, mode, nb, src);
-    const uint64_t all = (uint64_t)cus * (fit < waves ? fit : waves) / y, need = (n_take + abreast - 1) / abreast;
+// ... its workgroups along the table: as many as stay resident; few panels: fewer, so that a wave's start is not most of its work.
+// y > 1: workgroups side by side take the same panels, each with its own queries.  They are on one XCD (workgroups are dealt over eight)
+// and share its L2, which holds what they read while it is one workgroup a CU; for scores, and where panels are large (400K x 1536,
+// 256 queries: scores 285 -> 228 us, top-10 232 -> 224; 300K x 2048 with 4 bits: 266 -> 194, 218 -> 197; but top-10 of
+// 400K x 1100 179 -> 203, of 2M x 128 225 -> 329).
+inline uint64_t mx4_scan_grid(int bits, int qt, int mode, int nb, int src, size_t lds, uint64_t n_take, uint32_t kg, uint32_t abreast, int cus, uint32_t y) {
+    const bool alone = lds + 512 > 160 * 1024 || (src == MX4_SHARED && y > 1 && (mode == MX4_DENSE || kg > 5));
+    const uint64_t fit = alone ? 1 : (160 * 1024) / (lds + 512), waves = (uint64_t)mx4_scan_waves(bits, qt, mode, nb, src);
+    uint64_t all = (uint64_t)cus * (fit < waves ? fit : waves) / y;
+    if (y > 1 && all >= 16) all &= ~(uint64_t)7;
+    const uint64_t need = (n_take + abreast - 1) / abreast;
     return all < need ? (all ? all : 1) : need;
 }
 inline int mx4_scan_chunks(uint32_t kg) { return kg == 1 ? 1 : 4; }   // SHARED: a panel's chunks in flight

@@ -12,7 +12,7 @@ template <int BITS, int QT, int MODE, int NB, int SRC> static int launch_scan(hi
     const size_t lds = mx4_scan_lds(SRC, QT, groups, P.qtile_bytes);
     if (lds > 64 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(k_mx4_scan<BITS, QT, MODE, NB, SRC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    const uint64_t gx = MODE == MX4_FILTER ? P.segments : mx4_scan_grid(BITS, QT, MODE, NB, SRC, lds, P.n_take, abreast, shape.cus, y);
+    const uint64_t gx = MODE == MX4_FILTER ? P.segments : mx4_scan_grid(BITS, QT, MODE, NB, SRC, lds, P.n_take, P.rows.kg, abreast, shape.cus, y);
     hipLaunchKernelGGL((k_mx4_scan<BITS, QT, MODE, NB, SRC>), dim3((unsigned)gx, y), dim3(64 * waves), lds, s, P);
     HIPCHK(hipGetLastError());
     return VSGPU_OK;

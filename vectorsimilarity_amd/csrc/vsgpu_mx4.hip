@@ -125,7 +125,7 @@ static Plan plan_topk(size_t n, size_t dim, size_t nq, size_t k, int bits, int c
     if (p.shape.ring) p.segments = (uint32_t)std::min<uint64_t>(PLAN_CUS, p.panels);
     else p.segments = (uint32_t)mx4_scan_grid(bits, p.shape.qt, MX4_FILTER, p.shape.src == MX4_GLOBAL ? 4 : mx4_scan_chunks(mx4_groups((uint32_t)dim)),
                                               p.shape.src == MX4_GLOBAL ? MX4_GLOBAL : MX4_SHARED,
-                                              mx4_scan_lds(p.shape.src == MX4_GLOBAL ? MX4_GLOBAL : MX4_SHARED, p.shape.qt, 1, p.qtile_bytes), p.panels, 4, PLAN_CUS, p.shape.y);
+                                              mx4_scan_lds(p.shape.src == MX4_GLOBAL ? MX4_GLOBAL : MX4_SHARED, p.shape.qt, 1, p.qtile_bytes), p.panels, mx4_groups((uint32_t)dim), 4, PLAN_CUS, p.shape.y);
     p.segment = p.dense ? 0 : (uint32_t)std::min<uint64_t>((p.panels + p.segments - 1) / p.segments * 32, expected * 2 / p.segments + 72);
     // k rows or more are scored exactly, a workgroup 1024 / lanes of them at once: several of these rounds are worth a second workgroup
     const size_t rounds = k * mx4_row_lanes(mx4_steps((uint32_t)dim)) / 1024;
