@@ -495,3 +495,14 @@ def test_many_queries_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(got, (*mx4.topk(table, n, q, 10, ref.L2), *mx4.topk(table, n, q[:20], 1000, ref.IP))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("nq,n,dim,k", [(1, 64, 1024, 5), (40, 65, 1024, 64), (3, 512, 128, 100), (300, 513, 100, 7), (2, 1024, 64, 1024), (2, 1025, 64, 9), (5, 16, 9000, 4)])
+def test_topk_of_very_small_tables(nq, n, dim, k, metric):
+    """on both sides of the size up to which every row is scored without a probe; zero, short, long and NaN rows among them"""
+    x, q = vectors(n, dim, 1), vectors(nq, dim, 2)
+    x[1], x[2, 0], x[3], x[5] = 0, float("nan"), x[3] * 1e-30, x[5] * 2.0 ** 80
+    q[-1] *= 2.0 ** 90
+    check_topk(x, q, k, metric, 6)
+    check_topk(x, q, k, metric, 4)

@@ -738,7 +738,8 @@ __device__ __forceinline__ void mx4_emit(const Mx4Select &S, uint32_t q, const u
     }
 }
 // Of a query's candidates only those whose lower bound is at or below the k-th smallest upper bound (little more than k) are scored
-// exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds the probe's.  Few
+// exactly, a lane a block; then sorted.  DENSE: the candidates are all rows of a small table, their upper bounds the probe's
+// (without a probe none, and every row is scored).  Few
 // queries with many rows to score: `shares` workgroups a query, each with every shares-th 64 candidates; the last one to end joins them.
 // Steps of latency, then the gather: 1 query, k 10 9.1 us (lists 2, bounds and their k-th 3.5, scores 1.1, ranks 0.9); 256 queries
 // against 1M x 1024, k 100 34 us, of which 20 the 26 K rows' pieces (64 bytes of memory each); 7 queries, k 1000 27 us (one workgroup
@@ -819,7 +820,8 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
     };
     const uint32_t lanes = mx4_row_lanes(S.E.rows.ks), at_once = MX4_FINISH / lanes;
     uint32_t key = MX4_KEY_INF;
-    if (n > S.k) {
+    const bool all = DENSE && !S.minima;   // a table of few rows: every one of them
+    if (n > S.k && !all) {
         if (n <= MX4_LISTED) {
             for (uint32_t i = threadIdx.x; i < n; i += MX4_FINISH) up_s[i] = up_key(i);
             key = mx4_kth(bins, n, S.k, [&](uint64_t i) { return up_s[i]; });
@@ -835,7 +837,9 @@ template <int BITS, bool DENSE> static __global__ __launch_bounds__(1024) void k
         if (j < mine && i < n) {
             uint32_t row = i;
             float low;
-            if constexpr (DENSE) {
+            if (all) {
+                low = -__uint_as_float(0x7F800000u);
+            } else if constexpr (DENSE) {
                 const float up = S.minima[(size_t)q * S.E.rows.n + i];
                 const float x = reinterpret_cast<const float *>(S.E.rows.at(i / 32) + S.E.rows.panel - 128)[i & 31];
                 low = mx4_low(S.E.metric, up, x, y, S.slack);
