@@ -119,7 +119,8 @@ __device__ __forceinline__ int64_t mx4_slot(const void *slots, int is64, uint64_
     if (!slots) return (int64_t)(first + i);
     return is64 ? static_cast<const int64_t *>(slots)[i] : (int64_t)static_cast<const int32_t *>(slots)[i];
 }
-// Which vector a slot gets when several name it: the last.  Two passes over the norms: cleared, then the largest 2^31 | i.
+// Which vector a slot gets when several name it: the last.  Two passes over the norms: cleared, then the largest 2^31 | i (4097 slots
+// 2.7 us each, 1M 5.2; up to 4096 vectors k_mx4_write looks for later ones with its slots itself).
 static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) {
     const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= W.m) return;
@@ -284,7 +285,8 @@ static __global__ __launch_bounds__(256) void k_mx4_move(Mx4Rows R, uint64_t dst
 }
 
 // ---------------------------------------------------------------------------------------------------------------- queries
-// the query block: q_tiles operand tiles, then per query {norm fp32}, {|q|^2 fp64}
+// The query block: operand tiles, then per query {norm fp32}, {|q|^2 fp64}.  A workgroup rounds one tile of 32, as k_mx4_write does its
+// vectors, its waves the k-steps in turn: latency (1 x 128 2.4 us, 64 x 768 6.5, 256 x 1024 5.9).
 struct Mx4Queries {
     const char *x;
     size_t stride;
