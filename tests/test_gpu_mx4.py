@@ -506,3 +506,32 @@ def test_topk_of_very_small_tables(nq, n, dim, k, metric):
     q[-1] *= 2.0 ** 90
     check_topk(x, q, k, metric, 6)
     check_topk(x, q, k, metric, 4)
+
+
+# ---- many short rows read at once -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [1, 2, 7, 8, 9, 16, 17])
+@pytest.mark.parametrize("m", [2, 33, 700, 5000])
+def test_many_short_rows_come_back(m, dim):
+    x = vectors(m, dim, m + dim)
+    want = ref.micro(x.double().numpy(), 4)
+    table = store_of(x)
+    slots = torch.randint(-1, m, (m,), generator=torch.Generator().manual_seed(dim))
+    by_slots = np.where(slots.numpy()[:, None] < 0, 0.0, want[slots.numpy().clip(min=0)])
+    for dtype in DTYPES:
+        def rounded(v):
+            return torch.from_numpy(np.ascontiguousarray(v)).to(dtype).double().numpy()
+        same(mx4.read(table, dim, n=m, dtype=dtype), rounded(want))
+        same(mx4.read(table, dim, slots.to(DEV), dtype=dtype), rounded(by_slots))
+        same(mx4.read(table, dim, slots.int().to(DEV), dtype=dtype), rounded(by_slots))
+
+
+def test_reading_short_rows_writes_nothing_beside_them():
+    """rows a stride apart, the elements between them and behind the last one as they were"""
+    m, dim, stride = 1000, 5, 11
+    x = vectors(m, dim, 1)
+    table, out = store_of(x), torch.full((m + 3, stride), -7.0, device=DEV)
+    rc = mx4._load().vsgpu_mx4_read(0, torch.cuda.current_stream().cuda_stream, table.data_ptr(), m, dim, None, 0, 3, m - 3, out.data_ptr(),
+                                    mx4._TYPES[torch.float32], stride * 4)
+    assert rc == 0
+    same(out[:m - 3, :dim], ref.micro(x.double().numpy(), 4)[3:])
+    assert (out[:m - 3, dim:] == -7).all() and (out[m - 3:] == -7).all()

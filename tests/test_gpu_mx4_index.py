@@ -201,3 +201,16 @@ def test_refusals():
     ix.add_vectors(raw, np.arange(3))
     with pytest.raises(RuntimeError):
         ix.add_vectors(raw, np.arange(3))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dim", [1, 8, 9])
+def test_stored_rows_of_short_vectors(dim, kind):
+    n = 1000
+    raw, x = vectors(n, dim, 15, kind)
+    ix = make(dim, ref.L2, kind)
+    ix.add_vectors(raw, np.arange(n))
+    values = ref.micro(x, 4).astype(np.float32)
+    np.testing.assert_array_equal(ix.stored_rows(0, n), values)
+    np.testing.assert_array_equal(ix.stored_rows(3, 700), values[3:703])
+    np.testing.assert_array_equal(ix.get_vector(17), values[17:18])

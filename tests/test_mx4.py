@@ -1,5 +1,7 @@
 """CPU: the refusals of the MXFP4 entries (include/vsgpu.h), and the float64 definition the GPU tests compare with."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -10,6 +12,7 @@ from vectorsimilarity_amd import _capi, mx4
 
 ARG, UNSUPPORTED = 3, 4
 F32 = _capi.VecSimType_FLOAT32
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_panel_bytes():
@@ -90,3 +93,28 @@ def test_the_definition():
                 assert np.isin(got / s, values).all()
     np.testing.assert_array_equal(ref.micro(np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 4]]), 4), [[0, 1, 1, 2, 2, 4, 4, 4]])
     assert np.isnan(ref.micro(np.array([[1.0] * 31 + [np.inf] + [1.0]]), 6)).tolist() == [[True] * 32 + [False]]
+
+
+# ---- reading rows: how the kernel divides its work (csrc/mx4_read_plan.h) ---------------------------------------------------------
+@pytest.fixture(scope="module")
+def read_plan():
+    helpers = os.path.join(ROOT, "tests", "helpers")
+    csrc = os.path.join(ROOT, "vectorsimilarity_amd", "csrc")
+    so, src = os.path.join(helpers, "libmx4_read_plan.so"), os.path.join(helpers, "mx4_read_plan.cpp")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I", csrc, "-o", so, src], check=True)
+    L = C.CDLL(so)
+    L.wrong_rows.restype = C.c_long
+    L.wrong_rows.argtypes = [C.c_uint32, C.c_uint32]
+    L.pieces.restype = L.rows.restype = C.c_uint32
+    L.pieces.argtypes = [C.c_uint32]
+    L.rows.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32]
+    return L
+
+
+def test_read_takes_every_piece_of_every_row_once(read_plan):
+    """a piece of eight elements goes to row t / pieces of a row: for every row length that a store may have"""
+    assert [read_plan.pieces(d) for d in (1, 8, 9, 16, 17, 65536)] == [1, 1, 2, 2, 3, 8192]
+    for per_row in range(1, 8193):
+        most = max(read_plan.rows(m, per_row, cus) for cus in (1, 256, 304) for m in (1, 2, 255, 256, 257, 100000, 2 ** 31 - 1))
+        assert 1 <= most and most * per_row < 1 << 16
+        assert read_plan.wrong_rows(per_row, 1 << 16) == 0, per_row

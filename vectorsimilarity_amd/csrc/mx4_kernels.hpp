@@ -2,6 +2,7 @@
 // mx4_scan_kernels.hpp the passes over the table).
 #pragma once
 #include "mx4_common.hpp"
+#include "mx4_read_plan.h"
 
 #include <type_traits>
 
@@ -220,12 +221,12 @@ __device__ __forceinline__ float mx4_code_value(uint32_t c) {   // c: 4 bits
 // A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  Rows in
 // any order cost the sectors around their 16-byte pieces, four times their bytes: 700K of 1M x 1024 to bf16 708 us (1.43 GB written,
 // 1.7 GB read: 4.4 TB/s), 1M x 768 524 us; 100 rows of 128 2.7 us.  A
-// workgroup takes `rows` whole rows (rows * per_row < 2^16: the division is one multiplication, by ceil(2^32 / per_row)).
-template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t recip) {
+// workgroup takes `rows` whole rows (mx4_read_plan.h).
+template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t reciprocal) {
     const uint64_t i0 = (uint64_t)blockIdx.x * rows;
     const uint32_t work = (uint32_t)min((uint64_t)rows, R.m - i0) * per_row;
     for (uint32_t t = threadIdx.x; t < work; t += 256) {
-        const uint32_t r = __umulhi(t, recip), piece = t - r * per_row, e = piece * 8;
+        const uint32_t r = mx4_quotient(t, reciprocal), piece = t - r * per_row, e = piece * 8;
         const uint64_t i = i0 + r;
         const int64_t s = mx4_slot(R.slots, R.slots64, i, R.first);
         float v[8];

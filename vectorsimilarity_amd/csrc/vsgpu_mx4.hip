@@ -232,13 +232,10 @@ int mx4_launch_write(hipStream_t s, const Mx4Write &W0, int type) {
 }
 int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus) {
     if (R.m == 0) return VSGPU_OK;
-    const uint32_t per_row = (R.rows.dim + 7) / 8, recip = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
-    // about 1024 threads' work a workgroup, fewer rows when there are not enough of them to fill the chip
-    uint64_t rows = std::max<uint64_t>(1, 1024 / per_row);
-    rows = std::max<uint64_t>(std::min<uint64_t>(rows, R.m / ((uint64_t)cus * 8)), std::max<uint64_t>(1, std::min<uint64_t>(256 / per_row, R.m)));
+    const uint32_t per_row = mx4_read_pieces(R.rows.dim), rows = mx4_read_rows(R.m, per_row, (uint32_t)cus), reciprocal = mx4_reciprocal(per_row);
     const dim3 g((unsigned)((R.m + rows - 1) / rows)), b(256);
 #define MX4_CASE(T)                                                                                                           \
-    hipLaunchKernelGGL((k_mx4_read<T>), g, b, 0, s, R, (uint32_t)rows, per_row, recip);
+    hipLaunchKernelGGL((k_mx4_read<T>), g, b, 0, s, R, rows, per_row, reciprocal);
     if (type == VSGPU_F32) { MX4_CASE(MX4_F32) }
     else if (type == VSGPU_F16) { MX4_CASE(MX4_F16) }
     else { MX4_CASE(MX4_BF16) }
