@@ -131,7 +131,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_probe_dma(const char *rows, unsi
         plds = lds_base + fslot * UNIT + (unsigned)(wave * IPW * 1040);
     };
     auto piece = [&]() {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory", "m0");
         pbase += 1024;
         plds += 1040;
     };
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, 1) void k_probe_dma64(const char *rows, unsign
         plds = lds_base + fslot * UNIT + (unsigned)(wave * IPW * 1040);
     };
     auto piece = [&]() {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory", "m0");
         pbase += 1024;
         plds += 1040;
     };
@@ -363,7 +363,7 @@ template <int NW> __global__ __launch_bounds__(NW * 64, 2) void k_probe_share(co
         plds = lds_base + fslot * UNIT + (unsigned)(wave * IPW * 1040);
     };
     auto piece = [&]() {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(pbase), "s"(plds) : "memory", "m0");
         pbase += 1024;
         plds += 1040;
     };

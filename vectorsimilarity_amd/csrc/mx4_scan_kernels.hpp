@@ -126,7 +126,7 @@ constexpr int mx4_ring_bytes(int nb) { return mx4_ring_stages(nb) * mx4_ring_pie
 constexpr int MX4_RING_WAVES = 4;
 // 16 bytes a lane from base + offset to LDS (lds: the wave's first byte), without passing through registers
 __device__ __forceinline__ void mx4_to_lds(uint32_t lds, uint32_t offset, uint64_t base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void mx4_wait_loads() {   // until at most N of the wave's memory operations are under way
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -135,7 +135,7 @@ template <int N> __device__ __forceinline__ void mx4_wait_loads() {   // until a
 // stands before and behind them may be mixed.
 template <int N> __device__ __forceinline__ void mx4_to_lds_first(int wave, uint32_t lds, uint32_t offset, uint64_t base) {
     asm volatile("s_cmp_lt_i32 %0, %1\n\ts_cbranch_scc0 .Lmx4_none_%=\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %4\n.Lmx4_none_%=:"
-                 ::"s"(wave), "n"(N), "s"(lds), "v"(offset), "s"(base) : "memory", "scc");
+                 ::"s"(wave), "n"(N), "s"(lds), "v"(offset), "s"(base) : "memory", "scc", "m0");
 }
 template <int FIRST, int MANY, int FEW> __device__ __forceinline__ void mx4_wait_loads_first(int wave) {   // at most MANY or FEW
     asm volatile("s_cmp_lt_i32 %0, %1\n\ts_cbranch_scc0 .Lmx4_few_%=\n\ts_waitcnt vmcnt(%2)\n\ts_branch .Lmx4_there_%=\n.Lmx4_few_%=:\n\ts_waitcnt vmcnt(%3)\n.Lmx4_there_%=:"
