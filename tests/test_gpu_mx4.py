@@ -535,3 +535,38 @@ def test_reading_short_rows_writes_nothing_beside_them():
     assert rc == 0
     same(out[:m - 3, :dim], ref.micro(x.double().numpy(), 4)[3:])
     assert (out[:m - 3, dim:] == -7).all() and (out[m - 3:] == -7).all()
+
+
+# ---- matrix-core dots at their worst ----------------------------------------------------------------------------------------------
+# An instruction leaves a block of 32 products out when its scales' power of two is 2^32 below the sum so far: up to 32 x 7.5 x 6 x 2^-32 of
+# it (4 bits: 32 x 6 x 6), for each of its two blocks.
+def left_out_blocks(dim, bits, sign, first, q_first):
+    """a query and a row: a product of 2^40 in front, then blocks of the largest codes that are all left out beside it"""
+    q, x = np.zeros(dim), np.zeros(dim)
+    q[0] = x[0] = 2.0 ** 20
+    q[32:64], x[32:32 + len(first)] = q_first, first
+    q[64:], x[64:] = (7.5 if bits == 6 else 6) * 16, sign * 6 * 16
+    return q, x
+
+
+@pytest.mark.parametrize("dim,bits,lead", [(1024, 6, (1, .5)), (4096, 6, (4, 1)), (16384, 6, (4, 1)), (65536, 6, (4, 1)), (65536, 4, (6, 2, .5))])
+def test_topk_when_dots_are_off_by_their_most(dim, bits, lead):
+    """the nearest row's dot comes back too small, another's too large, by more than lies between them"""
+    n = 6200   # (more rows than are scored exactly or bounded one by one)
+    # the other row's lead: more than twice the errors' difference allows for, less than the errors
+    first = np.array(lead) * {1024: 2.0 ** 11, 4096: 2.0 ** 12, 16384: 2.0 ** 14, 65536: 2.0 ** 16 if bits == 6 else 2.0 ** 15}[dim]
+    q, near = left_out_blocks(dim, bits, 1, (), 4096.0)
+    _, other = left_out_blocks(dim, bits, -1, first, 4096.0)
+    assert near @ q > other @ q
+    rows = torch.from_numpy(np.stack([other, near])).float()
+    same(rows, ref.micro(rows.double().numpy(), 4))
+    assert np.array_equal(ref.micro(q[None], bits)[0], q)
+    table = mx4.empty(n, dim, DEV)
+    mx4.write(table, rows.to(DEV), torch.tensor([3, 5000], device=DEV))
+    query = torch.from_numpy(q[None]).float().to(DEV)
+    want = np.array([1 - near @ q, 1 - other @ q]).astype(np.float32)
+    for nq in (1, 70, 130):
+        for k in (1, 2):
+            ids, best = mx4.topk(table, n, query.expand(nq, -1), k, ref.IP, bits)
+            assert (ids.cpu().numpy() == np.array([5000, 3])[:k]).all()
+            assert (best.cpu().numpy() == want[:k]).all()

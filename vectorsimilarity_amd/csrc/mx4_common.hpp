@@ -6,8 +6,8 @@
 //   dot(q, x) = sum_blocks 2^(Eq + Ex) sum_j q_j x_j      IP 1 - dot    L2 |q|^2 + |x|^2 - 2 dot    Cosine 1 - dot / (|q| |x|)
 // (|.| of the rounded vectors).  A block's inner sum is a multiple of 1/16 below 2^11, so it is exact in fp32, whatever the order.
 // E2M3 and not E4M3 for the finer queries: at a block's own scale both keep four digits of its larger elements, the matrix
-// instruction takes six-bit operands at the four-bit rate, and it adds their products without loss (measured over random blocks:
-// within 2^-23.4 of sum|q x|, where E4M3 products came back up to 3e-4 of the largest product off).
+// instruction takes six-bit operands at the four-bit rate, and it adds up a block of their products exactly (what it does with blocks
+// far apart: mx4_slack), where E4M3 products came back up to 3e-4 of the largest product off.
 //
 // The layout.  32 rows form a panel, laid out as v_mfma_scale_f32_32x32x64_f8f6f4 takes its operand, so that a wave's load of one
 // k-step (64 elements of 32 rows) is one contiguous KiB straight into registers, without a pass through LDS:
@@ -62,10 +62,12 @@ struct Mx4Rows {
 };
 
 // ---------------------------------------------------------------------------------------------------------------- scan
-// How far a matrix-core dot may be from the exact one, over |q| |x|: each of the ks instructions adds its 64 products to the sum
-// so far within 2^-22 of what it adds up (measured 2^-23.4); eight more of the same for the rounded norms and the comparison's own
-// arithmetic, and twice all of it.
-__host__ __device__ inline float mx4_slack(uint32_t ks) { return (float)(ks + 8) * 4.76837158203125e-7f; }
+// How far a matrix-core dot may be from the exact one, over |q| |x|.  An instruction adds two blocks, each the exact sum of its 32
+// products, to the sum so far and rounds once (2^-24), but leaves a block out when its scales' power of two is 2^32 or more below the
+// largest of what it adds: up to 32 x 7.5 x 6 x 2^-32 = 2^-21.51 of that, for each of the two (the largest error of 6 x 10^7 random and
+// extreme instructions: 2^-20.508).  Sums whose every step loses that, in one direction, exist, so a step counts with 2^-20, a third
+// more than both; eight more steps for the rounded norms, the comparison's own arithmetic and subnormal dots.
+__host__ __device__ inline float mx4_slack(uint32_t ks) { return (float)(ks + 8) * 9.5367431640625e-7f; }
 constexpr float MX4_EPS = 1.9073486328125e-6f;    // 2^-19, of |q|^2 + |x|^2 (L2): the same for sums of squares
 constexpr float MX4_STEP = 9.5367431640625e-7f;   // 2^-20: what rounding a score to fp32 may move it, and more
 constexpr float MX4_TINY = 1e-36f;                // L2 scores below it: fp32 has no digits left to rank them by
