@@ -214,3 +214,18 @@ def test_stored_rows_of_short_vectors(dim, kind):
     np.testing.assert_array_equal(ix.stored_rows(0, n), values)
     np.testing.assert_array_equal(ix.stored_rows(3, 700), values[3:703])
     np.testing.assert_array_equal(ix.get_vector(17), values[17:18])
+
+
+@pytest.mark.parametrize("n,dim,nq,kernel", [(300, 100, 1, "k_mx4_finish"), (3000, 100, 70, "k_mx4_scan"), (9000, 100, 5, "k_mx4_scan"),
+                                             (9000, 640, 70, "k_mx4_ring"), (9000, 300, 130, "k_mx4_ring"), (9000, 64, 130, "k_mx4_scan")])
+def test_statistics_name_the_kernel_that_passed_over_the_rows(n, dim, nq, kernel):
+    raw, _ = vectors(n, dim, 16)
+    q, _ = vectors(nq, dim, 17)
+    ix = make(dim, ref.L2)
+    ix.add_vectors(raw, np.arange(n))
+    ix.knn_query(q, 10)
+    ix.reset_stats()
+    ix.knn_query(q, 10)
+    st = ix.stats()
+    assert (st["scan_kernel"], st["scan_launches"], st["scan_rows"]) == (kernel, 1, n)
+    assert st["scan_ms"] > 0

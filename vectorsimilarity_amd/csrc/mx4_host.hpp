@@ -38,9 +38,14 @@ int mx4_launch_write(hipStream_t s, const Mx4Write &W, int type);
 int mx4_launch_read(hipStream_t s, const Mx4Read &R, int type, int cus);
 int mx4_launch_queries(hipStream_t s, const void *x, int type, size_t stride, size_t nq, const Mx4Rows &R, int bits, uint32_t tiles, char *block,
                        float *norm, double *sq, uint32_t *zero, size_t zero_words);
+// the one pass of a top-k over every row, for the statistics: marked by these events, made by this kernel
+struct Mx4Pass {
+    hipEvent_t begin = nullptr, end = nullptr;
+    const char *kernel = "";
+};
 size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits);
 int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
-                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, hipEvent_t scan_begin = nullptr, hipEvent_t scan_end = nullptr);
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, Mx4Pass *pass = nullptr);
 }  // namespace vsg
 
 // a vsgpu_table of MXFP4 rows; host pointers, every call ends with its stream drained

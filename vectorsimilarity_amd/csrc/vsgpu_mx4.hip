@@ -256,7 +256,7 @@ size_t mx4_topk_bytes(size_t n, size_t dim, size_t nq, size_t k, int bits) {
 
 // queries of one batch -> ids / scores [nq][k] on the device
 int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *queries, int type, size_t nq, size_t qstride, size_t k, int metric,
-                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, hipEvent_t scan_begin, hipEvent_t scan_end) {
+                   int bits, int64_t *ids, float *scores, void *ws, size_t ws_bytes, Mx4Pass *pass) {
     const int cus = compute_units(device);
     const Plan p = plan_topk(R.n, R.dim, nq, k, bits, cus);
     Layout L;
@@ -283,7 +283,11 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
     P.segments = p.segments;
     P.segment = p.segment;
     P.slack = mx4_slack(R.ks);
-    if (p.dense && scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
+    // the pass over every row: the filter, the probe of a small table, the exact scores of a very small one
+    if (pass) pass->kernel = p.all ? "k_mx4_finish" : (!p.dense && p.shape.ring ? "k_mx4_ring" : "k_mx4_scan");
+    const auto mark = [&](hipEvent_t event) { return event ? hipEventRecord(event, s) : hipSuccess; };
+    const hipEvent_t begin = pass ? pass->begin : nullptr, end = pass ? pass->end : nullptr;
+    if (p.dense) HIPCHK(mark(begin));
     if (!p.all) rc = launch_scan(s, p.by_row ? MX4_PROBE_ROWS : MX4_PROBE, P, p, bits);
     if (rc) return rc;
     if (!p.dense) {
@@ -291,11 +295,11 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
         hipLaunchKernelGGL(k_mx4_threshold, dim3((unsigned)nq), dim3(1024), 0, s, T);
         HIPCHK(hipGetLastError());
         P.n_take = p.panels;
-        if (scan_begin) HIPCHK(hipEventRecord(scan_begin, s));
+        HIPCHK(mark(begin));
         rc = launch_scan(s, MX4_FILTER, P, p, bits);
         if (rc) return rc;
     }
-    if (scan_end) HIPCHK(hipEventRecord(scan_end, s));
+    if (!p.all) HIPCHK(mark(end));
     Mx4Select S{};
     S.E = Mx4Exact{R, b.q.tiles, p.qtile_bytes, (uint32_t)metric, b.q.sq};
     S.nq = (uint32_t)nq;
@@ -332,6 +336,7 @@ int mx4_topk_batch(hipStream_t s, int device, const Mx4Rows &R, const void *quer
         hipLaunchKernelGGL((k_mx4_again<4>), ag, dim3(512), 0, s, S);
     }
     HIPCHK(hipGetLastError());
+    if (p.all) HIPCHK(mark(end));
     return VSGPU_OK;
 }
 
@@ -487,16 +492,16 @@ int mx4_table_topk(vsgpu_table *t, const void *queries, size_t nq, size_t qstrid
         rc = upload_queries(t, static_cast<const char *>(queries) + q0 * qstride, m, qstride);
         if (rc) return rc;
         chain.before_scan();
-        const bool timed = (c->opt_events & 1) != 0;
+        Mx4Pass pass;
+        if (c->opt_events & 1) pass.begin = c->ev_a, pass.end = c->ev_b;
         rc = mx4_topk_batch(c->stream, c->device, R, c->qfrag.p, t->mx4_in, m, row, take, t->metric, t->mx4_bits, static_cast<int64_t *>(c->sel.p),
-                            reinterpret_cast<float *>(static_cast<char *>(c->sel.p) + ids_bytes), c->dense.p, c->dense.cap, timed ? c->ev_a : nullptr,
-                            timed ? c->ev_b : nullptr);
+                            reinterpret_cast<float *>(static_cast<char *>(c->sel.p) + ids_bytes), c->dense.p, c->dense.cap, &pass);
         if (rc) return rc;
         chain.submitted();
         HIPCHK(hipMemcpyAsync(c->pinned, c->sel.p, out_bytes, hipMemcpyDeviceToHost, c->stream));
         HIPCHK(hipStreamSynchronize(c->stream));
         if (c->poll && c->poll(c->poll_user)) return VSGPU_ERR_TIMEOUT;
-        account_scan(c, t, n, 1, "k_mx4_scan");
+        account_scan(c, t, n, 1, pass.kernel);
         const int64_t *rid = static_cast<const int64_t *>(c->pinned);
         const float *rsc = reinterpret_cast<const float *>(static_cast<const char *>(c->pinned) + ids_bytes);
         std::vector<std::pair<uint32_t, double>> hits;
