@@ -213,11 +213,6 @@ struct Mx4Read {
 __device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
     return byte == 255 ? __uint_as_float(0x7FC00000u) : (byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23));
 }
-__device__ __forceinline__ float mx4_code_value(uint32_t c) {   // c: 4 bits
-    const uint32_t m = c & 7u;
-    const float v = m < 2 ? 0.5f * (float)m : (float)((2u | (m & 1u)) << ((m >> 1) - 1)) * 0.5f;
-    return c & 8u ? -v : v;
-}
 // A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  Rows in
 // any order cost the sectors around their 16-byte pieces, four times their bytes: 700K of 1M x 1024 to bf16 708 us (1.43 GB written,
 // 1.7 GB read: 4.4 TB/s), 1M x 768 524 us; 100 rows of 128 2.7 us.  A
