@@ -570,3 +570,44 @@ def test_topk_when_dots_are_off_by_their_most(dim, bits, lead):
             ids, best = mx4.topk(table, n, query.expand(nq, -1), k, ref.IP, bits)
             assert (ids.cpu().numpy() == np.array([5000, 3])[:k]).all()
             assert (best.cpu().numpy() == want[:k]).all()
+
+
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("dim", [64, 1000, 4096])
+def test_scores_of_blocks_far_apart(dim, bits):
+    """steps of which a dot keeps nothing, and others: within 2^-20 of |q| |x| each"""
+    g = torch.Generator().manual_seed(dim + bits)
+    spread = torch.exp2(torch.randint(-20, 1, (300, (dim + 31) // 32), generator=g).float()).repeat_interleave(32, 1)[:, :dim]
+    x, q = vectors(300, dim, 1).abs() * spread, vectors(40, dim, 2).abs() * spread[:40]
+    far = left_out_blocks(dim, bits, 1, (), 0.0)
+    q[0], x[0] = torch.from_numpy(far[0]).float() * 2.0 ** -20, torch.from_numpy(far[1]).float() * 2.0 ** -20
+    values, q64 = ref.micro(x.double().numpy(), 4), ref.micro(q.double().numpy(), bits)
+    size = np.sqrt((q64 ** 2).sum(1))[:, None] * np.sqrt((values ** 2).sum(1))[None]
+    got = mx4.scores(store_of(x), 300, q.to(DEV), ref.IP, bits).double().cpu().numpy()
+    # 1 - dot is rounded once more
+    assert (np.abs(got - (1 - q64 @ values.T)) <= (dim + 63) // 64 * 2.0 ** -20 * size + 2.0 ** -24 * (1 + size)).all()
+
+
+@pytest.mark.parametrize("dim", [64, 1000])
+@pytest.mark.parametrize("power", [-25, -40, -50, -58])
+def test_cosine_scores_of_short_vectors(power, dim):
+    """on both sides, down to a product of norms of about 2^-116"""
+    x, q = vectors(200, dim, 3) * 2.0 ** power, vectors(20, dim, 4) * 2.0 ** power
+    values = ref.micro(x.double().numpy(), 4)
+    for bits in (4, 6):
+        got = mx4.scores(store_of(x), 200, q.to(DEV), ref.COSINE, bits).double().cpu().numpy()
+        want = ref.scores(q.double().numpy(), values, ref.COSINE, bits)
+        assert (np.abs(got - want) <= ref.bound(q.double().numpy(), values, ref.COSINE, bits)).all()
+
+
+@pytest.mark.parametrize("nq", [3, 70, 150])
+def test_topk_cosine_of_norms_beside_the_shortest_bounded_one(nq):
+    """rows and queries between 2e-19 and 5e-18: on both sides of 1e-18, below which no bound is made"""
+    n, dim = 9000, 64 if nq == 3 else 576
+    g = torch.Generator().manual_seed(nq)
+    x, q = vectors(n, dim, 5), vectors(nq, dim, 6)
+    x *= 1e-18 * torch.exp(3.2 * torch.rand(n, 1, generator=g) - 1.6) / x.norm(dim=1, keepdim=True)
+    q *= 1e-18 * torch.exp(3.2 * torch.rand(nq, 1, generator=g) - 1.6) / q.norm(dim=1, keepdim=True)
+    for bits in (4, 6):
+        check_topk(x, q, 10, ref.COSINE, bits)
+        check_topk(x, q, 200, ref.COSINE, bits)
