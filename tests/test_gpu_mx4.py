@@ -611,3 +611,13 @@ def test_topk_cosine_of_norms_beside_the_shortest_bounded_one(nq):
     for bits in (4, 6):
         check_topk(x, q, 10, ref.COSINE, bits)
         check_topk(x, q, 200, ref.COSINE, bits)
+
+
+@pytest.mark.parametrize("nq,dim", [(3, 64), (70, 300), (200, 1024), (40, 5000)])
+def test_l2_scores_of_zero_rows_are_the_squares_of_the_queries(nq, dim):
+    """|q|^2 comes from 64 bits, rounded once"""
+    q = vectors(nq, dim, 7)
+    for bits in (4, 6):
+        got = mx4.scores(mx4.empty(40, dim, DEV), 40, q.to(DEV), ref.L2, bits).cpu().numpy()
+        want = (ref.micro(q.double().numpy(), bits) ** 2).sum(1).astype(np.float32)
+        assert (got == want[:, None]).all()

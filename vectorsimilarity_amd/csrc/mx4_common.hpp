@@ -87,6 +87,7 @@ struct Mx4Scan {
     uint32_t nq, metric;
     uint32_t groups;              // waves that share a panel, each with its own query tiles
     const float *qnorm;
+    const double *qsq;            // DENSE: |q|^2
     uint64_t n_take;              // panels: all of them, or for a probe number i is (i * every) >> 24
     uint64_t every;
     float *minima;                // PROBE: [nq][2 n_take] upper bounds of 16 rows each; PROBE_ROWS: [nq][n] of each row

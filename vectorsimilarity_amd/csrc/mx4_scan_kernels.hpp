@@ -163,7 +163,7 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
     const char *tiles = P.tiles + (size_t)(q0 / 32) * P.qtile_bytes;
     const char *lds = SRC == MX4_SHARED ? shared : tiles;
     const uint32_t block_q = groups * QT * 32;
-    float *yn_b = reinterpret_cast<float *>(shared + (SRC == MX4_SHARED ? QT * P.qtile_bytes : 0));   // |q|, 1 / |q| of the workgroup's queries
+    float *yn_b = reinterpret_cast<float *>(shared + (SRC == MX4_SHARED ? QT * P.qtile_bytes : 0));   // |q|, 1 / |q| of the workgroup's queries (L2 scores: |q|, |q|^2)
     uint32_t *taken = reinterpret_cast<uint32_t *>(yn_b);   // FILTER: candidates of each of them so far
     if constexpr (SRC == MX4_SHARED) {
         const mx4_u4 *src = reinterpret_cast<const mx4_u4 *>(tiles);
@@ -176,7 +176,7 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
         } else {
             const float y = P.qnorm[block_q0 + i];   // (padded to whole tiles)
             yn_b[i] = y;
-            yn_b[block_q + i] = 1.f / y;
+            yn_b[block_q + i] = MODE == MX4_DENSE && P.metric == MX4_L2 ? (float)P.qsq[block_q0 + i] : 1.f / y;
         }
     }
     __syncthreads();
@@ -296,7 +296,7 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
                     for (int j = 0; j < 4; j++) {
                         const float d = acc[q][4 * i + j], y = y4[j];
                         float s;
-                        if constexpr (M == MX4_L2) s = __fmaf_rn(-2.f, d, __fmaf_rn(y, y, c0));
+                        if constexpr (M == MX4_L2) s = __fmaf_rn(-2.f, d, r4[j] + c0);
                         else if constexpr (M == MX4_IP) s = 1.f - d;
                         else if constexpr (decltype(divide)::value) s = 1.f - d / xrow / y;
                         else s = 1.f - d * rx * r4[j];

@@ -357,6 +357,7 @@ int mx4_scores_batch(hipStream_t s, int device, const Mx4Rows &R, const void *qu
     P.nq = (uint32_t)nq;
     P.metric = (uint32_t)metric;
     P.qnorm = b.norm;
+    P.qsq = b.sq;
     P.n_take = (R.n + 31) / 32;
     P.out = out;
     P.out_stride = out_stride;
