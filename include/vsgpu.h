@@ -160,9 +160,11 @@ int vsgpu_mx4_write(int device, void *stream, void *table, size_t capacity, size
  * hold them exactly).  A negative slot reads zeros, one that is not below capacity NaN. */
 int vsgpu_mx4_read(int device, void *stream, const void *table, size_t capacity, size_t dim, const void *slots, int slot_bytes, size_t first, size_t m,
                    void *out, int type, size_t stride);
-/* fp32 scores of every query against rows [0, n): scores[q * scores_stride + row].  Dots are accumulated in fp32 and norms are kept
- * in fp32, so a Cosine score of vectors shorter than 2^-100 has few digits, and one of vectors longer than 2^62 may be infinite or
- * NaN where a sum leaves fp32 (vsgpu_mx4_topk has neither limit).  Workspace: 256-byte aligned device memory. */
+/* fp32 scores of every query against rows [0, n): scores[q * scores_stride + row].  Dots are accumulated in fp32 on the matrix cores: a
+ * step of 64 elements that lie far below the sum so far may be off by 2^-20 |q| |x| (random vectors: a whole dot within 2^-22 of it);
+ * |x| is an fp32 number.  So Cosine scores keep their digits while |q| |x| is above 2^-120 (below, dots leave fp32's normal numbers,
+ * and at 2^-150 every one is 0 and its score 1), and scores of vectors longer than 2^62 may be infinite or NaN where a sum leaves
+ * fp32 (vsgpu_mx4_topk has none of these limits).  Workspace: 256-byte aligned device memory. */
 size_t vsgpu_mx4_scores_workspace(size_t dim, size_t nq, int bits);   /* 0: bad arguments */
 int vsgpu_mx4_scores(int device, void *stream, const void *table, size_t n, size_t dim, const void *queries, int type, size_t nq, size_t qstride,
                      int metric, int bits, float *scores, size_t scores_stride, void *workspace, size_t workspace_bytes);
@@ -174,7 +176,8 @@ int vsgpu_mx4_topk(int device, void *stream, const void *table, size_t n, size_t
                    int metric, int bits, int64_t *ids, float *scores, void *workspace, size_t workspace_bytes);
 /* The same rows as a table of the calls above: host vectors of `type` (VSGPU_F32, _F16 or _BF16) go in through _append and _write and
  * are rounded on the device, queries are host vectors of that type.  _read and _read_range return the rows' VALUES as dim fp32.
- * _topk, _range, _scores, _scores_of, _move, _truncate and views work as on other tables, with scores as in vsgpu_mx4_topk;
+ * _topk, _range, _scores, _scores_of, _move, _truncate and views work as on other tables, with scores as in vsgpu_mx4_topk (vsgpu_set_poll's
+ * function is asked once a batch of 256 queries, behind its kernels);
  * device-resident score vectors, synthetic rows and HNSW graphs do not exist for it. */
 vsgpu_table *vsgpu_table_create_mx4(vsgpu_ctx *ctx, int type, int metric, size_t dim, int query_bits);
 

@@ -121,7 +121,7 @@ __device__ __forceinline__ int64_t mx4_slot(const void *slots, int is64, uint64_
     return is64 ? static_cast<const int64_t *>(slots)[i] : (int64_t)static_cast<const int32_t *>(slots)[i];
 }
 // Which vector a slot gets when several name it: the last.  Two passes over the norms: cleared, then the largest 2^31 | i (4097 slots
-// 2.7 us each, 1M 5.2; up to 4096 vectors k_mx4_write looks for later ones with its slots itself).
+// 2.6 us each, 1M in order 5.0, 1M in any order 20 and 41; up to 4096 vectors k_mx4_write looks for later ones with its slots itself).
 static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) {
     const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= W.m) return;
@@ -132,8 +132,9 @@ static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) 
     else atomicMax(norm, 0x80000000u | (uint32_t)i);
 }
 // One workgroup takes 32 vectors, its waves (up to 16) the k-steps in turn; a lane rounds one block (half, row) by itself, so neither
-// the maximum nor the codes cross lanes.  Bound by memory: 1M x 768 bf16 into rows in any order 405 us, 1.95 GB at 4.8 TB/s (a copy of
-// the card's: 4.76), although a row's codes are 16-byte pieces 512 bytes apart; 4097 x 1000 fp16 10 us.
+// the maximum nor the codes cross lanes.  Bound by memory where slots follow each other: 1M x 768 bf16 into the first rows 350-375 us
+// (1.95 GB at 5.2 TB/s or more; a copy of the card's: 4.76), by slots in order 405.  In any order 1160: a row's codes are 16-byte pieces
+// 512 bytes apart, and each writes 64 bytes (1.0 GB for 0.41 by the counters).  4097 x 1000 fp16 9.7 us.
 template <int T> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
     __shared__ double part[16][64];
     __shared__ int64_t slot_s[32];
@@ -214,9 +215,10 @@ __device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
     return byte == 255 ? __uint_as_float(0x7FC00000u) : (byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23));
 }
 // A thread turns 8 codes (one dword) into 8 values; consecutive threads run along a row, so a wave's stores are contiguous.  Rows in
-// any order cost the sectors around their 16-byte pieces, four times their bytes: 700K of 1M x 1024 to bf16 708 us (1.43 GB written,
-// 1.7 GB read: 4.4 TB/s), 1M x 768 524 us; 100 rows of 128 2.7 us.  A
-// workgroup takes `rows` whole rows (mx4_read_plan.h).
+// any order cost the 64 bytes around each of their 16-byte pieces: 700K of 1M x 1024 to bf16 710 us (1.43 GB written, 1.79 GB read:
+// 4.5 TB/s), 1M x 768 765.  In order 700K x 1024 take 370 us and 1M x 768 520: ten rows of 768 are a workgroup's, which share panels
+// with rows of workgroups on other XCDs (0.70 GB read for 0.41).  100 rows of 128 2.6 us.  A workgroup takes `rows` whole rows
+// (mx4_read_plan.h).
 template <int T> static __global__ __launch_bounds__(256) void k_mx4_read(Mx4Read R, uint32_t rows, uint32_t per_row, uint32_t reciprocal) {
     const uint64_t i0 = (uint64_t)blockIdx.x * rows;
     const uint32_t work = (uint32_t)min((uint64_t)rows, R.m - i0) * per_row;

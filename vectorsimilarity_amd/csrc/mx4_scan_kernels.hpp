@@ -149,7 +149,7 @@ template <int FIRST, int MANY, int FEW> __device__ __forceinline__ void mx4_wait
 //                             panels through the CU's cache; LDS would be read 1.5 KiB a tile and step against 32 cycles of matrix
 //                             work on each of four SIMDs.  Probe and filter: LDS too, or k_mx4_ring
 //   rows beyond the LDS       in global memory, through the caches
-// 64 queries x 4M x 768, top-10: filter 250 us, 1.65 GB at 6.6 TB/s.  Scores: 256 x 1M x 1024 335-350 us, 1.57 GB at 4.6 TB/s, two thirds
+// 64 queries x 4M x 768, top-10: filter 255 us, 1.65 GB at 6.5 TB/s.  Scores: 256 x 1M x 1024 335-350 us, 1.57 GB at 4.6 TB/s, two thirds
 // of it stores; 33 x 200K x 1000 (4 bits) 37 us, 136 MB; 1 x 100K x 128 5.2 us, where a launch is most of it.
 template <int BITS, int QT, int MODE, int NB, int SRC>
 static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)) void k_mx4_scan(Mx4Scan P) {
@@ -384,10 +384,10 @@ static __global__ __launch_bounds__(256, mx4_scan_waves(BITS, QT, MODE, NB, SRC)
 // The same passes for 65 to 256 queries against rows of at most 1024 elements.  Four waves, QT tiles each, take every panel together; it
 // comes through LDS, so that the memory's latency is covered by a ring of panels and not by registers, which hold the operands.  One
 // wave a SIMD: the comparisons of the panel before are made between the matrix instructions of this one, whose last chunk covers the
-// barrier and the first reads of the next. 
-// 1M x 1024, few survivors: 128 queries 105 us (5.2 TB/s: the memory), 256 queries 160 us (537 GFLOP at 3.4 PFLOP/s; the chip's clock
-// falls to 1.7 GHz under it, and with less work beside the matrix instructions hardly rises).  Each panel with survivors costs its
-// wave some 800 cycles: 256 queries, top-100: 245 us.  Eight waves of one tile each read the LDS twice as often: 207 us.
+// barrier and the first reads of the next.
+// Filter of 1M x 1024 (549 MB): 128 queries, the nearest one 140 us; 256 queries, 1 | 10 | 100 nearest 190 | 210 | 250 us (524 GFLOP at
+// 2.8 | 2.5 | 2.1 PFLOP/s): each panel with survivors costs its wave some 800 cycles.  Eight waves of one tile each read the LDS twice
+// as often (without survivors 207 us against 160).
 template <int BITS, int QT, int MODE, int NB, int M> static __global__ __launch_bounds__(256, 1) void k_mx4_ring(Mx4Scan P) {
     extern __shared__ char shared[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;

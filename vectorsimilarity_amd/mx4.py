@@ -185,8 +185,8 @@ def _query(table, n, queries, metric, query_bits):
 
 
 def scores(table, n, queries, metric, query_bits=6):
-    """fp32 scores [nq, n] of every query [nq, dim] against rows 0 .. n - 1 of the store.  Dots and norms are fp32 sums: vectors
-    longer than 2^62 may score infinite or NaN, and the Cosine of ones shorter than 2^-100 has few digits."""
+    """fp32 scores [nq, n] of every query [nq, dim] against rows 0 .. n - 1 of the store.  Dots are fp32 sums: Cosine scores have
+    few digits where |q| |x| is below 2^-120, vectors longer than 2^62 may score infinite or NaN (topk has neither limit)."""
     lib = _lib or _load()
     dim, q, kind, nq, stride = _query(table, n, queries, metric, query_bits)
     out = torch.empty((nq, n), dtype=torch.float32, device=table.device)
