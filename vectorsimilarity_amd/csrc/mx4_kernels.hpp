@@ -134,7 +134,7 @@ static __global__ __launch_bounds__(256) void k_mx4_claim(Mx4Write W, int pass) 
 // One workgroup takes 32 vectors, its waves (up to 16) the k-steps in turn; a lane rounds one block (half, row) by itself, so neither
 // the maximum nor the codes cross lanes.  Bound by memory where slots follow each other: 1M x 768 bf16 into the first rows 350-375 us
 // (1.95 GB at 5.2 TB/s or more; a copy of the card's: 4.76), by slots in order 405.  In any order 1160: a row's codes are 16-byte pieces
-// 512 bytes apart, and each writes 64 bytes (1.0 GB for 0.41 by the counters).  4097 x 1000 fp16 9.7 us.
+// 512 bytes apart (the counters: 1.0 GB stored for 0.41).  4097 x 1000 fp16 9.7 us.
 template <int T> static __global__ __launch_bounds__(1024) void k_mx4_write(Mx4Write W) {
     __shared__ double part[16][64];
     __shared__ int64_t slot_s[32];
